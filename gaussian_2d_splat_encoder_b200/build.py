@@ -9,6 +9,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -38,15 +39,17 @@ def build(verbose: bool = False, force: bool = False) -> Path:
         return OUT
     objdir = PKG / "_build"
     objdir.mkdir(exist_ok=True)
-    objs = []
-    for s in srcs:
-        o = objdir / (s.stem + ".o")
-        cmd = [nvcc(), *ARCH, *FLAGS, "-c", str(s), "-o", str(o)]
+    objs = [str(objdir / (s.stem + ".o")) for s in srcs]
+
+    def compile_one(s, o):
+        cmd = [nvcc(), *ARCH, *FLAGS, "-c", str(s), "-o", o]
         if verbose:
             cmd += ["-Xptxas", "-v"]
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
-        objs.append(str(o))
+
+    with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:  # one nvcc per source file
+        list(pool.map(compile_one, srcs, objs))
     tmp = OUT.with_suffix(".so.tmp")
     subprocess.run([nvcc(), *ARCH, "-shared", "-o", str(tmp), *objs], check=True)
     os.replace(tmp, OUT)

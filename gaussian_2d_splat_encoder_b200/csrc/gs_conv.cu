@@ -26,40 +26,13 @@
 #include <algorithm>
 
 #include "../../include/gsplat_b200.h"
+#include "gs_act.cuh"
 #include "gs_conv.cuh"
 #include "gs_tc.cuh"
 
 using namespace gs_tc;
 
 namespace {
-
-__device__ __forceinline__ float ex2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float rcp_approx(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// GELU(x) = 0.5 x (1 + erf(x / sqrt 2)) with erf from the rational approximation of Abramowitz &
-// Stegun, Handbook of Mathematical Functions, formula 7.1.26: for z >= 0,
-// erf(z) = 1 - t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) exp(-z^2), t = 1 / (1 + p z), |error| <= 1.5e-7.
-// 1 + erf(x / sqrt 2) is formed as 2 - q (x >= 0) or q (x < 0), q = t (...) exp(-z^2), so the negative
-// tail keeps its relative accuracy.  In fp32 the GELU error stays below 7e-7 absolute over [-12, 12],
-// far under the bf16 rounding of the stored activation.
-__device__ __forceinline__ float gelu_erf(float x) {
-    const float z = fabsf(x) * 0.70710678118654752f;
-    const float t = rcp_approx(fmaf(0.3275911f, z, 1.0f));
-    float q = fmaf(1.061405429f, t, -1.453152027f);
-    q = fmaf(q, t, 1.421413741f);
-    q = fmaf(q, t, -0.284496736f);
-    q = fmaf(q, t, 0.254829592f);
-    q *= t * ex2_approx(-(z * z) * 1.4426950408889634f);
-    return 0.5f * x * (x >= 0.f ? 2.0f - q : q);
-}
 
 // Persistent, warp-specialised convolution.  Work item = MT vertically stacked 128-pixel M-tiles x
 // one BN-wide slice of the output channels; CTAs stride over the items.
@@ -68,7 +41,7 @@ __device__ __forceinline__ float gelu_erf(float x) {
 //                 double-buffered in TMEM so the epilogue of item i overlaps the K loop of item i+1
 //   warps 2..     4*MT*CS epilogue warps: warp w drains TMEM lanes 32*(w%4).. of one accumulator, one of
 //                 CS column slices --
-//                 bias, GELU (gelu_erf), GroupNorm(8) partial sums, bf16 NHWC store
+//                 bias, GELU (gs_gelu), GroupNorm(8) partial sums, bf16 NHWC store
 // Every wait is bounded; a wait that gives up records its stage in *err and raises a CTA-wide abort
 // flag so the other roles stop issuing, then the CTA drains its copies and MMAs and frees TMEM.
 template <int BN, int KC, int STAGES, int MT, int CPG, int MINB, int CS, bool HALO>
@@ -384,7 +357,7 @@ __global__ void __launch_bounds__(64 + 128 * MT * CS, MINB)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     float x = v[i];
-                    if (a.gelu) x = gelu_erf(x);
+                    if (a.gelu) x = gs_gelu(x);
                     v[i] = x;
                     if (CPG == 8 && i >= 8) {
                         s1 += x;

@@ -1,0 +1,301 @@
+"""Layer operators with gradients on the library's kernels, for training what surrounds the frozen encoder.
+
+The encoder's forward fuses its own convolutions, GroupNorms and heads and is inference-only.  A stage, head
+or projection that is trained needs the same pieces one by one, differentiable, at sizes of its own:
+
+* ``group_norm_act``  GroupNorm with an activation before or after it, on channels-last maps (the encoder's
+  stages are Conv -> GELU -> GroupNorm, efficient_encoder.py:53-58)
+* ``linear_act``      ``act(x @ weight.T + bias) + residual``: 1x1 heads, projections of ``backbone_features``,
+  ``splat_features`` or ``gather_splat_latents`` and the layers of a residual block
+
+Both take fp32, bf16 or fp16 CUDA tensors, keep every sum and statistic in fp32, round once to the tensor's
+type and give the same bits for the same inputs.  They run on the current stream of the tensors' device
+and can be captured into a CUDA graph.  The gradients are once differentiable.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import functools
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ACTS = {"none": 0, "gelu": 1, "silu": 2}
+
+
+class _NormDesc(C.Structure):
+    """Mirror of gs_norm_desc."""
+
+    _fields_ = [("B", C.c_int32), ("C", C.c_int32), ("groups", C.c_int32), ("dtype", C.c_int32),
+                ("param_dtype", C.c_int32), ("act", C.c_int32), ("act_first", C.c_int32), ("eps", C.c_float),
+                ("rows", C.c_int64), ("x_row", C.c_int64), ("x_img", C.c_int64), ("dy_row", C.c_int64),
+                ("dy_img", C.c_int64)]
+
+
+class _LinearDesc(C.Structure):
+    """Mirror of gs_linear_desc."""
+
+    _fields_ = [("M", C.c_int64), ("N", C.c_int32), ("K", C.c_int32), ("dtype", C.c_int32), ("act", C.c_int32),
+                ("ldx", C.c_int64), ("ldw", C.c_int64), ("ldr", C.c_int64), ("ldy", C.c_int64)]
+
+
+def _act_code(act):
+    if act not in _ACTS:
+        raise ValueError(f"act must be one of {', '.join(_ACTS)}, got {act!r}")
+    return _ACTS[act]
+
+
+def _dtype_code(name, t):
+    if t.dtype not in _DTYPES:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    return _DTYPES[t.dtype]
+
+
+def _scope(dev):
+    """The tensors' device made current; the usual case, already current, costs nothing."""
+    return _NO_SCOPE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+class _NoScope:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NO_SCOPE = _NoScope()
+
+
+def _rows_of(t, first):
+    """Stride of the flattened axes first..-2 of `t` (whose last axis is adjacent), or None where they do
+    not form one axis."""
+    stride = size = None
+    for i in range(t.dim() - 2, first - 1, -1):
+        n = t.shape[i]
+        if n == 1:
+            continue
+        if stride is None:
+            stride, size = t.stride(i), n
+        elif t.stride(i) != stride * size:
+            return None
+        else:
+            size *= n
+    return t.shape[-1] if stride is None else stride
+
+
+# ------------------------------------------------------------------------------------ GroupNorm
+@functools.lru_cache(maxsize=1024)
+def _norm_plan(B, rows, channels, groups, dtype, param_dtype, act, act_first, eps, x_row, x_img, dy_row, dy_img):
+    """Descriptor of a call's sizes and the workspace of its forward and backward."""
+    d = _NormDesc(B, channels, groups, dtype, param_dtype, act, act_first, eps, rows, x_row, x_img, dy_row, dy_img)
+    L = _lib.load()
+    size = L.gs_group_norm_act_workspace_size
+    return C.byref(d), int(size(C.byref(d), 0)), int(size(C.byref(d), 1)), d
+
+
+def _image_layout(t):
+    """`t` [B, ..., C] with its row and image strides; a copy where the layout has no such strides."""
+    if t.is_contiguous():
+        C_ = t.shape[-1]
+        return t, C_, t.numel() // max(1, t.shape[0])
+    row = _rows_of(t, 1) if t.stride(-1) == 1 or t.shape[-1] == 1 else None
+    if row is None:
+        return _image_layout(t.contiguous())
+    return t, row, t.stride(0) if t.shape[0] > 1 else 0
+
+
+def _norm_forward(x, weight, bias, groups, eps, act, act_first, train):
+    x, x_row, x_img = _image_layout(x)
+    p = weight if weight is not None else bias
+    key = (x.shape[0], x.numel() // (x.shape[0] * x.shape[-1]), x.shape[-1], groups, _DTYPES[x.dtype],
+           0 if p is None else _DTYPES[p.dtype], act, act_first, eps, x_row, x_img)
+    desc, nbytes, _, _ = _norm_plan(*key, 0, 0)
+    if nbytes == 0:
+        raise ValueError(f"unsupported sizes: {tuple(x.shape)} in {groups} groups")
+    dev = x.device
+    with _scope(dev):
+        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float32, device=dev) if train else None
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ptr = _lib.ptr
+        _lib.check(_lib.load().gs_group_norm_act_fwd(desc, ptr(x), ptr(weight), ptr(bias), ptr(y), ptr(stats), ptr(ws),
+                                                     nbytes, _lib.stream_of(dev)), "gs_group_norm_act_fwd")
+    return y, x, stats, key
+
+
+class _GroupNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act, act_first):
+        y, x, stats, ctx.key = _norm_forward(x, weight, bias, groups, eps, act, act_first, True)
+        ctx.save_for_backward(x, weight, bias, stats)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dy, dy_row, dy_img = _image_layout(dy)
+        desc, _, nbytes, _ = _norm_plan(*ctx.key, dy_row, dy_img)
+        dev = x.device
+        with _scope(dev):
+            dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
+            dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if need[1] else None
+            db = torch.empty_like(bias, memory_format=torch.contiguous_format) if need[2] else None
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            ptr = _lib.ptr
+            _lib.check(_lib.load().gs_group_norm_act_bwd(desc, ptr(x), ptr(weight), ptr(bias), ptr(stats), ptr(dy),
+                                                         ptr(dx), ptr(dw), ptr(db), ptr(ws), nbytes,
+                                                         _lib.stream_of(dev)), "gs_group_norm_act_bwd")
+        return dx, dw, db, None, None, None, None
+
+
+def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None,
+                   bias: torch.Tensor | None = None, eps: float = 1e-5, *, act: str = "none",
+                   act_first: bool = False) -> torch.Tensor:
+    """GroupNorm of a channels-last map ``x`` [B, ..., C] with an activation, differentiable in x, weight and
+    bias.
+
+    Statistics are per image and group of C / num_groups adjacent channels over all axes between the first and
+    the last (biased variance, as nn.GroupNorm).  ``act`` ("none", "gelu" in the erf form, "silu") is applied
+    to the result, or with ``act_first`` to the input before it is normalised: the encoder's stages.
+    num_groups = C is an instance norm.  weight and bias [C] are float32 or of x's type, both alike, and
+    default to 1 and 0.  An NCHW tensor in channels_last memory format enters as ``x.permute(0, 2, 3, 1)``
+    without a copy; so do channel slices of a wider map and expanded tensors, while other strides are
+    copied.  Returns a contiguous tensor of x's shape and type.  C is at most 2048."""
+    dev = _lib.require_cuda(x, weight, bias)
+    code = _act_code(act)
+    _dtype_code("x", x)
+    if x.dim() < 2:
+        raise ValueError(f"x must be [B, ..., C], got {tuple(x.shape)}")
+    num_groups, channels = int(num_groups), x.shape[-1]
+    if num_groups < 1 or channels < 1 or channels % num_groups:
+        raise ValueError(f"{channels} channels do not divide into {num_groups} groups")
+    if channels > 2048:
+        raise ValueError(f"at most 2048 channels, got {channels}")
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is None:
+            continue
+        if p.shape != (channels,):
+            raise ValueError(f"{name} must be [{channels}], got {tuple(p.shape)}")
+        if p.dtype != x.dtype and p.dtype != torch.float32:
+            raise ValueError(f"{name} must be float32 or {x.dtype}, got {p.dtype}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError(f"weight and bias must be of one type, got {weight.dtype} and {bias.dtype}")
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    args = (x, weight, bias, num_groups, float(eps), code, int(bool(act_first)))
+    if x.numel() == 0:
+        # nothing to normalise; the graph stays connected, with zero gradients
+        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        return y + sum((p.sum() * 0).to(x.dtype) for p in (x, weight, bias) if p is not None)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _GroupNormAct.apply(*args)
+    return _norm_forward(*args, False)[0]
+
+
+# --------------------------------------------------------------------------------------- linear
+@functools.lru_cache(maxsize=1024)
+def _linear_plan(M, N, K, dtype, act, ldx, ldw, ldr, ldy):
+    d = _LinearDesc(M, N, K, dtype, act, ldx, ldw, ldr, ldy)
+    L = _lib.load()
+    size = L.gs_linear_act_workspace_size
+    return C.byref(d), int(size(C.byref(d), 0)), int(size(C.byref(d), 1)), d
+
+
+def _row_layout(t):
+    """`t` [..., n] with the stride of its flattened rows, at least n; a copy where there is none."""
+    n = t.shape[-1]
+    if t.is_contiguous():
+        return t, n
+    row = _rows_of(t, 0) if t.stride(-1) == 1 or n == 1 else None
+    return (t.contiguous(), n) if row is None or row < n else (t, row)
+
+
+def _linear_forward(x, weight, bias, residual, act, train):
+    x, ldx = _row_layout(x)
+    weight, ldw = _row_layout(weight)
+    ldr = 0
+    if residual is not None:
+        residual, ldr = _row_layout(residual)
+    N, K = weight.shape
+    key = (x.numel() // K, N, K, _DTYPES[x.dtype], act, ldx, ldw, ldr)
+    desc, nbytes, _, _ = _linear_plan(*key, N)
+    if nbytes == 0:
+        raise ValueError(f"unsupported sizes: {tuple(x.shape)} and {tuple(weight.shape)}")
+    dev = x.device
+    with _scope(dev):
+        shape = x.shape[:-1] + (N,)
+        y = torch.empty(shape, dtype=x.dtype, device=dev)
+        z = torch.empty(shape, dtype=x.dtype, device=dev) if train and act else None
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ptr = _lib.ptr
+        _lib.check(_lib.load().gs_linear_act_fwd(desc, ptr(x), ptr(weight), ptr(bias), ptr(residual), ptr(y), ptr(z),
+                                                 ptr(ws), nbytes, _lib.stream_of(dev)), "gs_linear_act_fwd")
+    return y, x, weight, z, key
+
+
+class _LinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        y, x, weight, z, ctx.key = _linear_forward(x, weight, bias, residual, act, True)
+        ctx.save_for_backward(x, weight, z)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, z = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx = dw = db = None
+        if need[0] or need[1] or need[2]:
+            g, ldy = _row_layout(dy)
+            desc, _, nbytes, _ = _linear_plan(*ctx.key, ldy)
+            dev = x.device
+            with _scope(dev):
+                dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
+                dw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if need[1] else None
+                db = torch.empty(weight.shape[0], dtype=x.dtype, device=dev) if need[2] else None
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+                ptr = _lib.ptr
+                _lib.check(_lib.load().gs_linear_act_bwd(desc, ptr(x), ptr(weight), ptr(z), ptr(g), ptr(dx), ptr(dw),
+                                                         ptr(db), ptr(ws), nbytes, _lib.stream_of(dev)),
+                           "gs_linear_act_bwd")
+        return dx, dw, db, dy if need[3] else None, None
+
+
+def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, act: str = "none",
+               residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``act(x @ weight.T + bias) + residual``, differentiable in all four tensors.
+
+    x [..., K], weight [N, K] (nn.Linear's, or a 1x1 convolution's ``weight.flatten(1)``), bias [N],
+    residual [..., N] of the output's shape; all of one type, float32, bfloat16 or float16.  ``act`` is
+    "none", "gelu" (erf form) or "silu".  Sums are fp32 (fp32 inputs keep fp32 accuracy); the result is
+    rounded once, after the residual.  Rows may be strided (channel slices of a wider map); other strides are
+    copied.  Returns a contiguous tensor [..., N]."""
+    _lib.require_cuda(x, weight, bias, residual)
+    code = _act_code(act)
+    _dtype_code("x", x)
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x must be [..., K] and weight [N, K], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    N, K = weight.shape
+    if not (1 <= N <= 1 << 20 and 1 <= K <= 1 << 20):
+        raise ValueError(f"weight sides must be 1..2^20, got {tuple(weight.shape)}")
+    if bias is not None and bias.shape != (N,):
+        raise ValueError(f"bias must be [{N}], got {tuple(bias.shape)}")
+    if residual is not None and residual.shape != x.shape[:-1] + (N,):
+        raise ValueError(f"residual must be {tuple(x.shape[:-1] + (N,))}, got {tuple(residual.shape)}")
+    for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):
+        if t is not None and t.dtype != x.dtype:
+            raise ValueError(f"{name} must be {x.dtype} like x, got {t.dtype}")
+    bias = None if bias is None else bias.contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        return _LinearAct.apply(x, weight, bias, residual, code)
+    return _linear_forward(x, weight, bias, residual, code, False)[0]

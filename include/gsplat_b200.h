@@ -238,6 +238,67 @@ int gs_l2_loss_grad(const float *out, const float *target, int64_t planes, int32
 /* activate_scale (params.py:18-28): out = softplus(log_scale) + 1e-4, n elements. */
 int gs_activate_scale(const float *log_scale, float *out, int64_t n, void *stream);
 
+/* ---- layer operators with gradients (no counterpart in the reference, which trains through torch) ----
+ * Element types and activations; 0-valued members are the defaults. */
+typedef enum { GS_F32 = 0, GS_BF16 = 1, GS_F16 = 2 } gs_dtype;
+typedef enum {
+    GS_ACT_NONE = 0,
+    GS_ACT_GELU = 1, /* x Phi(x), the erf form */
+    GS_ACT_SILU = 2  /* x / (1 + exp(-x)) */
+} gs_activation;
+
+/* GroupNorm with an activation on channels-last maps: x [B][rows][C] with free image and row strides (in
+ * elements; channels adjacent), C / groups channels per group, statistics per (image, group) in fp32.
+ * act_first 0: y = act(w xh + b); act_first 1: xh is normalised act(x), y = w xh + b (the order of the
+ * encoder's stages, efficient_encoder.py:53-58).  The stages of gs_encoder_fwd keep their own fused form;
+ * this one stands alone, for any group count, and has a backward.  C <= GS_NORM_MAX_C. */
+#define GS_NORM_MAX_C 2048
+typedef struct {
+    int32_t B, C, groups;
+    int32_t dtype;       /* gs_dtype of x, y, dy, dx */
+    int32_t param_dtype; /* gs_dtype of weight, bias and their gradients: GS_F32 or dtype */
+    int32_t act, act_first;
+    float eps;
+    int64_t rows;          /* pixels of an image */
+    int64_t x_row, x_img;  /* strides of x */
+    int64_t dy_row, dy_img; /* strides of dy (backward) */
+} gs_norm_desc;
+
+/* Workspace bytes of a forward (backward = 0) or a backward (1) call; 0 for an invalid descriptor.  The
+ * two calls share nothing through it. */
+size_t gs_group_norm_act_workspace_size(const gs_norm_desc *d, int backward);
+/* y [B][rows][C], tightly packed; stats (may be NULL without a backward) receives fp32 [B][groups][2]:
+ * mean and 1 / sqrt(var + eps).  weight and bias [C] may be NULL (1 and 0). */
+int gs_group_norm_act_fwd(const gs_norm_desc *d, const void *x, const void *weight, const void *bias, void *y,
+                          float *stats, void *workspace, size_t workspace_bytes, void *stream);
+/* Gradients for upstream dy: dx [B][rows][C] tightly packed, dweight and dbias [C]; each may be NULL.
+ * Sums run in a fixed order: the same inputs give the same bits. */
+int gs_group_norm_act_bwd(const gs_norm_desc *d, const void *x, const void *weight, const void *bias,
+                          const float *stats, const void *dy, void *dx, void *dweight, void *dbias, void *workspace,
+                          size_t workspace_bytes, void *stream);
+
+/* Linear layer y = act(x W^T + bias) + residual: x [M][K], W [N][K], residual, y, z [M][N], bias [N], all of
+ * one element type, sums in fp32; x, W, residual and dy have free row strides (in elements, at least the
+ * row's length), outputs are tightly packed.  N, K <= GS_LINEAR_MAX_DIM. */
+#define GS_LINEAR_MAX_DIM (1 << 20)
+typedef struct {
+    int64_t M;
+    int32_t N, K;
+    int32_t dtype, act;
+    int64_t ldx, ldw, ldr; /* row strides of x, W and the residual */
+    int64_t ldy;           /* row stride of dy (backward) */
+} gs_linear_desc;
+
+/* Workspace bytes of a forward (backward = 0) or a backward (1) call; 0 for an invalid descriptor. */
+size_t gs_linear_act_workspace_size(const gs_linear_desc *d, int backward);
+/* bias, residual and z may be NULL; z receives x W^T + bias for the backward of an activation. */
+int gs_linear_act_fwd(const gs_linear_desc *d, const void *x, const void *w, const void *bias, const void *residual,
+                      void *y, void *z, void *workspace, size_t workspace_bytes, void *stream);
+/* Gradients for upstream dy: dx [M][K], dw [N][K], dbias [N]; each may be NULL (not computed).  z is the
+ * forward's, not read without an activation.  The residual's gradient is dy itself. */
+int gs_linear_act_bwd(const gs_linear_desc *d, const void *x, const void *w, const void *z, const void *dy, void *dx,
+                      void *dw, void *dbias, void *workspace, size_t workspace_bytes, void *stream);
+
 /* Text of the last CUDA error seen by the calling thread (empty when none). */
 const char *gs_last_error(void);
 
