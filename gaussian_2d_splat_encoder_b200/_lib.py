@@ -67,6 +67,7 @@ SIGNATURES = {
     "gs_linear_act_workspace_size": (C.c_size_t, [_P, C.c_int]),
     "gs_linear_act_fwd": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
     "gs_linear_act_bwd": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
+    "gs_linear_error_flag": (C.c_int, [_P]),
     "gs_last_error": (C.c_char_p, []),
     "gs_kernel_launches": (C.c_uint64, []),
     "gs_profile_enable": (None, [C.c_int]),

@@ -35,7 +35,7 @@ __device__ __forceinline__ float gs_gelu_slope(float x) {
     const float q = gs_erfc_as(x, e);
     return fmaf(x * 0.39894228040143268f, e, 0.5f * (x >= 0.f ? 2.0f - q : q));
 }
-// SiLU(x) = x s, s = 1 / (1 + exp(-x)); slope s (1 + x (1 - s))
+// SiLU(x) = x s, s = 1 / (1 + exp(-x)); slope s + x s (1 - s)
 __device__ __forceinline__ float gs_sigmoid(float x) { return gs_rcp(1.0f + gs_ex2(-1.4426950408889634f * x)); }
 
 enum { ACT_NONE = 0, ACT_GELU = 1, ACT_SILU = 2 };  // gs_activation
@@ -51,9 +51,26 @@ __device__ __forceinline__ float gs_act_slope(float x) {
     if (ACT == ACT_GELU) return gs_gelu_slope(x);
     if (ACT == ACT_SILU) {
         const float s = gs_sigmoid(x);
-        return s * fmaf(x, 1.0f - s, 1.0f);
+        return fmaf(x * s, 1.0f - s, s);
     }
     return 1.0f;
+}
+// activation and slope together; the activation has gs_act's bits
+template <int ACT>
+__device__ __forceinline__ float gs_act_both(float x, float &slope) {
+    if (ACT == ACT_GELU) {
+        float e;
+        const float q = gs_erfc_as(x, e), c = x >= 0.f ? 2.0f - q : q;
+        slope = fmaf(x * 0.39894228040143268f, e, 0.5f * c);
+        return 0.5f * x * c;
+    }
+    if (ACT == ACT_SILU) {
+        const float s = gs_sigmoid(x), y = x * s;
+        slope = fmaf(y, 1.0f - s, s);
+        return y;
+    }
+    slope = 1.0f;
+    return x;
 }
 
 // ---- element types: fp32, bf16, fp16 (gs_dtype); a vector is 16 bytes

@@ -1,9 +1,24 @@
 // gs_linear.cu -- linear layer with bias, activation and residual, forward and backward (sm_100a).
 //
-//   z = x W^T + b,  y = act(z) + residual        x [M][K], W [N][K], y and z [M][N]
+//   z = x W^T + b,  y = act(z) + residual        x [M][K], W [N][K], y [M][N]
 //   dz = dy act'(z),  dx = dz W,  dW = dz^T x,  db = sum over rows of dz,  dresidual = dy
 //
-// First form: one tiled fp32 product with free strides serves the three matrix products.
+// All three products run in one kernel, D[i][j] = sum_k A(i, k) B(j, k) on tcgen05.mma (kind::f16, fp32
+// accumulators in TMEM); an operand is read as it lies in memory, with k adjacent (K-major: x and W of the
+// forward, dz of dx) or with i / j adjacent (MN-major: W of dx, dz and x of dW), so nothing is transposed.
+// fp32 operands enter as three bf16 terms (x = h + m + l, exact to 2^-24 of x) and a product as the six of
+// the nine term products that reach 2^-24: the same kernel runs over six times the k-blocks.
+//
+// The forward keeps, for the backward, the activation's slope instead of z: the epilogue has its parts at
+// hand, the backward needs no activation, and in 16-bit types it is a 16-bit fixed-point number in
+// [-1/6, 7/6] (GELU's and SiLU's slopes lie in [-0.13, 1.13]) with steps of 1/49152: an error of 1e-5 where a
+// bf16 z would cost 4e-3 |z|.  dz is rounded to the operand type once, as the products need it; db sums the
+// unrounded values.
+//
+// Sums over a long k with few output tiles are split along k over the SMs; the parts go to the workspace
+// in fp32 and a second kernel adds them in order (the same bits every time) and applies the epilogue.
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include <stdio.h>
@@ -14,173 +29,908 @@
 #include "../../include/gsplat_b200.h"
 #include "gs_act.cuh"
 #include "gs_prof.cuh"
+#include "gs_tc.cuh"
 
 void gs_set_last_error(const char *msg);
 
+using namespace gs_tc;
+
 namespace {
+
+constexpr int SMS = 148;  // of a B200: tiles, splits and the workspace are a matter of sizes alone
+constexpr int BM = 128, BK = 64;
+
+__device__ int g_wait_error;  // code of a bounded wait that gave up (gs_linear_error_flag), 0 if none did
+
+// ---- the kept slope: fp32, or 16-bit fixed point (0 and 1 exact, 65535 is NaN)
+__device__ __forceinline__ uint32_t slope_code(float s) {
+    return s == s ? __float2uint_rn(fmaf(s, 49152.f, 8192.f)) : 65535u;
+}
+__device__ __forceinline__ float slope_of(uint32_t c) {
+    return c == 65535u ? __int_as_float(0x7fffffff) : ((float)c - 8192.f) * (1.f / 49152.f);
+}
 
 __device__ __forceinline__ float act_rt(float z, int act) {
     return act == ACT_GELU ? gs_act<ACT_GELU>(z) : act == ACT_SILU ? gs_act<ACT_SILU>(z) : z;
 }
-__device__ __forceinline__ float slope_rt(float z, int act) {
-    return act == ACT_GELU ? gs_act_slope<ACT_GELU>(z) : act == ACT_SILU ? gs_act_slope<ACT_SILU>(z) : 1.f;
+__device__ __forceinline__ float act_both_rt(float z, int act, float &slope) {
+    return act == ACT_GELU   ? gs_act_both<ACT_GELU>(z, slope)
+           : act == ACT_SILU ? gs_act_both<ACT_SILU>(z, slope)
+                             : gs_act_both<ACT_NONE>(z, slope);
 }
 
-// out[i][j] = act(sum_k A[i ai + k ak] B[j bj + k bk] + bias[j]) + residual[i][j]; z before the activation.
-// 64 x 64 outputs per block, 4 x 4 per thread; long sums fold every 1024 terms.
-template <typename T>
-__global__ void __launch_bounds__(256) k_product(const T *A, long long ai, long long ak, const T *B, long long bj,
-                                                 long long bk, long long I, int J, long long K, const T *bias,
-                                                 const T *residual, long long ldr, int act, T *out, T *z) {
-    __shared__ float sa[16][65], sb[16][65];
-    const long long i0 = (long long)blockIdx.x * 64;
-    const int j0 = blockIdx.y * 64, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    float acc[4][4] = {}, tot[4][4] = {};
-    for (long long k0 = 0; k0 < K; k0 += 16) {
-        for (int e = threadIdx.x; e < 1024; e += 256) {
-            // neighbouring threads walk the adjacent axis
-            const int ka = ak == 1 ? e & 15 : e >> 6, ia = ak == 1 ? e >> 4 : e & 63;
-            sa[ka][ia] = i0 + ia < I && k0 + ka < K ? to_f32(A[(i0 + ia) * ai + (k0 + ka) * ak]) : 0.f;
-            const int kb = bk == 1 ? e & 15 : e >> 6, jb = bk == 1 ? e >> 4 : e & 63;
-            sb[kb][jb] = j0 + jb < J && k0 + kb < K ? to_f32(B[(j0 + jb) * bj + (k0 + kb) * bk]) : 0.f;
+struct GemmArgs {
+    long long I;          // rows of D
+    int J;                // columns of D
+    int kb, npair;        // k-blocks of 64 per term product, term products (1, or 6 for fp32)
+    int a_mn, b_mn;       // operand has i / j adjacent instead of k
+    int f16;              // operands fp16 (else bf16)
+    int splits;           // > 1: parts of the k sum, raw fp32 to part
+    int tiles_i, tiles_j;
+    // epilogue
+    int out_f16;          // 16-bit output type
+    int act;
+    int out_tma, res_tma; // whole 16-byte rows: TMA boxes, else element by element
+    const void *bias, *residual;
+    void *out, *slope;
+    long long ldr;
+};
+
+// term products of fp32 operands, small ones first: (a term, b term), 0 = high
+__constant__ const unsigned char PAIR_A[6] = {2, 0, 1, 1, 0, 0}, PAIR_B[6] = {0, 2, 1, 0, 1, 0};
+
+// Persistent and warp-specialised.  Work item = a 128 x BN tile of D times a k split; CTAs stride over
+// the items, neighbouring CTAs on neighbouring columns of the same rows (A from L2).
+//   warp 0   TMA producer: A and B k-blocks into a STAGES-deep ring of 128-byte-swizzled tiles
+//   warp 1   TMEM owner, MMA issuer; accumulators double-buffered, so the epilogue runs under the next item
+//   warps 2..9  epilogue: quarter warp % 4 of the rows; BN >= 128: half of the columns each, BN = 64: every
+//            second item.  A unit is 32 rows x 128 bytes of the output, staged in shared memory in the
+//            128-byte swizzle (a thread writes its row without bank conflicts) and moved by TMA; the residual
+//            comes by TMA into the same place and is added in registers before the only rounding.
+// Every wait is bounded; one that gives up records a code in g_wait_error and raises the CTA's abort flag.
+template <int BN, bool OUT32>
+struct Shape {
+    static constexpr uint32_t A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE = A_BYTES + B_BYTES;
+    static constexpr int STAGES = BN == 256 ? 3 : BN == 128 ? 5 : 6;
+    static constexpr int CS = BN >= 128 ? 2 : 1;  // warps sharing a row quarter's columns
+    static constexpr int EC = OUT32 ? 32 : 64;    // columns of a unit
+    static constexpr int UNITS = BN / CS / EC;
+    static constexpr uint32_t EPI = 8 * 2 * 4096;  // two units per epilogue warp
+    static constexpr size_t SMEM = 1024 + STAGES * STAGE + EPI;
+};
+
+template <int BN, bool OUT32>
+__global__ void __launch_bounds__(320, 1)
+    k_gemm(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+           const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmS,
+           const __grid_constant__ CUtensorMap tmR, const GemmArgs a) {
+    using S = Shape<BN, OUT32>;
+    constexpr int STAGES = S::STAGES, EC = S::EC;
+    extern __shared__ uint8_t dsmem[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~(uintptr_t)1023);
+    __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], tfull[2], tempty[2], mdone, rbar[8][2];
+    __shared__ uint32_t tmem_base;
+    __shared__ volatile int abort_flag;
+    __shared__ int issued, consumed;
+    __shared__ __align__(16) float sbias[8][32];
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int kbt = a.kb * a.npair;
+    const int n_items = a.tiles_i * a.tiles_j * a.splits;
+
+    if (warp == 1) {
+        tmem_alloc(&tmem_base, 2 * BN);
+        tmem_relinquish();
+    }
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
         }
-        __syncthreads();
+        for (int j = 0; j < 2; j++) {
+            mbar_init(&tfull[j], 1);
+            mbar_init(&tempty[j], 4 * S::CS);
+        }
+        for (int w = 0; w < 8; w++)
+            for (int j = 0; j < 2; j++) mbar_init(&rbar[w][j], 1);
+        mbar_init(&mdone, 1);
+        abort_flag = 0;
+        issued = 0;
+        consumed = 0;
+        fence_barrier_init();
+        prefetch_tensormap(&tmA);
+        prefetch_tensormap(&tmB);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tbase = tmem_base;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            for (int item = blockIdx.x; item < n_items && !abort_flag; item += gridDim.x) {
+                int t = item;
+                const int j0 = t % a.tiles_j * BN;
+                t /= a.tiles_j;
+                const int i0 = t % a.tiles_i * BM;
+                const int s = t / a.tiles_i;
+                const int k1 = (int)((long long)kbt * (s + 1) / a.splits);
+                for (int k = (int)((long long)kbt * s / a.splits); k < k1; k++, it++) {
+                    const int st = it % STAGES;
+                    if (it >= STAGES && !mbar_wait_or_abort(&empty[st], ((it / STAGES) - 1) & 1, &abort_flag,
+                                                            &g_wait_error, 1))
+                        break;
+                    if (abort_flag) break;
+                    mbar_arrive_expect_tx(&full[st], S::STAGE);
+                    uint8_t *sa = smem + st * S::STAGE, *sb = sa + S::A_BYTES;
+                    const int p = k / a.kb, kk = (k - p * a.kb) * BK;
+                    const int ta = a.npair > 1 ? PAIR_A[p] : 0, tb = a.npair > 1 ? PAIR_B[p] : 0;
+                    if (a.a_mn) {
 #pragma unroll
-        for (int k = 0; k < 16; k++)
+                        for (int c = 0; c < BM / 64; c++)
+                            tma_load_3d(sa + c * 64 * 128, &tmA, &full[st], i0 + 64 * c, kk, ta);
+                    } else {
+                        tma_load_3d(sa, &tmA, &full[st], kk, i0, ta);
+                    }
+                    if (a.b_mn) {
+#pragma unroll
+                        for (int c = 0; c < BN / 64; c++)
+                            tma_load_3d(sb + c * 64 * 128, &tmB, &full[st], j0 + 64 * c, kk, tb);
+                    } else {
+                        tma_load_3d(sb, &tmB, &full[st], kk, j0, tb);
+                    }
+                    issued = it + 1;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t fmt = a.f16 ? 0u : 1u;
+            const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)a.a_mn << 15) |
+                                   ((uint32_t)a.b_mn << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+            // per 16 of k: 32 bytes inside the swizzled row (K-major), two 8-row groups (MN-major)
+            const uint32_t stepA = a.a_mn ? 2048u : 32u, stepB = a.b_mn ? 2048u : 32u;
+            int it = 0, tc = 0;
+            for (int item = blockIdx.x; item < n_items && !abort_flag; item += gridDim.x, tc++) {
+                const int s = item / (a.tiles_j * a.tiles_i);
+                const int k0 = (int)((long long)kbt * s / a.splits), k1 = (int)((long long)kbt * (s + 1) / a.splits);
+                const int buf = tc & 1;
+                if (tc >= 2 && !mbar_wait_or_abort(&tempty[buf], ((tc >> 1) - 1) & 1, &abort_flag, &g_wait_error, 2))
+                    break;
+                tc_fence_after();
+                const uint32_t dcol = tbase + (uint32_t)buf * BN;
+                bool ok = true;
+                for (int k = k0; k < k1; k++, it++) {
+                    const int st = it % STAGES;
+                    if (!mbar_wait_or_abort(&full[st], (it / STAGES) & 1, &abort_flag, &g_wait_error, 3)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t sa = smem_u32(smem + st * S::STAGE), sb = sa + S::A_BYTES;
+#pragma unroll
+                    for (int q = 0; q < BK / 16; q++) {
+                        const uint64_t ad = a.a_mn ? sdesc_mn(sa + stepA * q, 8192, 1024) : sdesc(sa + stepA * q, 1024, 2);
+                        const uint64_t bd = a.b_mn ? sdesc_mn(sb + stepB * q, 8192, 1024) : sdesc(sb + stepB * q, 1024, 2);
+                        mma_bf16(dcol, ad, bd, idesc, (k > k0 || q) ? 1u : 0u);
+                    }
+                    mma_commit(&empty[st]);
+                    consumed = it + 1;
+                }
+                if (!ok) break;
+                mma_commit(&tfull[buf]);
+            }
+            // all MMAs of this CTA (also those of an aborted item) have finished once mdone flips
+            mma_commit(&mdone);
+            mbar_wait(&mdone, 0, &g_wait_error, 4);
+        }
+    } else {
+        const int e = warp - 2, q = warp & 3, half = e >> 2;
+        uint8_t *const slots = smem + STAGES * S::STAGE + e * 8192;
+        const bool has_res = a.residual != nullptr, has_slope = a.slope != nullptr;
+        int tc = 0, use = 0, rphase[2] = {0, 0};
+        for (int item = blockIdx.x; item < n_items; item += gridDim.x, tc++) {
+            const int buf = tc & 1;
+            if (S::CS == 1 && half != buf) continue;
+            int t = item;
+            const int jt = t % a.tiles_j * BN;
+            t /= a.tiles_j;
+            const long long row0 = (long long)(t % a.tiles_i) * BM + q * 32;
+            const int sp = t / a.tiles_i;
+            bool ready = false, dead = false;
+#pragma unroll
+            for (int u = 0; u < S::UNITS; u++) {
+                const int lc = (S::CS == 2 ? half * (BN / 2) : 0) + u * EC;  // column inside the tile
+                const int col0 = jt + lc;
+                const bool live = col0 < a.J && row0 < a.I;
+                // the slot: alternating, or with a slope always the first (the second is the slope's)
+                const int sl = has_slope ? 0 : use & 1;
+                uint8_t *const out = slots + sl * 4096, *const slo = slots + 4096;
+                if (live) {
+                    use++;
+                    if (lane == 0) {
+                        if (has_slope) bulk_wait_read<0>();
+                        else bulk_wait_read<1>();
+                    }
+                    __syncwarp();
+                    if (has_res && a.res_tma) {
+                        if (lane == 0) {
+                            mbar_arrive_expect_tx(&rbar[e][sl], 4096);
+                            tma_load_3d(out, &tmR, &rbar[e][sl], col0, (int)row0, 0);
+                        }
+                    } else if (has_res) {
+                        for (int r = 0; r < 32 && row0 + r < a.I; r++)
+#pragma unroll
+                            for (int c = lane; c < EC; c += 32)
+                                if (col0 + c < a.J) {
+                                    const long long at = (row0 + r) * a.ldr + col0 + c;
+                                    const int b = c * (128 / EC);
+                                    uint8_t *d = out + r * 128 + ((b & ~15) ^ ((r & 7) << 4)) + (b & 15);
+                                    if (OUT32) *reinterpret_cast<float *>(d) = reinterpret_cast<const float *>(a.residual)[at];
+                                    else *reinterpret_cast<uint16_t *>(d) = reinterpret_cast<const uint16_t *>(a.residual)[at];
+                                }
+                        __syncwarp();
+                    }
+                }
+                float bias[EC / 32];
+#pragma unroll
+                for (int h = 0; h < EC / 32; h++) {
+                    const int c = col0 + 32 * h + lane;
+                    bias[h] = 0.f;
+                    if (a.bias && c < a.J)
+                        bias[h] = OUT32       ? reinterpret_cast<const float *>(a.bias)[c]
+                                  : a.out_f16 ? to_f32(reinterpret_cast<const __half *>(a.bias)[c])
+                                              : to_f32(reinterpret_cast<const __nv_bfloat16 *>(a.bias)[c]);
+                }
+                if (!ready) {
+                    if (!mbar_wait_or_abort(&tfull[buf], (tc >> 1) & 1, &abort_flag, &g_wait_error, 5)) dead = true;
+                    tc_fence_after();
+                    ready = true;
+                }
+                if (live && has_res && a.res_tma) {
+                    // (after an abort too: the copy lands in this CTA's shared memory)
+                    if (!mbar_wait(&rbar[e][sl], rphase[sl] & 1, &g_wait_error, 6)) {
+                        abort_flag = 1;
+                        dead = true;
+                    }
+                    rphase[sl]++;
+                }
+#pragma unroll
+                for (int h = 0; h < EC / 32; h++) {
+                    uint32_t r[32];
+                    __syncwarp();
+                    sbias[e][lane] = bias[h];
+                    __syncwarp();
+                    if (live && !dead) {
+                        tmem_ld32(tbase + ((uint32_t)(q * 32) << 16) + (uint32_t)buf * BN + (uint32_t)(lc + 32 * h), r);
+                        tmem_wait_ld();
+                    }
+                    if (u == S::UNITS - 1 && h == EC / 32 - 1) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&tempty[buf]);
+                    }
+                    if (!live || dead) continue;
+                    // 16 bytes of output at a time: 8 columns (16 bit) or 4 (fp32)
+                    constexpr int W = OUT32 ? 4 : 8;
+#pragma unroll
+                    for (int g = 0; g < 32 / W; g++) {
+                        float v[W], sv[W];
+                        const uint32_t at = (uint32_t)lane * 128u + ((uint32_t)(((OUT32 ? 0 : 4 * h) + g) ^ (lane & 7)) << 4);
+#pragma unroll
+                        for (int i = 0; i < W; i++) v[i] = __uint_as_float(r[g * W + i]) + sbias[e][g * W + i];
+                        if (has_slope) {
+#pragma unroll
+                            for (int i = 0; i < W; i++) v[i] = act_both_rt(v[i], a.act, sv[i]);
+                            uint4 p;
+                            if (OUT32) {
+                                p = pack16<float>(sv);
+                            } else {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int i = 0; i < 4; i++)
+                                    w[i] = slope_code(sv[(2 * i) % W]) | slope_code(sv[(2 * i + 1) % W]) << 16;
+                                p = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                            *reinterpret_cast<uint4 *>(slo + at) = p;
+                        } else if (a.act) {
+#pragma unroll
+                            for (int i = 0; i < W; i++) v[i] = act_rt(v[i], a.act);
+                        }
+                        if (has_res) {
+                            const uint4 p = *reinterpret_cast<const uint4 *>(out + at);
+                            float f[8];
+                            if (OUT32) unpack16<float>(p, f);
+                            else if (a.out_f16) unpack16<__half>(p, f);
+                            else unpack16<__nv_bfloat16>(p, f);
+#pragma unroll
+                            for (int i = 0; i < W; i++) v[i] = __fadd_rn(v[i], f[i]);
+                        }
+                        *reinterpret_cast<uint4 *>(out + at) = OUT32       ? pack16<float>(v)
+                                                               : a.out_f16 ? pack16<__half>(v)
+                                                                           : pack16<__nv_bfloat16>(v);
+                    }
+                }
+                if (!live || dead) continue;
+                if (a.out_tma) {
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_3d(&tmO, out, col0, (int)row0, sp);
+                        if (has_slope) tma_store_3d(&tmS, slo, col0, (int)row0, 0);
+                        bulk_commit();
+                    }
+                } else {
+                    __syncwarp();
+                    constexpr int ES = 128 / EC;  // bytes of an element
+                    for (int r = 0; r < 32 && row0 + r < a.I; r++)
+#pragma unroll
+                        for (int c = lane; c < EC; c += 32)
+                            if (col0 + c < a.J) {
+                                const long long at = (row0 + r) * a.J + col0 + c;
+                                const int b = c * ES, off = r * 128 + ((b & ~15) ^ ((r & 7) << 4)) + (b & 15);
+                                if (OUT32) {
+                                    reinterpret_cast<float *>(a.out)[at] = *reinterpret_cast<const float *>(out + off);
+                                    if (has_slope)
+                                        reinterpret_cast<float *>(a.slope)[at] = *reinterpret_cast<const float *>(slo + off);
+                                } else {
+                                    reinterpret_cast<uint16_t *>(a.out)[at] = *reinterpret_cast<const uint16_t *>(out + off);
+                                    if (has_slope)
+                                        reinterpret_cast<uint16_t *>(a.slope)[at] = *reinterpret_cast<const uint16_t *>(slo + off);
+                                }
+                            }
+                    fence_proxy_async();  // the next residual's copy overwrites what was just read
+                    __syncwarp();
+                }
+            }
+            if (dead) break;
+        }
+        if (lane == 0) bulk_wait<0>();
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (abort_flag && threadIdx.x == 0)
+        // copies that were issued but never consumed still land in shared memory: wait for them
+        for (int j = consumed; j < issued; j++) mbar_wait(&full[j % STAGES], (j / STAGES) & 1, &g_wait_error, 7);
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tbase, 2 * BN);
+}
+
+// ---- operands that TMA cannot read in place (rows not on 16 bytes, fp32): rows padded to a multiple of eight
+// elements, fp32 as three bf16 terms
+struct PrepJob {
+    const void *src;
+    void *dst;
+    long long rows, ld;  // source row stride
+    int cols, ldp;       // destination row stride
+};
+__device__ __forceinline__ void split3(float x, float &h, float &m, float &l) {
+    h = __bfloat162float(__float2bfloat16_rn(x));
+    // an infinite or NaN head has no remainder
+    const float r = fabsf(h) <= 3.4028234e38f ? x - h : 0.f;
+    m = __bfloat162float(__float2bfloat16_rn(r));
+    l = r - m;
+}
+__device__ __forceinline__ void store_terms(float *v, __nv_bfloat16 *dst, long long term_stride) {
+    float h[8], m[8], l[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) split3(v[i], h[i], m[i], l[i]);
+    *reinterpret_cast<uint4 *>(dst) = pack16<__nv_bfloat16>(h);
+    *reinterpret_cast<uint4 *>(dst + term_stride) = pack16<__nv_bfloat16>(m);
+    *reinterpret_cast<uint4 *>(dst + 2 * term_stride) = pack16<__nv_bfloat16>(l);
+}
+template <typename T>
+__global__ void __launch_bounds__(256) k_prep_operand(PrepJob a, PrepJob b) {
+    const PrepJob &j = blockIdx.y ? b : a;
+    const int nv = j.ldp / 8;
+    const long long n = j.rows * nv;
+    for (long long t = blockIdx.x * 256LL + threadIdx.x; t < n; t += gridDim.x * 256LL) {
+        const long long r = t / nv;
+        const int c = (int)(t - r * nv) * 8;
+        const T *p = reinterpret_cast<const T *>(j.src) + r * j.ld + c;
+        if (sizeof(T) == 4) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = c + i < j.cols ? to_f32(p[i]) : 0.f;
+            store_terms(v, reinterpret_cast<__nv_bfloat16 *>(j.dst) + r * j.ldp + c, j.rows * j.ldp);
+        } else {
+            uint32_t w[4];
+            const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
 #pragma unroll
             for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] = fmaf(sa[k][ty * 4 + i], sb[k][tx * 4 + j], acc[i][j]);
-        __syncthreads();
-        if ((k0 & 1023) == 1008 || k0 + 16 >= K)
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                (&tot[0][0])[i] += (&acc[0][0])[i];
-                (&acc[0][0])[i] = 0.f;
-            }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const long long r = i0 + ty * 4 + i;
-            const int c = j0 + tx * 4 + j;
-            if (r >= I || c >= J) continue;
-            float v = tot[i][j] + (bias ? to_f32(bias[c]) : 0.f);
-            if (z) from_f32(v, z[r * J + c]);
-            // (an explicit addition: no fusing with the activation in one of the branches and not in another)
-            v = act_rt(v, act);
-            if (residual) v = __fadd_rn(v, to_f32(residual[r * ldr + c]));
-            from_f32(v, out[r * J + c]);
+                w[i] = (c + 2 * i < j.cols ? h[2 * i] : 0u) | (c + 2 * i + 1 < j.cols ? (uint32_t)h[2 * i + 1] << 16 : 0u);
+            *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(j.dst) + r * j.ldp + c) = make_uint4(w[0], w[1], w[2], w[3]);
         }
+    }
 }
 
+// ---- dz = dy slope as an operand (dz NULL: not written, dy serves), and its column sums per block of rows
+struct DzArgs {
+    const void *dy, *slope;
+    void *dz;
+    float *colsum;  // [blocks][N], or NULL
+    long long M, ldy;
+    int N, ldp, cvec, rl;  // vectors of eight columns per block, row lanes
+    int vec;               // dy and slope rows lie on 16 bytes
+};
 template <typename T>
-__global__ void __launch_bounds__(256) k_dz(const T *dy, long long ldy, const T *z, T *dz, long long M, int N, int act) {
-    const long long n = M * N;
-    for (long long k = blockIdx.x * 256LL + threadIdx.x; k < n; k += gridDim.x * 256LL) {
-        const long long r = k / N;
-        const int c = (int)(k - r * N);
-        from_f32(to_f32(dy[r * ldy + c]) * (z ? slope_rt(to_f32(z[k]), act) : 1.f), dz[k]);
+__global__ void __launch_bounds__(256) k_dz(DzArgs a) {
+    __shared__ float buf[256 * 8];
+    const int r = threadIdx.x / a.cvec, cv = threadIdx.x - r * a.cvec;
+    const int c = (blockIdx.y * a.cvec + cv) * 8;
+    const bool live = r < a.rl && c < a.ldp;
+    const long long lo = a.M * blockIdx.x / gridDim.x, hi = a.M * (blockIdx.x + 1LL) / gridDim.x;
+    float s[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) s[i] = 0.f;
+    if (live)
+#pragma unroll 2
+        for (long long m = lo + r; m < hi; m += a.rl) {
+            const T *p = reinterpret_cast<const T *>(a.dy) + m * a.ldy + c;
+            float v[8];
+            if (a.vec) {
+                if (sizeof(T) == 4) {
+                    unpack16<float>(reinterpret_cast<const uint4 *>(p)[0], v);
+                    unpack16<float>(reinterpret_cast<const uint4 *>(p)[1], v + 4);
+                } else {
+                    unpack16<T>(*reinterpret_cast<const uint4 *>(p), v);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = c + i < a.N ? to_f32(p[i]) : 0.f;
+            }
+            if (a.slope) {  // (products of their own rounding: db's bits do not depend on dz being written)
+                if (sizeof(T) == 4) {
+                    const float *q = reinterpret_cast<const float *>(a.slope) + m * a.N + c;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[i] = __fmul_rn(v[i], a.vec || c + i < a.N ? q[i] : 0.f);
+                } else {
+                    const uint16_t *q = reinterpret_cast<const uint16_t *>(a.slope) + m * a.N + c;
+                    if (a.vec) {
+                        const uint4 w = *reinterpret_cast<const uint4 *>(q);
+                        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            v[i] = __fmul_rn(v[i], slope_of(i & 1 ? x[i >> 1] >> 16 : x[i >> 1] & 0xffffu));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) v[i] = c + i < a.N ? __fmul_rn(v[i], slope_of(q[i])) : 0.f;
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) s[i] += v[i];
+            if (a.dz) {
+                if (sizeof(T) == 4)
+                    store_terms(v, reinterpret_cast<__nv_bfloat16 *>(a.dz) + m * a.ldp + c, a.M * a.ldp);
+                else
+                    *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.dz) + m * a.ldp + c) = pack16<T>(v);
+            }
+        }
+    if (!a.colsum) return;
+    const int w = a.cvec * 8;
+    if (r < a.rl)
+#pragma unroll
+        for (int i = 0; i < 8; i++) buf[r * w + cv * 8 + i] = s[i];
+    for (int n = a.rl; n > 1;) {
+        const int h = (n + 1) >> 1;
+        __syncthreads();
+        if (r < n - h)
+#pragma unroll
+            for (int i = 0; i < 8; i++) buf[r * w + cv * 8 + i] += buf[(r + h) * w + cv * 8 + i];
+        n = h;
     }
-}
-// column sums: 32 columns per block, 32 row lanes
-template <typename T>
-__global__ void __launch_bounds__(1024) k_colsum(const T *dz, T *db, long long M, int N) {
-    __shared__ float s[32][33];
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = blockIdx.x * 32 + tx;
-    float t = 0.f;
-    if (c < N)
-        for (long long r = ty; r < M; r += 32) t += to_f32(dz[r * N + c]);
-    s[ty][tx] = t;
     __syncthreads();
-    if (ty == 0 && c < N) {
-        for (int k = 1; k < 32; k++) t += s[k][tx];
-        from_f32(t, db[c]);
+    for (int k = threadIdx.x; k < w; k += 256) {
+        const int cc = blockIdx.y * w + k;
+        if (cc < a.N) a.colsum[(long long)blockIdx.x * a.N + cc] = buf[k];
     }
 }
+
+// ---- adds the k splits' parts in order and applies the epilogue; blocks from sum_blocks on fold the column
+// sums of dz into db
+struct JoinArgs {
+    const float *part;
+    long long I, ldr, part_stride;
+    int J, ldp, splits, sum_blocks, act;
+    const void *bias, *residual;
+    void *out, *slope;
+    const float *colsum;
+    int ncol, nsum;  // columns, and blocks that were summed
+    void *db;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) k_join(JoinArgs a) {
+    if ((int)blockIdx.x >= a.sum_blocks) {
+        __shared__ float red[8][33];
+        const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = ((int)blockIdx.x - a.sum_blocks) * 32 + lane;
+        float t = 0.f;
+        if (c < a.ncol)
+#pragma unroll 4
+            for (int k = w; k < a.nsum; k += 8) t += a.colsum[(long long)k * a.ncol + c];
+        red[w][lane] = t;
+        __syncthreads();
+        if (w == 0 && c < a.ncol) {
+            for (int k = 1; k < 8; k++) t += red[k][lane];
+            from_f32(t, reinterpret_cast<T *>(a.db)[c]);
+        }
+        return;
+    }
+    const int nv = a.ldp / 4;
+    const long long n = a.I * nv;
+    for (long long t = blockIdx.x * 256LL + threadIdx.x; t < n; t += a.sum_blocks * 256LL) {
+        const long long i = t / nv;
+        const int c = (int)(t - i * nv) * 4;
+        const float *p = a.part + i * a.ldp + c;
+        float4 s = *reinterpret_cast<const float4 *>(p);
+#pragma unroll 4
+        for (int k = 1; k < a.splits; k++) {
+            const float4 e = *reinterpret_cast<const float4 *>(p + k * a.part_stride);
+            s.x += e.x;
+            s.y += e.y;
+            s.z += e.z;
+            s.w += e.w;
+        }
+        const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (c + k >= a.J) break;
+            float z = v[k] + (a.bias ? to_f32(reinterpret_cast<const T *>(a.bias)[c + k]) : 0.f), sl;
+            const long long at = i * a.J + c + k;
+            if (a.slope) {
+                z = act_both_rt(z, a.act, sl);
+                if (sizeof(T) == 4) reinterpret_cast<float *>(a.slope)[at] = sl;
+                else reinterpret_cast<uint16_t *>(a.slope)[at] = (uint16_t)slope_code(sl);
+            } else {
+                z = act_rt(z, a.act);
+            }
+            if (a.residual) z = __fadd_rn(z, to_f32(reinterpret_cast<const T *>(a.residual)[i * a.ldr + c + k]));
+            from_f32(z, reinterpret_cast<T *>(a.out)[at]);
+        }
+    }
+}
+
+// ================================================================================================ host
+size_t al(size_t n) { return (n + 255) & ~(size_t)255; }
+int up8(int n) { return (n + 7) & ~7; }
+long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
 
 bool valid(const gs_linear_desc *d) {
-    return d && d->M >= 0 && d->M <= (1LL << 31) && d->N >= 1 && d->K >= 1 && d->N <= GS_LINEAR_MAX_DIM &&
+    return d && d->M >= 0 && d->M <= GS_LINEAR_MAX_ROWS && d->N >= 1 && d->K >= 1 && d->N <= GS_LINEAR_MAX_DIM &&
            d->K <= GS_LINEAR_MAX_DIM && d->dtype >= GS_F32 && d->dtype <= GS_F16 && d->act >= GS_ACT_NONE &&
-           d->act <= GS_ACT_SILU;
+           d->act <= GS_ACT_SILU && d->ldx >= d->K && d->ldw >= d->K && (d->unaligned & ~7) == 0 &&
+           d->ldx <= GS_LINEAR_MAX_LD && d->ldw <= GS_LINEAR_MAX_LD && d->ldr <= GS_LINEAR_MAX_LD &&
+           d->ldy <= GS_LINEAR_MAX_LD && d->M * std::max(d->N, d->K) <= 1LL << 40;
 }
-size_t elem(const gs_linear_desc *d) { return d->dtype == GS_F32 ? 4 : 2; }
-size_t al(size_t n) { return (n + 255) & ~(size_t)255; }
 
-int done(const char *where) {
-    const cudaError_t e = cudaGetLastError();
-    if (e == cudaSuccess) return GS_OK;
+// The tile of one product: the columns whose waves over the SMs cost least (a tile's cost: its columns of
+// MMA and epilogue work and a fixed part), then k splits while SMs are left over and a part keeps at least
+// four k-blocks.
+struct Tiling {
+    int bn, tiles_i, tiles_j, splits;
+};
+Tiling tiling(long long I, int J, long long kbt) {
+    Tiling best{64, 0, 0, 1};
+    double least = 0;
+    for (int bn : {256, 128, 64}) {
+        if (bn > 64 && J <= bn / 2) continue;
+        const long long tiles = cdiv(I, BM) * cdiv(J, bn);
+        long long s = 1;
+        if (tiles < SMS) s = std::max<long long>(1, std::min<long long>(SMS / tiles, kbt / 4));
+        const double waves = (double)cdiv(tiles * s, SMS);
+        const double cost = waves * ((double)cdiv(kbt, s) * (bn + 32) + 3.0 * bn + 200);
+        if (least == 0 || cost < least) {
+            least = cost;
+            best = Tiling{bn, (int)cdiv(I, BM), (int)cdiv(J, bn), (int)s};
+        }
+    }
+    return best;
+}
+
+// Workspace of a call: padded or split operands, the parts of split sums, column sums.
+struct Plan {
+    int es, terms, npair;  // element size of the operands' source, bf16 terms, term products
+    int ldx, ldw, ldn;     // row strides of the padded x, W and dz
+    bool prep_x, prep_w, need_dz;
+    Tiling fwd, gx, gw;
+    int dz_rows, dz_cols, dz_cvec, dz_rl;
+    size_t o_x, o_w, o_dz, o_part, o_col, bytes;
+};
+bool ragged(long long ld, int unaligned) { return unaligned || ld % 8 != 0; }
+
+size_t parts(const Tiling &t, long long I, int J) {
+    return t.splits > 1 ? al((size_t)t.splits * I * ((J + 3) & ~3) * 4) : 0;
+}
+Plan plan(const gs_linear_desc *d, bool bwd) {
+    Plan p;
+    memset(&p, 0, sizeof(p));
+    const bool f32 = d->dtype == GS_F32;
+    p.es = f32 ? 4 : 2;
+    p.terms = f32 ? 3 : 1;
+    p.npair = f32 ? 6 : 1;
+    p.ldx = p.ldw = up8(d->K);
+    p.ldn = up8(d->N);
+    p.prep_x = f32 || ragged(d->ldx, d->unaligned & 1);
+    p.prep_w = f32 || ragged(d->ldw, d->unaligned & 2);
+    p.bytes = 256;
+    if (d->M == 0) return p;
+    size_t o = 0;
+    auto take = [&](size_t n) {
+        const size_t at = o;
+        o += al(n);
+        return at;
+    };
+    p.o_x = take(p.prep_x ? (size_t)d->M * p.ldx * 2 * p.terms : 0);
+    p.o_w = take(p.prep_w ? (size_t)d->N * p.ldw * 2 * p.terms : 0);
+    if (!bwd) {
+        p.fwd = tiling(d->M, d->N, cdiv(d->K, BK) * p.npair);
+        p.o_part = take(parts(p.fwd, d->M, d->N));
+    } else {
+        p.need_dz = f32 || d->act != GS_ACT_NONE || ragged(d->ldy, d->unaligned & 4);
+        p.o_dz = take(p.need_dz ? (size_t)d->M * p.ldn * 2 * p.terms : 0);
+        p.gx = tiling(d->M, d->K, cdiv(d->N, BK) * p.npair);
+        p.gw = tiling(d->N, d->K, cdiv(d->M, BK) * p.npair);
+        p.o_part = take(std::max(parts(p.gx, d->M, d->K), parts(p.gw, d->N, d->K)));
+        // dz: blocks of 256 threads, up to 256 column vectors each, about four blocks per SM
+        const int nv = p.ldn / 8;
+        p.dz_cvec = std::min(nv, 256);
+        p.dz_cols = (int)cdiv(nv, p.dz_cvec);
+        p.dz_rl = 256 / p.dz_cvec;
+        p.dz_rows = (int)std::max<long long>(1, std::min<long long>(cdiv(4 * SMS, p.dz_cols), d->M / (4 * p.dz_rl)));
+        p.o_col = take((size_t)p.dz_rows * d->N * 4);
+    }
+    p.bytes = o + 256;
+    return p;
+}
+
+int cuda_error(const char *where, const char *what) {
     char msg[256];
-    snprintf(msg, sizeof(msg), "%s: %s", where, cudaGetErrorString(e));
+    snprintf(msg, sizeof(msg), "%s: %s", where, what);
     gs_set_last_error(msg);
     return GS_ERR_CUDA;
 }
+int done(const char *where) {
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? GS_OK : cuda_error(where, cudaGetErrorString(e));
+}
 
-template <typename T>
-void product(const void *A, long long ai, long long ak, const void *B, long long bj, long long bk, long long I, int J,
-             long long K, const void *bias, const void *res, long long ldr, int act, void *out, void *z,
-             cudaStream_t s) {
-    dim3 grid((unsigned)((I + 63) / 64), (unsigned)((J + 63) / 64));
-    k_product<T><<<grid, 256, 0, s>>>((const T *)A, ai, ak, (const T *)B, bj, bk, I, J, K, (const T *)bias,
-                                      (const T *)res, ldr, act, (T *)out, (T *)z);
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        cudaDriverEntryPointQueryResult q;
+        void *p = nullptr;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    }();
+    return fn;
+}
+// [terms][rows][cols] elements of es bytes with row stride ld: boxes of box_cols x box_rows, 128-byte swizzle
+bool make_map(CUtensorMap *tm, CUtensorMapDataType type, int es, const void *base, long long cols, long long rows,
+              long long ld, int terms, int box_cols, int box_rows) {
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)terms};
+    const cuuint64_t str[2] = {(cuuint64_t)ld * es, (cuuint64_t)(terms > 1 ? rows : 1) * ld * es};
+    const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1}, one[3] = {1, 1, 1};
+    auto fn = encode_fn();
+    return fn && fn(tm, type, 3, const_cast<void *>(base), dims, str, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int BN, bool OUT32>
+int launch(const CUtensorMap *m, const GemmArgs &a, cudaStream_t s) {
+    using S = Shape<BN, OUT32>;
+    auto kern = k_gemm<BN, OUT32>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM) != cudaSuccess)
+        return done("gs_linear_act");
+    const int items = a.tiles_i * a.tiles_j * a.splits;
+    kern<<<std::min(items, SMS), 320, S::SMEM, s>>>(m[0], m[1], m[2], m[3], m[4], a);
+    return GS_OK;
+}
+
+// one operand of a product: [terms][rows][cols], row stride ld
+struct Operand {
+    const void *p;
+    long long rows, cols, ld;
+    int mn;  // the product's own axis is adjacent (else k is)
+};
+struct Epilogue {
+    const void *bias, *residual;
+    long long ldr;
+    int act;
+    void *out, *slope;
+};
+
+// D [I][J] over k = K; with splits the parts go to `part` and the caller joins them
+int product(const gs_linear_desc *d, const Plan &p, const Tiling &t, long long I, int J, long long K, const Operand &A,
+            const Operand &B, const Epilogue &e, void *part, cudaStream_t s) {
+    GemmArgs a;
+    memset(&a, 0, sizeof(a));
+    const bool f32 = d->dtype == GS_F32, raw = t.splits > 1, out32 = f32 || raw;
+    a.I = I; a.J = J;
+    a.kb = (int)cdiv(K, BK);
+    a.npair = p.npair;
+    a.a_mn = A.mn; a.b_mn = B.mn;
+    a.f16 = d->dtype == GS_F16;
+    a.out_f16 = a.f16;
+    a.splits = t.splits; a.tiles_i = t.tiles_i; a.tiles_j = t.tiles_j;
+    CUtensorMap m[5];
+    const CUtensorMapDataType in = a.f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    bool ok = make_map(&m[0], in, 2, A.p, A.cols, A.rows, A.ld, p.terms, 64, A.mn ? BK : BM) &&
+              make_map(&m[1], in, 2, B.p, B.cols, B.rows, B.ld, p.terms, 64, B.mn ? BK : t.bn);
+    m[2] = m[3] = m[4] = m[0];
+    if (raw) {
+        a.out_tma = 1;
+        ok = ok && make_map(&m[2], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, part, J, I, (J + 3) & ~3, t.splits, 32, 32);
+    } else {
+        const int es = f32 ? 4 : 2, ec = f32 ? 32 : 64;
+        const CUtensorMapDataType ty = f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+        a.bias = e.bias; a.residual = e.residual; a.ldr = e.ldr; a.act = e.act; a.out = e.out; a.slope = e.slope;
+        const auto whole = [&](const void *q, long long ld) { return ((uintptr_t)q & 15) == 0 && ld * es % 16 == 0; };
+        a.out_tma = whole(e.out, J) && (!e.slope || whole(e.slope, J));
+        a.res_tma = e.residual && whole(e.residual, e.ldr);
+        if (a.out_tma) ok = ok && make_map(&m[2], ty, es, e.out, J, I, J, 1, ec, 32);
+        if (a.out_tma && e.slope) ok = ok && make_map(&m[3], ty, es, e.slope, J, I, J, 1, ec, 32);
+        if (a.res_tma) ok = ok && make_map(&m[4], ty, es, e.residual, J, I, e.ldr, 1, ec, 32);
+    }
+    if (!ok) return cuda_error("gs_linear_act", "cuTensorMapEncodeTiled refused a tensor");
+    gs_count_launch(1);
+    if (out32)
+        return t.bn == 256 ? launch<256, true>(m, a, s) : t.bn == 128 ? launch<128, true>(m, a, s) : launch<64, true>(m, a, s);
+    return t.bn == 256 ? launch<256, false>(m, a, s) : t.bn == 128 ? launch<128, false>(m, a, s) : launch<64, false>(m, a, s);
 }
 
 template <typename T>
-int forward(const gs_linear_desc *d, const void *x, const void *w, const void *bias, const void *res, void *y, void *z,
-            cudaStream_t s) {
-    product<T>(x, d->ldx, 1, w, d->ldw, 1, d->M, d->N, d->K, bias, res, d->ldr, d->act, y, z, s);
+void prep(const PrepJob *jobs, int n, cudaStream_t s) {
+    if (!n) return;
+    long long most = 0;
+    for (int k = 0; k < n; k++) most = std::max(most, jobs[k].rows * (jobs[k].ldp / 8));
+    k_prep_operand<T><<<dim3((unsigned)std::min<long long>(cdiv(most, 256), 16 * SMS), n), 256, 0, s>>>(jobs[0], jobs[n - 1]);
     gs_count_launch(1);
+}
+template <typename T>
+void join(const Tiling *t, long long I, int J, const Epilogue &e, const void *part, const float *colsum, int ncol, int nsum,
+          void *db, cudaStream_t s) {
+    JoinArgs a;
+    memset(&a, 0, sizeof(a));
+    if (t) {
+        a.part = reinterpret_cast<const float *>(part);
+        a.I = I; a.J = J; a.ldp = (J + 3) & ~3; a.part_stride = I * a.ldp; a.splits = t->splits;
+        a.sum_blocks = (int)std::min<long long>(cdiv(I * (a.ldp / 4), 256), 8 * SMS);
+        a.bias = e.bias; a.residual = e.residual; a.ldr = e.ldr; a.act = e.act; a.out = e.out; a.slope = e.slope;
+    }
+    a.colsum = colsum; a.ncol = ncol; a.nsum = nsum; a.db = db;
+    const int fold = db ? (int)cdiv(ncol, 32) : 0;
+    if (a.sum_blocks + fold == 0) return;
+    k_join<T><<<a.sum_blocks + fold, 256, 0, s>>>(a);
+    gs_count_launch(1);
+}
+
+char *base_of(void *ws) { return reinterpret_cast<char *>(al((uintptr_t)ws)); }
+
+// x and W as the products read them: in place, or prepared in the workspace
+template <typename T>
+void operands(const gs_linear_desc *d, const Plan &p, const void *x, const void *w, char *ws, bool want_x, bool want_w,
+              Operand &X, Operand &W, cudaStream_t s) {
+    PrepJob jobs[2];
+    int n = 0;
+    X = Operand{x, d->M, d->K, d->ldx, 0};
+    W = Operand{w, d->N, d->K, d->ldw, 0};
+    if (want_x && p.prep_x) {
+        jobs[n++] = PrepJob{x, ws + p.o_x, d->M, d->ldx, d->K, p.ldx};
+        X.p = ws + p.o_x;
+        X.ld = p.ldx;
+    }
+    if (want_w && p.prep_w) {
+        jobs[n++] = PrepJob{w, ws + p.o_w, d->N, d->ldw, d->K, p.ldw};
+        W.p = ws + p.o_w;
+        W.ld = p.ldw;
+    }
+    prep<T>(jobs, n, s);
+}
+
+template <typename T>
+int forward(const gs_linear_desc *d, const Plan &p, const void *x, const void *w, const Epilogue &e, void *workspace,
+            cudaStream_t s) {
+    char *ws = base_of(workspace);
+    Operand X, W;
+    operands<T>(d, p, x, w, ws, true, true, X, W, s);
+    const int st = product(d, p, p.fwd, d->M, d->N, d->K, X, W, e, ws + p.o_part, s);
+    if (st != GS_OK) return st;
+    if (p.fwd.splits > 1) join<T>(&p.fwd, d->M, d->N, e, ws + p.o_part, nullptr, 0, 0, nullptr, s);
     return done("gs_linear_act_fwd");
 }
+
 template <typename T>
-int backward(const gs_linear_desc *d, const void *x, const void *w, const void *z, const void *dy, void *dx, void *dw,
-             void *db, void *ws, cudaStream_t s) {
-    const long long n = d->M * d->N;
-    T *dz = (T *)al((uintptr_t)ws);
-    k_dz<T><<<(unsigned)std::min<long long>((n + 255) / 256, 4096), 256, 0, s>>>((const T *)dy, d->ldy, (const T *)z,
-                                                                                 dz, d->M, d->N, d->act);
-    if (dx) product<T>(dz, d->N, 1, w, 1, d->ldw, d->M, d->K, d->N, nullptr, nullptr, 0, 0, dx, nullptr, s);
-    if (dw) product<T>(dz, 1, d->N, x, 1, d->ldx, d->N, d->K, d->M, nullptr, nullptr, 0, 0, dw, nullptr, s);
-    if (db) k_colsum<T><<<(unsigned)((d->N + 31) / 32), 1024, 0, s>>>(dz, (T *)db, d->M, d->N);
-    gs_count_launch(1 + (dx != nullptr) + (dw != nullptr) + (db != nullptr));
+int backward(const gs_linear_desc *d, const Plan &p, const void *x, const void *w, const void *slope, const void *dy,
+             void *dx, void *dw, void *db, void *workspace, cudaStream_t s) {
+    char *ws = base_of(workspace);
+    Operand X, W;
+    operands<T>(d, p, x, w, ws, dw != nullptr, dx != nullptr, X, W, s);
+    Operand Z{dy, d->M, d->N, d->ldy, 0};
+    const bool make_dz = p.need_dz && (dx || dw);
+    float *colsum = db ? reinterpret_cast<float *>(ws + p.o_col) : nullptr;
+    if (make_dz) {
+        Z.p = ws + p.o_dz;
+        Z.ld = p.ldn;
+    }
+    if (make_dz || db) {
+        DzArgs a{dy, slope, make_dz ? ws + p.o_dz : nullptr, colsum, d->M, d->ldy, d->N, p.ldn, p.dz_cvec, p.dz_rl, 0};
+        a.vec = !ragged(d->ldy, d->unaligned & 4) && d->N % 8 == 0 && ((uintptr_t)slope & 15) == 0;
+        k_dz<T><<<dim3((unsigned)p.dz_rows, (unsigned)p.dz_cols), 256, 0, s>>>(a);
+        gs_count_launch(1);
+    }
+    int st = GS_OK;
+    if (dx) {
+        Operand B = W;
+        B.mn = 1;
+        const Epilogue e{nullptr, nullptr, 0, 0, dx, nullptr};
+        st = product(d, p, p.gx, d->M, d->K, d->N, Z, B, e, ws + p.o_part, s);
+        if (st != GS_OK) return st;
+        if (p.gx.splits > 1) join<T>(&p.gx, d->M, d->K, e, ws + p.o_part, nullptr, 0, 0, nullptr, s);
+    }
+    const Epilogue e{nullptr, nullptr, 0, 0, dw, nullptr};
+    if (dw) {
+        Operand A = Z, B = X;
+        A.mn = B.mn = 1;
+        st = product(d, p, p.gw, d->N, d->K, d->M, A, B, e, ws + p.o_part, s);
+        if (st != GS_OK) return st;
+    }
+    join<T>(dw && p.gw.splits > 1 ? &p.gw : nullptr, d->N, d->K, e, ws + p.o_part, colsum, d->N, p.dz_rows, db, s);
     return done("gs_linear_act_bwd");
 }
 
 }  // namespace
 
 extern "C" size_t gs_linear_act_workspace_size(const gs_linear_desc *d, int backward) {
-    if (!valid(d)) return 0;
-    return 256 + (backward ? al((size_t)d->M * d->N * elem(d)) : 0);
+    return valid(d) ? plan(d, backward != 0).bytes : 0;
 }
 
 extern "C" int gs_linear_act_fwd(const gs_linear_desc *d, const void *x, const void *w, const void *bias,
-                                 const void *residual, void *y, void *z, void *workspace, size_t workspace_bytes,
+                                 const void *residual, void *y, void *slope, void *workspace, size_t workspace_bytes,
                                  void *stream) {
-    if (!valid(d) || d->ldx < d->K || d->ldw < d->K || (residual && d->ldr < d->N)) return GS_ERR_BAD_ARGUMENT;
+    if (!valid(d) || (residual && d->ldr < d->N)) return GS_ERR_BAD_ARGUMENT;
     if (d->M == 0) return GS_OK;
     if (!x || !w || !y) return GS_ERR_BAD_ARGUMENT;
-    if (!workspace || workspace_bytes < gs_linear_act_workspace_size(d, 0)) return GS_ERR_WORKSPACE;
+    if ((((uintptr_t)x & 15) && !(d->unaligned & 1)) || (((uintptr_t)w & 15) && !(d->unaligned & 2)))
+        return GS_ERR_BAD_ARGUMENT;
+    const Plan p = plan(d, false);
+    if (!workspace || workspace_bytes < p.bytes) return GS_ERR_WORKSPACE;
     cudaStream_t s = (cudaStream_t)stream;
-    if (d->dtype == GS_F32) return forward<float>(d, x, w, bias, residual, y, z, s);
-    if (d->dtype == GS_BF16) return forward<__nv_bfloat16>(d, x, w, bias, residual, y, z, s);
-    return forward<__half>(d, x, w, bias, residual, y, z, s);
+    const Epilogue e{bias, residual, d->ldr, d->act, y, d->act == GS_ACT_NONE ? nullptr : slope};
+    if (d->dtype == GS_F32) return forward<float>(d, p, x, w, e, workspace, s);
+    if (d->dtype == GS_BF16) return forward<__nv_bfloat16>(d, p, x, w, e, workspace, s);
+    return forward<__half>(d, p, x, w, e, workspace, s);
 }
 
-extern "C" int gs_linear_act_bwd(const gs_linear_desc *d, const void *x, const void *w, const void *z, const void *dy,
-                                 void *dx, void *dw, void *dbias, void *workspace, size_t workspace_bytes,
-                                 void *stream) {
-    if (!valid(d) || d->ldx < d->K || d->ldw < d->K || d->ldy < d->N) return GS_ERR_BAD_ARGUMENT;
+extern "C" int gs_linear_act_bwd(const gs_linear_desc *d, const void *x, const void *w, const void *slope,
+                                 const void *dy, void *dx, void *dw, void *dbias, void *workspace,
+                                 size_t workspace_bytes, void *stream) {
+    if (!valid(d) || d->ldy < d->N) return GS_ERR_BAD_ARGUMENT;
     cudaStream_t s = (cudaStream_t)stream;
+    const size_t es = d->dtype == GS_F32 ? 4 : 2;
     if (d->M == 0) {
-        if (dw) cudaMemsetAsync(dw, 0, (size_t)d->N * d->K * elem(d), s);
-        if (dbias) cudaMemsetAsync(dbias, 0, (size_t)d->N * elem(d), s);
+        if (dw) cudaMemsetAsync(dw, 0, (size_t)d->N * d->K * es, s);
+        if (dbias) cudaMemsetAsync(dbias, 0, (size_t)d->N * es, s);
         return done("gs_linear_act_bwd");
     }
-    if (!x || !w || !dy || (d->act != GS_ACT_NONE && !z)) return GS_ERR_BAD_ARGUMENT;
-    if (!workspace || workspace_bytes < gs_linear_act_workspace_size(d, 1)) return GS_ERR_WORKSPACE;
-    if (d->act == GS_ACT_NONE) z = nullptr;
-    if (d->dtype == GS_F32) return backward<float>(d, x, w, z, dy, dx, dw, dbias, workspace, s);
-    if (d->dtype == GS_BF16) return backward<__nv_bfloat16>(d, x, w, z, dy, dx, dw, dbias, workspace, s);
-    return backward<__half>(d, x, w, z, dy, dx, dw, dbias, workspace, s);
+    if (!x || !w || !dy || (d->act != GS_ACT_NONE && !slope)) return GS_ERR_BAD_ARGUMENT;
+    if ((((uintptr_t)x & 15) && !(d->unaligned & 1)) || (((uintptr_t)w & 15) && !(d->unaligned & 2)) ||
+        (((uintptr_t)dy & 15) && !(d->unaligned & 4)))
+        return GS_ERR_BAD_ARGUMENT;
+    const Plan p = plan(d, true);
+    if (!workspace || workspace_bytes < p.bytes) return GS_ERR_WORKSPACE;
+    if (d->act == GS_ACT_NONE) slope = nullptr;
+    if (d->dtype == GS_F32) return backward<float>(d, p, x, w, slope, dy, dx, dw, dbias, workspace, s);
+    if (d->dtype == GS_BF16) return backward<__nv_bfloat16>(d, p, x, w, slope, dy, dx, dw, dbias, workspace, s);
+    return backward<__half>(d, p, x, w, slope, dy, dx, dw, dbias, workspace, s);
+}
+
+extern "C" int gs_linear_error_flag(int *flag_host) {
+    if (!flag_host) return GS_ERR_BAD_ARGUMENT;
+    const cudaError_t e = cudaMemcpyFromSymbol(flag_host, g_wait_error, sizeof(int));
+    return e == cudaSuccess ? GS_OK : cuda_error("gs_linear_error_flag", cudaGetErrorString(e));
 }

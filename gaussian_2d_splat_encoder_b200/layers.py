@@ -40,7 +40,8 @@ class _LinearDesc(C.Structure):
     """Mirror of gs_linear_desc."""
 
     _fields_ = [("M", C.c_int64), ("N", C.c_int32), ("K", C.c_int32), ("dtype", C.c_int32), ("act", C.c_int32),
-                ("ldx", C.c_int64), ("ldw", C.c_int64), ("ldr", C.c_int64), ("ldy", C.c_int64)]
+                ("ldx", C.c_int64), ("ldw", C.c_int64), ("ldr", C.c_int64), ("ldy", C.c_int64),
+                ("unaligned", C.c_int32)]
 
 
 def _act_code(act):
@@ -203,8 +204,8 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
 
 # --------------------------------------------------------------------------------------- linear
 @functools.lru_cache(maxsize=1024)
-def _linear_plan(M, N, K, dtype, act, ldx, ldw, ldr, ldy):
-    d = _LinearDesc(M, N, K, dtype, act, ldx, ldw, ldr, ldy)
+def _linear_plan(M, N, K, dtype, act, ldx, ldw, ldr, ldy, unaligned):
+    d = _LinearDesc(M, N, K, dtype, act, ldx, ldw, ldr, ldy, unaligned)
     L = _lib.load()
     size = L.gs_linear_act_workspace_size
     return C.byref(d), int(size(C.byref(d), 0)), int(size(C.byref(d), 1)), d
@@ -226,38 +227,43 @@ def _linear_forward(x, weight, bias, residual, act, train):
     if residual is not None:
         residual, ldr = _row_layout(residual)
     N, K = weight.shape
-    key = (x.numel() // K, N, K, _DTYPES[x.dtype], act, ldx, ldw, ldr)
-    desc, nbytes, _, _ = _linear_plan(*key, N)
+    unaligned = bool(x.data_ptr() & 15) | bool(weight.data_ptr() & 15) << 1
+    key = (x.numel() // K, N, K, _DTYPES[x.dtype], act, ldx, ldw)
+    desc, nbytes, _, _ = _linear_plan(*key, ldr, 0, unaligned)
     if nbytes == 0:
         raise ValueError(f"unsupported sizes: {tuple(x.shape)} and {tuple(weight.shape)}")
     dev = x.device
     with _scope(dev):
         shape = x.shape[:-1] + (N,)
         y = torch.empty(shape, dtype=x.dtype, device=dev)
-        z = torch.empty(shape, dtype=x.dtype, device=dev) if train and act else None
+        # the activation's slope, as the backward takes it: fp32, or 16-bit fixed point
+        slope = torch.empty(shape, dtype=x.dtype if x.dtype == torch.float32 else torch.int16,
+                            device=dev) if train and act else None
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         ptr = _lib.ptr
-        _lib.check(_lib.load().gs_linear_act_fwd(desc, ptr(x), ptr(weight), ptr(bias), ptr(residual), ptr(y), ptr(z),
-                                                 ptr(ws), nbytes, _lib.stream_of(dev)), "gs_linear_act_fwd")
-    return y, x, weight, z, key
+        _lib.check(_lib.load().gs_linear_act_fwd(desc, ptr(x), ptr(weight), ptr(bias), ptr(residual), ptr(y),
+                                                 ptr(slope), ptr(ws), nbytes, _lib.stream_of(dev)),
+                   "gs_linear_act_fwd")
+    return y, x, weight, slope, key + (unaligned,)
 
 
 class _LinearAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
-        y, x, weight, z, ctx.key = _linear_forward(x, weight, bias, residual, act, True)
-        ctx.save_for_backward(x, weight, z)
+        y, x, weight, slope, ctx.key = _linear_forward(x, weight, bias, residual, act, True)
+        ctx.save_for_backward(x, weight, slope)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, z = ctx.saved_tensors
+        x, weight, slope = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dw = db = None
         if need[0] or need[1] or need[2]:
             g, ldy = _row_layout(dy)
-            desc, _, nbytes, _ = _linear_plan(*ctx.key, ldy)
+            *key, unaligned = ctx.key
+            desc, _, nbytes, _ = _linear_plan(*key, 0, ldy, unaligned | bool(g.data_ptr() & 15) << 2)
             dev = x.device
             with _scope(dev):
                 dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
@@ -265,8 +271,8 @@ class _LinearAct(torch.autograd.Function):
                 db = torch.empty(weight.shape[0], dtype=x.dtype, device=dev) if need[2] else None
                 ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
                 ptr = _lib.ptr
-                _lib.check(_lib.load().gs_linear_act_bwd(desc, ptr(x), ptr(weight), ptr(z), ptr(g), ptr(dx), ptr(dw),
-                                                         ptr(db), ptr(ws), nbytes, _lib.stream_of(dev)),
+                _lib.check(_lib.load().gs_linear_act_bwd(desc, ptr(x), ptr(weight), ptr(slope), ptr(g), ptr(dx),
+                                                         ptr(dw), ptr(db), ptr(ws), nbytes, _lib.stream_of(dev)),
                            "gs_linear_act_bwd")
         return dx, dw, db, dy if need[3] else None, None
 

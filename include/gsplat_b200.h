@@ -279,25 +279,34 @@ int gs_group_norm_act_bwd(const gs_norm_desc *d, const void *x, const void *weig
 
 /* Linear layer y = act(x W^T + bias) + residual: x [M][K], W [N][K], residual, y, z [M][N], bias [N], all of
  * one element type, sums in fp32; x, W, residual and dy have free row strides (in elements, at least the
- * row's length), outputs are tightly packed.  N, K <= GS_LINEAR_MAX_DIM. */
+ * row's length), outputs are tightly packed.  Limits: M <= GS_LINEAR_MAX_ROWS, N and K <= GS_LINEAR_MAX_DIM, row strides <=
+ * GS_LINEAR_MAX_LD, M * N and M * K <= 2^40. */
+#define GS_LINEAR_MAX_ROWS (1 << 30)
 #define GS_LINEAR_MAX_DIM (1 << 20)
+#define GS_LINEAR_MAX_LD (1LL << 36)
 typedef struct {
     int64_t M;
     int32_t N, K;
     int32_t dtype, act;
     int64_t ldx, ldw, ldr; /* row strides of x, W and the residual */
     int64_t ldy;           /* row stride of dy (backward) */
+    int32_t unaligned;     /* bit 0 x, 1 W, 2 dy: the pointer is not on 16 bytes (the call then keeps a copy in
+                              the workspace); a less aligned pointer without its bit is refused */
 } gs_linear_desc;
 
 /* Workspace bytes of a forward (backward = 0) or a backward (1) call; 0 for an invalid descriptor. */
 size_t gs_linear_act_workspace_size(const gs_linear_desc *d, int backward);
-/* bias, residual and z may be NULL; z receives x W^T + bias for the backward of an activation. */
+/* bias, residual and slope may be NULL; slope [M][N] (2 bytes an element for 16-bit types, else 4) receives
+ * the activation's slope for the backward, in the library's own encoding; not written without an activation. */
 int gs_linear_act_fwd(const gs_linear_desc *d, const void *x, const void *w, const void *bias, const void *residual,
-                      void *y, void *z, void *workspace, size_t workspace_bytes, void *stream);
-/* Gradients for upstream dy: dx [M][K], dw [N][K], dbias [N]; each may be NULL (not computed).  z is the
- * forward's, not read without an activation.  The residual's gradient is dy itself. */
-int gs_linear_act_bwd(const gs_linear_desc *d, const void *x, const void *w, const void *z, const void *dy, void *dx,
+                      void *y, void *slope, void *workspace, size_t workspace_bytes, void *stream);
+/* Gradients for upstream dy: dx [M][K], dw [N][K], dbias [N]; each may be NULL (not computed).
+ * slope is the forward's, not read without an activation.  The residual's gradient is dy itself. */
+int gs_linear_act_bwd(const gs_linear_desc *d, const void *x, const void *w, const void *slope, const void *dy, void *dx,
                       void *dw, void *dbias, void *workspace, size_t workspace_bytes, void *stream);
+/* Reads (synchronously) the code of a bounded device wait of the linear kernels that gave up on the current
+ * device since the library was loaded; 0 if none did.  Outputs of such a call are not valid. */
+int gs_linear_error_flag(int *flag_host);
 
 /* Text of the last CUDA error seen by the calling thread (empty when none). */
 const char *gs_last_error(void);

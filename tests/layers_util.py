@@ -141,8 +141,10 @@ def check_linear(got, grads, x, w, b, r, act, dy):
     (s,) = torch.autograd.grad(ACTS[act](Zl).sum(), Zl)
     with torch.no_grad():
         dz = D * s
-        # z is kept and dz enters the products in x's type; second derivatives stay below 1
-        edz = 0 if act == "none" else (h * z.abs() + ez + lo + ACT_U * U * (1 + z.abs())) * D.abs() + h * dz.abs() + lo
+        # the slope is kept in steps of 1 / 49152 for 16-bit types and dz enters the products in x's type; second
+        # derivatives stay below 1
+        step = 0 if x.dtype == torch.float32 else 0.5 / 49152
+        edz = 0 if act == "none" else (step + ez + ACT_U * U * (1 + z.abs())) * D.abs() + h * dz.abs() + lo
         M = X.shape[0]
         if grads[0] is not None:
             e = edz @ W.abs() if act != "none" else 0

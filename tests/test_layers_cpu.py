@@ -63,15 +63,20 @@ def test_linear_workspace_and_refusals(lib, ops):
         assert lib.gs_linear_act_fwd(C.byref(d), *[None] * 7, 0, None) == 2, bad
         assert lib.gs_linear_act_bwd(C.byref(d), *[None] * 8, 0, None) == 2, bad
     p = C.c_void_p(256)
-    for bad in (dict(ldx=63), dict(ldw=63), dict(ldr=31)):
+    for bad in (dict(ldx=63), dict(ldw=63), dict(ldr=31), dict(unaligned=8), dict(M=(1 << 30) + 1), dict(ldx=1 << 37)):
         d = linear_desc(ops, **bad)
         assert lib.gs_linear_act_fwd(C.byref(d), p, p, None, p, p, None, p, 1 << 30, None) == 2, bad
     assert lib.gs_linear_act_bwd(C.byref(linear_desc(ops, ldy=31)), p, p, p, p, p, p, p, p, 1 << 30, None) == 2
     d = linear_desc(ops)
     assert lib.gs_linear_act_fwd(C.byref(d), p, p, None, None, p, None, p, 16, None) == 5
     assert lib.gs_linear_act_bwd(C.byref(d), p, p, p, p, p, p, p, p, 16, None) == 5
-    # the backward of an activation needs the kept pre-activation
+    q = C.c_void_p(264)  # off 16 bytes, without the descriptor's bit
+    assert lib.gs_linear_act_fwd(C.byref(d), q, p, None, None, p, None, p, 1 << 40, None) == 2
+    assert lib.gs_linear_act_fwd(C.byref(d), p, q, None, None, p, None, p, 1 << 40, None) == 2
+    assert lib.gs_linear_act_bwd(C.byref(d), p, p, p, q, p, p, p, p, 1 << 40, None) == 2
+    # the backward of an activation needs the kept slope
     assert lib.gs_linear_act_bwd(C.byref(d), p, p, None, p, p, p, p, p, 1 << 40, None) == 2
+    assert size(C.byref(linear_desc(ops, M=0)), 0) > 0 and size(C.byref(linear_desc(ops, M=0)), 1) > 0
     assert lib.gs_linear_act_fwd(C.byref(linear_desc(ops, M=0)), *[None] * 7, 0, None) == 0
 
 

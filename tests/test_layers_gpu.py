@@ -399,3 +399,12 @@ def test_refusals_on_the_device(ops):
     (g,) = torch.autograd.grad(y.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), x)
+
+
+def test_no_wait_gave_up(ops, lib):
+    """No bounded device wait of the linear kernels ran out in this process."""
+    import ctypes as C
+
+    flag = C.c_int(-1)
+    torch.cuda.synchronize()
+    assert lib.gs_linear_error_flag(C.byref(flag)) == 0 and flag.value == 0
