@@ -42,21 +42,36 @@ constexpr int BM = 128, BK = 64;
 
 __device__ int g_wait_error;  // code of a bounded wait that gave up (gs_linear_error_flag), 0 if none did
 
-// ---- the kept slope: fp32, or 16-bit fixed point (0 and 1 exact, 65535 is NaN)
-__device__ __forceinline__ uint32_t slope_code(float s) {
-    return s == s ? __float2uint_rn(fmaf(s, 49152.f, 8192.f)) : 65535u;
+// ---- the kept slope: fp32, or 16-bit fixed point (0 and 1 exact, 65535 is NaN).  s 49152 + 8192 + 2^23 rounds
+// to the code in the low mantissa bits; the canonical NaN's low bits are 65535.
+__device__ __forceinline__ uint32_t slope_codes(f2 s) {  // two codes, the first in the low half
+    const f2 c = fma2(s, both(49152.f), both(8192.f + 8388608.f));
+    return __byte_perm(__float_as_uint(c.x), __float_as_uint(c.y), 0x5410);
 }
 __device__ __forceinline__ float slope_of(uint32_t c) {
-    return c == 65535u ? __int_as_float(0x7fffffff) : ((float)c - 8192.f) * (1.f / 49152.f);
+    const float s = (__uint_as_float(0x4B000000u | c) - (8192.f + 8388608.f)) * (1.f / 49152.f);
+    return c == 65535u ? __int_as_float(0x7fffffff) : s;
 }
 
-__device__ __forceinline__ float act_rt(float z, int act) {
-    return act == ACT_GELU ? gs_act<ACT_GELU>(z) : act == ACT_SILU ? gs_act<ACT_SILU>(z) : z;
+// activation, and with `slope` its slope, of n pairs
+template <int N>
+__device__ __forceinline__ void activate(f2 *v, int act, const Act<ACT_GELU, true> &gelu, const Act<ACT_SILU, true> &silu) {
+    if (act == ACT_GELU)
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = gelu(v[i]);
+    else if (act == ACT_SILU)
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = silu(v[i]);
 }
-__device__ __forceinline__ float act_both_rt(float z, int act, float &slope) {
-    return act == ACT_GELU   ? gs_act_both<ACT_GELU>(z, slope)
-           : act == ACT_SILU ? gs_act_both<ACT_SILU>(z, slope)
-                             : gs_act_both<ACT_NONE>(z, slope);
+template <int N>
+__device__ __forceinline__ void activate(f2 *v, f2 *slope, int act, const Act<ACT_GELU, true> &gelu,
+                                         const Act<ACT_SILU, true> &silu) {
+    if (act == ACT_GELU)
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = gelu(v[i], slope[i]);
+    else
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = silu(v[i], slope[i]);
 }
 
 struct GemmArgs {
@@ -229,6 +244,8 @@ __global__ void __launch_bounds__(320, 1)
         const int e = warp - 2, q = warp & 3, half = e >> 2;
         uint8_t *const slots = smem + STAGES * S::STAGE + e * 8192;
         const bool has_res = a.residual != nullptr, has_slope = a.slope != nullptr;
+        const Act<ACT_GELU, true> gelu;
+        const Act<ACT_SILU, true> silu;
         int tc = 0, use = 0, rphase[2] = {0, 0};
         for (int item = blockIdx.x; item < n_items; item += gridDim.x, tc++) {
             const int buf = tc & 1;
@@ -316,40 +333,34 @@ __global__ void __launch_bounds__(320, 1)
                     constexpr int W = OUT32 ? 4 : 8;
 #pragma unroll
                     for (int g = 0; g < 32 / W; g++) {
-                        float v[W], sv[W];
+                        f2 v[W / 2];
                         const uint32_t at = (uint32_t)lane * 128u + ((uint32_t)(((OUT32 ? 0 : 4 * h) + g) ^ (lane & 7)) << 4);
 #pragma unroll
-                        for (int i = 0; i < W; i++) v[i] = __uint_as_float(r[g * W + i]) + sbias[e][g * W + i];
+                        for (int i = 0; i < W / 2; i++) {
+                            const float2 b = *reinterpret_cast<const float2 *>(&sbias[e][g * W + 2 * i]);
+                            v[i] = add2({__uint_as_float(r[g * W + 2 * i]), __uint_as_float(r[g * W + 2 * i + 1])}, {b.x, b.y});
+                        }
                         if (has_slope) {
-#pragma unroll
-                            for (int i = 0; i < W; i++) v[i] = act_both_rt(v[i], a.act, sv[i]);
-                            uint4 p;
-                            if (OUT32) {
-                                p = pack16<float>(sv);
-                            } else {
-                                uint32_t w[4];
-#pragma unroll
-                                for (int i = 0; i < 4; i++)
-                                    w[i] = slope_code(sv[(2 * i) % W]) | slope_code(sv[(2 * i + 1) % W]) << 16;
-                                p = make_uint4(w[0], w[1], w[2], w[3]);
-                            }
-                            *reinterpret_cast<uint4 *>(slo + at) = p;
-                        } else if (a.act) {
-#pragma unroll
-                            for (int i = 0; i < W; i++) v[i] = act_rt(v[i], a.act);
+                            f2 sv[W / 2];
+                            activate<W / 2>(v, sv, a.act, gelu, silu);
+                            *reinterpret_cast<uint4 *>(slo + at) =
+                                OUT32 ? pack16<float>(sv)
+                                      : make_uint4(slope_codes(sv[0]), slope_codes(sv[1]), slope_codes(sv[2 % (W / 2)]),
+                                                   slope_codes(sv[3 % (W / 2)]));
+                        } else {
+                            activate<W / 2>(v, a.act, gelu, silu);
                         }
                         if (has_res) {
                             const uint4 p = *reinterpret_cast<const uint4 *>(out + at);
-                            float f[8];
+                            f2 f[4];
                             if (OUT32) unpack16<float>(p, f);
                             else if (a.out_f16) unpack16<__half>(p, f);
                             else unpack16<__nv_bfloat16>(p, f);
 #pragma unroll
-                            for (int i = 0; i < W; i++) v[i] = __fadd_rn(v[i], f[i]);
+                            for (int i = 0; i < W / 2; i++) v[i] = add2(v[i], f[i]);
                         }
-                        *reinterpret_cast<uint4 *>(out + at) = OUT32       ? pack16<float>(v)
-                                                               : a.out_f16 ? pack16<__half>(v)
-                                                                           : pack16<__nv_bfloat16>(v);
+                        if (OUT32) *reinterpret_cast<uint4 *>(out + at) = pack16<float>(v);
+                        else *reinterpret_cast<uint4 *>(out + at) = a.out_f16 ? pack16<__half>(v) : pack16<__nv_bfloat16>(v);
                     }
                 }
                 if (!live || dead) continue;
@@ -414,10 +425,10 @@ __device__ __forceinline__ void split3(float x, float &h, float &m, float &l) {
     m = __bfloat162float(__float2bfloat16_rn(r));
     l = r - m;
 }
-__device__ __forceinline__ void store_terms(float *v, __nv_bfloat16 *dst, long long term_stride) {
-    float h[8], m[8], l[8];
+__device__ __forceinline__ void store_terms(const f2 *v, __nv_bfloat16 *dst, long long term_stride) {
+    f2 h[4], m[4], l[4];
 #pragma unroll
-    for (int i = 0; i < 8; i++) split3(v[i], h[i], m[i], l[i]);
+    for (int i = 0; i < 8; i++) split3(at(v, i), at(h, i), at(m, i), at(l, i));
     *reinterpret_cast<uint4 *>(dst) = pack16<__nv_bfloat16>(h);
     *reinterpret_cast<uint4 *>(dst + term_stride) = pack16<__nv_bfloat16>(m);
     *reinterpret_cast<uint4 *>(dst + 2 * term_stride) = pack16<__nv_bfloat16>(l);
@@ -432,9 +443,9 @@ __global__ void __launch_bounds__(256) k_prep_operand(PrepJob a, PrepJob b) {
         const int c = (int)(t - r * nv) * 8;
         const T *p = reinterpret_cast<const T *>(j.src) + r * j.ld + c;
         if (sizeof(T) == 4) {
-            float v[8];
+            f2 v[4];
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = c + i < j.cols ? to_f32(p[i]) : 0.f;
+            for (int i = 0; i < 8; i++) at(v, i) = c + i < j.cols ? to_f32(p[i]) : 0.f;
             store_terms(v, reinterpret_cast<__nv_bfloat16 *>(j.dst) + r * j.ldp + c, j.rows * j.ldp);
         } else {
             uint32_t w[4];
@@ -463,58 +474,57 @@ __global__ void __launch_bounds__(256) k_dz(DzArgs a) {
     const int c = (blockIdx.y * a.cvec + cv) * 8;
     const bool live = r < a.rl && c < a.ldp;
     const long long lo = a.M * blockIdx.x / gridDim.x, hi = a.M * (blockIdx.x + 1LL) / gridDim.x;
-    float s[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) s[i] = 0.f;
+    f2 s[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
     if (live)
 #pragma unroll 2
         for (long long m = lo + r; m < hi; m += a.rl) {
             const T *p = reinterpret_cast<const T *>(a.dy) + m * a.ldy + c;
-            float v[8];
+            f2 v[4];
             if (a.vec) {
-                if (sizeof(T) == 4) {
-                    unpack16<float>(reinterpret_cast<const uint4 *>(p)[0], v);
-                    unpack16<float>(reinterpret_cast<const uint4 *>(p)[1], v + 4);
-                } else {
-                    unpack16<T>(*reinterpret_cast<const uint4 *>(p), v);
-                }
+                unpack8<T>(*reinterpret_cast<const Raw8<T> *>(p), v);
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = c + i < a.N ? to_f32(p[i]) : 0.f;
+                for (int i = 0; i < 8; i++) at(v, i) = c + i < a.N ? to_f32(p[i]) : 0.f;
             }
-            if (a.slope) {  // (products of their own rounding: db's bits do not depend on dz being written)
+            if (a.slope) {
+                f2 g[4];
                 if (sizeof(T) == 4) {
                     const float *q = reinterpret_cast<const float *>(a.slope) + m * a.N + c;
+                    if (a.vec) {
+                        unpack8<float>(*reinterpret_cast<const Raw8<float> *>(q), g);
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) v[i] = __fmul_rn(v[i], a.vec || c + i < a.N ? q[i] : 0.f);
+                        for (int i = 0; i < 8; i++) at(g, i) = c + i < a.N ? q[i] : 0.f;
+                    }
                 } else {
                     const uint16_t *q = reinterpret_cast<const uint16_t *>(a.slope) + m * a.N + c;
                     if (a.vec) {
                         const uint4 w = *reinterpret_cast<const uint4 *>(q);
                         const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                        for (int i = 0; i < 8; i++)
-                            v[i] = __fmul_rn(v[i], slope_of(i & 1 ? x[i >> 1] >> 16 : x[i >> 1] & 0xffffu));
+                        for (int i = 0; i < 8; i++) at(g, i) = slope_of(i & 1 ? x[i >> 1] >> 16 : x[i >> 1] & 0xffffu);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 8; i++) v[i] = c + i < a.N ? __fmul_rn(v[i], slope_of(q[i])) : 0.f;
+                        for (int i = 0; i < 8; i++) at(g, i) = c + i < a.N ? slope_of(q[i]) : 0.f;
                     }
                 }
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[i] = mul2(v[i], g[i]);
             }
 #pragma unroll
-            for (int i = 0; i < 8; i++) s[i] += v[i];
+            for (int i = 0; i < 4; i++) s[i] = add2(s[i], v[i]);
             if (a.dz) {
                 if (sizeof(T) == 4)
                     store_terms(v, reinterpret_cast<__nv_bfloat16 *>(a.dz) + m * a.ldp + c, a.M * a.ldp);
                 else
-                    *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.dz) + m * a.ldp + c) = pack16<T>(v);
+                    *reinterpret_cast<Raw8<T> *>(reinterpret_cast<T *>(a.dz) + m * a.ldp + c) = pack8<T>(v);
             }
         }
     if (!a.colsum) return;
     const int w = a.cvec * 8;
     if (r < a.rl)
 #pragma unroll
-        for (int i = 0; i < 8; i++) buf[r * w + cv * 8 + i] = s[i];
+        for (int i = 0; i < 8; i++) buf[r * w + cv * 8 + i] = at(s, i);
     for (int n = a.rl; n > 1;) {
         const int h = (n + 1) >> 1;
         __syncthreads();
@@ -559,6 +569,8 @@ __global__ void __launch_bounds__(256) k_join(JoinArgs a) {
         }
         return;
     }
+    const Act<ACT_GELU, true> gelu;
+    const Act<ACT_SILU, true> silu;
     const int nv = a.ldp / 4;
     const long long n = a.I * nv;
     for (long long t = blockIdx.x * 256LL + threadIdx.x; t < n; t += a.sum_blocks * 256LL) {
@@ -574,18 +586,23 @@ __global__ void __launch_bounds__(256) k_join(JoinArgs a) {
             s.z += e.z;
             s.w += e.w;
         }
-        const float v[4] = {s.x, s.y, s.z, s.w};
+        f2 v[2] = {{s.x, s.y}, {s.z, s.w}}, sl[2];
+        const int n = min(4, a.J - c);
+        if (a.bias) {
+            const T *b = reinterpret_cast<const T *>(a.bias) + c;
+            v[0] = add2(v[0], {to_f32(b[0]), n > 1 ? to_f32(b[1]) : 0.f});
+            v[1] = add2(v[1], {n > 2 ? to_f32(b[2]) : 0.f, n > 3 ? to_f32(b[3]) : 0.f});
+        }
+        if (a.slope) activate<2>(v, sl, a.act, gelu, silu);
+        else activate<2>(v, a.act, gelu, silu);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            if (c + k >= a.J) break;
-            float z = v[k] + (a.bias ? to_f32(reinterpret_cast<const T *>(a.bias)[c + k]) : 0.f), sl;
+            if (k >= n) break;
             const long long at = i * a.J + c + k;
+            float z = k & 1 ? v[k >> 1].y : v[k >> 1].x;
             if (a.slope) {
-                z = act_both_rt(z, a.act, sl);
-                if (sizeof(T) == 4) reinterpret_cast<float *>(a.slope)[at] = sl;
-                else reinterpret_cast<uint16_t *>(a.slope)[at] = (uint16_t)slope_code(sl);
-            } else {
-                z = act_rt(z, a.act);
+                if (sizeof(T) == 4) reinterpret_cast<float *>(a.slope)[at] = k & 1 ? sl[k >> 1].y : sl[k >> 1].x;
+                else reinterpret_cast<uint16_t *>(a.slope)[at] = (uint16_t)(slope_codes(sl[k >> 1]) >> (16 * (k & 1)));
             }
             if (a.residual) z = __fadd_rn(z, to_f32(reinterpret_cast<const T *>(a.residual)[i * a.ldr + c + k]));
             from_f32(z, reinterpret_cast<T *>(a.out)[at]);
@@ -898,7 +915,7 @@ extern "C" int gs_linear_act_fwd(const gs_linear_desc *d, const void *x, const v
     if ((((uintptr_t)x & 15) && !(d->unaligned & 1)) || (((uintptr_t)w & 15) && !(d->unaligned & 2)))
         return GS_ERR_BAD_ARGUMENT;
     const Plan p = plan(d, false);
-    if (!workspace || workspace_bytes < p.bytes) return GS_ERR_WORKSPACE;
+    if (p.bytes > 256 && (!workspace || workspace_bytes < p.bytes)) return GS_ERR_WORKSPACE;
     cudaStream_t s = (cudaStream_t)stream;
     const Epilogue e{bias, residual, d->ldr, d->act, y, d->act == GS_ACT_NONE ? nullptr : slope};
     if (d->dtype == GS_F32) return forward<float>(d, p, x, w, e, workspace, s);
@@ -922,7 +939,7 @@ extern "C" int gs_linear_act_bwd(const gs_linear_desc *d, const void *x, const v
         (((uintptr_t)dy & 15) && !(d->unaligned & 4)))
         return GS_ERR_BAD_ARGUMENT;
     const Plan p = plan(d, true);
-    if (!workspace || workspace_bytes < p.bytes) return GS_ERR_WORKSPACE;
+    if (p.bytes > 256 && (!workspace || workspace_bytes < p.bytes)) return GS_ERR_WORKSPACE;
     if (d->act == GS_ACT_NONE) slope = nullptr;
     if (d->dtype == GS_F32) return backward<float>(d, p, x, w, slope, dy, dx, dw, dbias, workspace, s);
     if (d->dtype == GS_BF16) return backward<__nv_bfloat16>(d, p, x, w, slope, dy, dx, dw, dbias, workspace, s);

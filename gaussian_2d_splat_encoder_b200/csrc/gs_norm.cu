@@ -10,12 +10,17 @@
 //   du = r (w dz - mean(w dz) - xh mean(w dz xh)),  dx = du, or du act'(x)
 // where the two group means follow from the image's channel sums: sum_c w_c db_c and sum_c w_c dw_c.
 //
-// The operator moves bytes: x is needed twice (statistics, then the map) and fits no SM, so each direction
-// is two launches over the same slices, the second of which finds what L2 (126 MB) still holds.  A block
-// takes a run of rows of one image (and, where there are many groups, a chunk of whole groups); a thread
-// keeps one 16-byte vector of channels for all its rows, so parameters and sums stay in registers and a
-// warp reads contiguous memory.  Statistics are two passes over the slice in fp32 around the slice's own
-// mean, joined across slices as (n, mean, M2): no difference of large squares.  All sums run in a fixed order.
+// The operator moves bytes: x is needed twice (statistics, then the map) and a map of training size fits no
+// SM, so each direction is two launches over the same slices, the second of which finds what L2 (126 MB)
+// still holds.  A block takes a run of rows of one image (and, where there are many groups, a chunk of
+// whole groups); a thread keeps one 16-byte vector of channels for all its rows, so parameters and sums stay
+// in registers and a warp reads contiguous memory.  A forward whose image and group chunk fit the registers
+// of a cluster is one launch: values are read once, the cluster joins its sums over distributed shared
+// memory.  Statistics are taken around means, never as a difference of large squares: four rows at a time
+// exactly around their own mean, joined as (n, mean, M2).  All sums run in a fixed order.
+//
+// With an activation the FMA and MUFU pipes bind as much as memory does (GELU: 0.125 cycles of an SM per
+// element and evaluation), so each launch evaluates it once per element.
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include <stdio.h>
@@ -31,7 +36,9 @@ void gs_set_last_error(const char *msg);
 
 namespace {
 
-constexpr int MAX_T = 512;       // threads of a block
+constexpr int MAX_T = 256;  // threads of a block
+constexpr int V = 8;        // channels of a thread's vector
+constexpr int FUSED_R = 16; // most vectors a thread of the one-launch form holds
 
 struct NormArgs {
     const void *x, *dy, *w, *b;
@@ -43,7 +50,7 @@ struct NormArgs {
     int B, C, G, cpg, splits;
     int chunk, nchunk, cvec, rl;  // channels per block, blocks over channels, vectors per row, rows in flight
     int nslice;                   // blocks of the backward's second launch that map slices
-    int param_f32;
+    int param_f32, fused, held;  // held: vectors a thread of the one-launch form holds
     float eps;
 };
 
@@ -59,22 +66,29 @@ __device__ __forceinline__ void set_param(void *p, int f32, int c, float v) {
 
 // one vector of channels; without 16-byte alignment (or at a ragged end) element by element, zeros beyond
 template <typename T, bool VEC>
-__device__ __forceinline__ void load(const T *p, int valid, float *v) {
-    if (VEC) {
-        unpack16<T>(*reinterpret_cast<const uint4 *>(p), v);
+__device__ __forceinline__ Raw8<T> fetch(const T *p, int valid) {
+    if constexpr (VEC) {
+        return *reinterpret_cast<const Raw8<T> *>(p);
     } else {
+        union {
+            Raw8<T> q;
+            T e[V];
+        } u;
 #pragma unroll
-        for (int i = 0; i < Vec<T>::N; i++) v[i] = i < valid ? to_f32(p[i]) : 0.f;
+        for (int i = 0; i < V; i++)
+            if (i < valid) u.e[i] = p[i];
+            else from_f32(0.f, u.e[i]);
+        return u.q;
     }
 }
 template <typename T, bool VEC>
-__device__ __forceinline__ void store(T *p, int valid, const float *v) {
+__device__ __forceinline__ void store(T *p, int valid, const f2 *v) {
     if (VEC) {
-        *reinterpret_cast<uint4 *>(p) = pack16<T>(v);
+        *reinterpret_cast<Raw8<T> *>(p) = pack8<T>(v);
     } else {
 #pragma unroll
-        for (int i = 0; i < Vec<T>::N; i++)
-            if (i < valid) from_f32(v[i], p[i]);
+        for (int i = 0; i < V; i++)
+            if (i < valid) from_f32(at(v, i), p[i]);
     }
 }
 
@@ -83,12 +97,19 @@ struct Slice {
     int b, s, c0, cc;   // image, split, first channel, channels of this chunk
     int r, cv, c, valid;  // row lane, vector, its first channel, its channels (<= 0: idle thread)
     long long lo, hi;   // rows
-    __device__ Slice(const NormArgs &a, int V) {
-        int t = blockIdx.x;
-        const int k = t % a.nchunk;
-        t /= a.nchunk;
-        s = t % a.splits;
-        b = t / a.splits;
+    __device__ Slice(const NormArgs &a, bool cluster = false) {
+        int t = blockIdx.x, k;
+        if (cluster) {  // the splits of a chunk are neighbours
+            s = t % a.splits;
+            t /= a.splits;
+            k = t % a.nchunk;
+            b = t / a.nchunk;
+        } else {
+            k = t % a.nchunk;
+            t /= a.nchunk;
+            s = t % a.splits;
+            b = t / a.splits;
+        }
         c0 = k * a.chunk;
         cc = min(a.chunk, a.C - c0);
         r = (int)threadIdx.x / a.cvec;
@@ -98,33 +119,118 @@ struct Slice {
         lo = a.rows * s / a.splits;
         hi = a.rows * (s + 1) / a.splits;
     }
+    // rows of this thread: lo + r, lo + r + rl, ...
+    __device__ int rows(const NormArgs &a) const {
+        return valid > 0 && lo + r < hi ? (int)((hi - 1 - lo - r) / a.rl) + 1 : 0;
+    }
 };
 
-// Sums of the block's threads by channel: the row lanes fold in a tree, buf[0..cvec*V) holds the result.
-template <int V>
-__device__ __forceinline__ void fold_rows(float *buf, const float *v, const NormArgs &a, const Slice &sl) {
-    const int w = a.cvec * V;
+// A thread's rows of S tensors, fed through a ring of its own in shared memory: NB batches of B rows, cp.async
+// keeps NB - 1 of them in flight without holding registers.  Unaligned rows are read in place.
+__device__ __forceinline__ void cp_async16(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+                 : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+template <typename T>
+constexpr int ring_batches(int batches) {  // fp32 rows are twice as wide
+    return sizeof(T) == 4 ? (batches + 1) / 2 : batches;
+}
+template <typename T, bool VEC, int S, int B, int BATCHES>
+struct Feed {
+    static constexpr int NB = ring_batches<T>(BATCHES);
+    const T *p[S];
+    long long step[S];
+    int n, valid;  // rows of this thread
+    uint4 *ring;
+    __device__ __forceinline__ uint4 *slot(int j, int s, int q) const {
+        return ring + ((j % (NB * B) * S + s) * ((int)sizeof(T) / 2) + q) * (int)blockDim.x + (int)threadIdx.x;
+    }
+    __device__ __forceinline__ void issue(int batch) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int k = 0; k < B; k++) {
+                const int j = batch * B + k;
+                if (j < n)
+#pragma unroll
+                    for (int s = 0; s < S; s++)
+#pragma unroll
+                        for (int q = 0; q < (int)sizeof(T) / 2; q++)
+                            cp_async16(slot(j, s, q), reinterpret_cast<const uint4 *>(p[s] + j * step[s]) + q);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+    }
+    __device__ __forceinline__ void start() {
+#pragma unroll
+        for (int t = 0; t < NB - 1; t++) issue(t);
+    }
+    // batch t is here, batch t + NB - 1 on its way
+    __device__ __forceinline__ void turn(int t) {
+        issue(t + NB - 1);
+        if (VEC) cp_async_wait<NB - 1>();
+    }
+    __device__ __forceinline__ Raw8<T> get(int j, int s) const {
+        if constexpr (VEC) {
+            Raw8<T> r;
+#pragma unroll
+            for (int q = 0; q < (int)sizeof(T) / 2; q++) r.q[q] = *slot(j, s, q);
+            return r;
+        } else {
+            return fetch<T, false>(p[s] + j * step[s], valid);
+        }
+    }
+};
+template <typename T, int S, int B, int BATCHES>
+constexpr size_t ring_bytes() {
+    return (size_t)ring_batches<T>(BATCHES) * B * S * V * sizeof(T) * MAX_T;
+}
+
+// Sums over the row lanes of W values per thread (0 from idle ones): buf[0..cvec*W) holds the result.  Within
+// a warp by shuffles where its lanes' vectors repeat evenly, across rows or warps in a fixed order.
+template <int W>
+__device__ __forceinline__ void fold_rows(float *buf, float *v, const NormArgs &a, const Slice &sl) {
+    const int w = a.cvec * W;
     __syncthreads();
-    if (sl.r < a.rl)
+    if (32 % a.cvec == 0) {
+        for (int o = a.cvec; o < 32; o <<= 1)
 #pragma unroll
-        for (int i = 0; i < V; i++) buf[sl.r * w + sl.cv * V + i] = i < sl.valid ? v[i] : 0.f;
-    int n = a.rl;
-    while (n > 1) {
-        const int h = (n + 1) >> 1;
+            for (int i = 0; i < W; i++) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+        if (lane < a.cvec)
+#pragma unroll
+            for (int i = 0; i < W; i++) buf[warp * w + lane * W + i] = v[i];
         __syncthreads();
-        if (sl.r < n - h)
+        for (int k = threadIdx.x; k < w; k += blockDim.x) {
+            float s = buf[k];
+            for (int q = 1; q < nw; q++) s += buf[q * w + k];
+            buf[k] = s;
+        }
+    } else {
+        if (sl.r < a.rl)
 #pragma unroll
-            for (int i = 0; i < V; i++) buf[sl.r * w + sl.cv * V + i] += buf[(sl.r + h) * w + sl.cv * V + i];
-        n = h;
+            for (int i = 0; i < W; i++) buf[sl.r * w + sl.cv * W + i] = v[i];
+        int n = a.rl;
+        while (n > 1) {
+            const int h = (n + 1) >> 1;
+            __syncthreads();
+            if (sl.r < n - h)
+#pragma unroll
+                for (int i = 0; i < W; i++) buf[sl.r * w + sl.cv * W + i] += buf[(sl.r + h) * w + sl.cv * W + i];
+            n = h;
+        }
     }
     __syncthreads();
 }
-// Sums of the chunk's groups from channel sums, a warp per group; f maps a channel's sum.
+// Sums over each group's `per` consecutive entries, a warp per group; f gives an entry.
 template <typename F>
-__device__ __forceinline__ void fold_groups(float *gsum, int groups, int cpg, F f) {
+__device__ __forceinline__ void fold_groups(float *gsum, int groups, int per, F f) {
     for (int g = threadIdx.x >> 5; g < groups; g += blockDim.x >> 5) {
         float s = 0.f;
-        for (int c = threadIdx.x & 31; c < cpg; c += 32) s += f(g * cpg + c);
+        for (int c = threadIdx.x & 31; c < per; c += 32) s += f(g * per + c);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if ((threadIdx.x & 31) == 0) gsum[g] = s;
@@ -132,184 +238,378 @@ __device__ __forceinline__ void fold_groups(float *gsum, int groups, int cpg, F 
     __syncthreads();
 }
 
-// ---- forward, first launch: mean and M2 of the slice's groups
-template <typename T, bool VEC, int PRE>
-__global__ void __launch_bounds__(MAX_T) k_gn_stats(NormArgs a) {
-    constexpr int V = Vec<T>::N;
-    extern __shared__ float sm[];
-    const Slice sl(a, V);
-    const int groups = sl.cc / a.cpg, w = a.cvec * V;
-    float *buf = sm, *gsum = sm + (size_t)a.rl * w, *gsq = gsum + a.chunk / a.cpg;
-    const T *x = reinterpret_cast<const T *>(a.x) + sl.b * a.x_img + sl.c;
-    float s[V], v[V];
+// Running statistics of one thread: count, mean, sum of squares around the mean; W of them with one count
+// (W = 1: the thread's vector lies in one group; else one per channel).
+template <int W>
+struct Running {
+    float n, mean[W], m2[W];
+    // joins a batch of `k` values with mean m and square sum q, k the same for all W
+    __device__ __forceinline__ void join(float k, const float *m, const float *q) {
+        if (n == 0.f) {
+            n = k;
 #pragma unroll
-    for (int i = 0; i < V; i++) s[i] = 0.f;
-    if (sl.valid > 0)
-#pragma unroll 4
-        for (long long r = sl.lo + sl.r; r < sl.hi; r += a.rl) {
-            load<T, VEC>(x + r * a.x_row, sl.valid, v);
-#pragma unroll
-            for (int i = 0; i < V; i++) s[i] += gs_act<PRE>(v[i]);
-        }
-    fold_rows<V>(buf, s, a, sl);
-    fold_groups(gsum, groups, a.cpg, [&](int c) { return buf[c]; });
-    // second pass around the slice's mean; its first moment corrects the mean's own rounding
-    const float inv = 1.0f / ((float)(sl.hi - sl.lo) * (float)a.cpg);
-    float m[V], q[V];
-#pragma unroll
-    for (int i = 0; i < V; i++) {
-        m[i] = i < sl.valid ? gsum[(sl.cv * V + i) / a.cpg] * inv : 0.f;
-        s[i] = q[i] = 0.f;
-    }
-    if (sl.valid > 0)
-#pragma unroll 4
-        for (long long r = sl.lo + sl.r; r < sl.hi; r += a.rl) {
-            load<T, VEC>(x + r * a.x_row, sl.valid, v);
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                const float d = gs_act<PRE>(v[i]) - m[i];
-                s[i] += d;
-                q[i] = fmaf(d, d, q[i]);
+            for (int i = 0; i < W; i++) {
+                mean[i] = m[i];
+                m2[i] = q[i];
             }
+            return;
         }
-    fold_rows<V>(buf, q, a, sl);
-    fold_groups(gsq, groups, a.cpg, [&](int c) { return buf[c]; });
-    fold_rows<V>(buf, s, a, sl);
-    for (int g = threadIdx.x >> 5; g < groups; g += blockDim.x >> 5) {
-        float d = 0.f;
-        for (int c = threadIdx.x & 31; c < a.cpg; c += 32) d += buf[g * a.cpg + c];
+        const float t = n + k, f = k * gs_rcp(t);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-        if ((threadIdx.x & 31) == 0) {
-            float2 *out = reinterpret_cast<float2 *>(a.part) + ((long long)sl.b * a.splits + sl.s) * a.G;
-            out[sl.c0 / a.cpg + g] = make_float2(gsum[g] * inv + d * inv, gsq[g] - d * d * inv);
+        for (int i = 0; i < W; i++) {
+            const float d = m[i] - mean[i];
+            mean[i] = fmaf(d, f, mean[i]);
+            m2[i] = fmaf(d * d, n * f, m2[i] + q[i]);
         }
+        n = t;
+    }
+};
+// One batch of R rows of a vector, already activated
+template <int W, int R>
+__device__ __forceinline__ void take(Running<W> &run, const f2 (*u)[V / 2]) {
+    float m[W], q[W];
+    if (W == 1) {
+        f2 s = u[0][0];
+#pragma unroll
+        for (int k = 1; k < R * V / 2; k++) s = add2(s, u[k / (V / 2)][k % (V / 2)]);
+        m[0] = (s.x + s.y) * (1.0f / (R * V));
+        f2 t = {0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < R * V / 2; k++) {
+            const f2 d = add2(u[k / (V / 2)][k % (V / 2)], both(-m[0]));
+            t = fma2(d, d, t);
+        }
+        q[0] = t.x + t.y;
+        run.join((float)(R * V), m, q);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 2; i++) {
+            f2 s = u[0][i];
+#pragma unroll
+            for (int k = 1; k < R; k++) s = add2(s, u[k][i]);
+            s = mul2(s, both(1.0f / R));
+            f2 t = {0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < R; k++) {
+                const f2 d = fma2(s, both(-1.0f), u[k][i]);
+                t = fma2(d, d, t);
+            }
+            m[2 * i % W] = s.x;
+            m[(2 * i + 1) % W] = s.y;
+            q[2 * i % W] = t.x;
+            q[(2 * i + 1) % W] = t.y;
+        }
+        run.join((float)R, m, q);
     }
 }
 
-// mean and 1 / sqrt(var + eps) of the chunk's groups from the slices' (n, mean, M2), a warp per group
-__device__ __forceinline__ void join_stats(const NormArgs &a, const Slice &sl, float *mean, float *rstd) {
-    const int groups = sl.cc / a.cpg, lane = threadIdx.x & 31;
-    for (int g = threadIdx.x >> 5; g < groups; g += blockDim.x >> 5) {
-        const int gg = sl.c0 / a.cpg + g;
-        const float2 *p = reinterpret_cast<const float2 *>(a.part) + (long long)sl.b * a.splits * a.G + gg;
-        const float m0 = p[0].x;
-        const float inv = 1.0f / (float)a.rows;
-        float d = 0.f;
-        for (int s = lane; s < a.splits; s += 32) {
-            const float n = (float)(a.rows * (s + 1) / a.splits - a.rows * s / a.splits);
-            d = fmaf(n * inv, p[(long long)s * a.G].x - m0, d);
+// Mean and M2 of the slice's groups, W = 1 where a vector lies in one group: emit(group, mean, M2), one lane
+// per group.  KEEP: the activated values also go to `keep`, a place of the thread's own in shared memory.
+template <typename T, bool VEC, int PRE, int W, bool KEEP, typename Emit>
+__device__ __forceinline__ void slice_stats(const NormArgs &a, const Slice &sl, uint8_t *ring, float *buf, float4 *keep,
+                                            Emit emit) {
+    constexpr int R = 4;
+    const int groups = sl.cc / a.cpg, per = W == 1 ? a.cpg / V : a.cpg;
+    float *gmean = buf + MAX_T * W, *gsum = gmean + a.chunk / a.cpg;
+    const Act<PRE> act;
+    Running<W> run;
+    run.n = 0.f;
+#pragma unroll
+    for (int i = 0; i < W; i++) run.mean[i] = run.m2[i] = 0.f;
+    Feed<T, VEC, 1, R, 3> feed;
+    feed.p[0] = reinterpret_cast<const T *>(a.x) + sl.b * a.x_img + sl.c + (sl.lo + sl.r) * a.x_row;
+    feed.step[0] = a.rl * a.x_row;
+    feed.n = sl.rows(a);
+    feed.valid = sl.valid;
+    feed.ring = reinterpret_cast<uint4 *>(ring);
+    feed.start();
+    for (int t = 0; t * R < feed.n; t++) {
+        feed.turn(t);
+        f2 u[R][V / 2];
+#pragma unroll
+        for (int k = 0; k < R; k++) {
+            const int j = t * R + k;
+            if (j >= feed.n) break;
+            unpack8<T>(feed.get(j, 0), u[k]);
+#pragma unroll
+            for (int i = 0; i < V / 2; i++) u[k][i] = act(u[k][i]);
+            if (KEEP) {
+                keep[(2 * j) * (int)blockDim.x + (int)threadIdx.x] = make_float4(u[k][0].x, u[k][0].y, u[k][1].x, u[k][1].y);
+                keep[(2 * j + 1) * (int)blockDim.x + (int)threadIdx.x] = make_float4(u[k][2].x, u[k][2].y, u[k][3].x, u[k][3].y);
+            }
         }
+        if (t * R + R <= feed.n) {
+            take<W, R>(run, u);
+        } else {
+#pragma unroll
+            for (int k = 0; k < R - 1; k++)
+                if (t * R + k < feed.n) take<W, 1>(run, u + k);
+        }
+    }
+    // the slice's group means, then square sums around them; the first moments correct the means' own rounding
+    float v[W], m[W];
+#pragma unroll
+    for (int i = 0; i < W; i++) v[i] = W == 1 || i < sl.valid ? run.n * run.mean[i] : 0.f;
+    const float inv = sl.hi > sl.lo ? 1.0f / ((float)(sl.hi - sl.lo) * (float)a.cpg) : 0.f;
+    fold_rows<W>(buf, v, a, sl);
+    fold_groups(gmean, groups, per, [&](int c) { return buf[c] * inv; });
+#pragma unroll
+    for (int i = 0; i < W; i++) {
+        const bool live = W == 1 ? sl.valid > 0 : i < sl.valid;
+        m[i] = live && run.n > 0.f ? run.mean[i] - gmean[(sl.cv * W + i) / per] : 0.f;
+        v[i] = live ? run.n * m[i] : 0.f;
+    }
+    fold_rows<W>(buf, v, a, sl);
+    fold_groups(gsum, groups, per, [&](int c) { return buf[c]; });
+#pragma unroll
+    for (int i = 0; i < W; i++) v[i] = (W == 1 ? sl.valid > 0 : i < sl.valid) ? fmaf(run.n * m[i], m[i], run.m2[i]) : 0.f;
+    fold_rows<W>(buf, v, a, sl);
+    for (int g = threadIdx.x >> 5; g < groups; g += blockDim.x >> 5) {
+        float q = 0.f;
+        for (int c = threadIdx.x & 31; c < per; c += 32) q += buf[g * per + c];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+        const float d = gsum[g] * inv;
+        if ((threadIdx.x & 31) == 0) emit(g, gmean[g] + d, fmaf(-d, gsum[g], q));
+    }
+}
+
+// ---- forward, first launch
+template <typename T, bool VEC, int PRE, int W>
+__global__ void __launch_bounds__(MAX_T, 2) k_gn_stats(NormArgs a) {
+    extern __shared__ __align__(16) uint8_t dsm[];
+    const Slice sl(a);
+    float2 *out = reinterpret_cast<float2 *>(a.part) + ((long long)sl.b * a.G + sl.c0 / a.cpg) * a.splits + sl.s;
+    slice_stats<T, VEC, PRE, W, false>(a, sl, dsm, reinterpret_cast<float *>(dsm + ring_bytes<T, 1, 4, 3>()), nullptr,
+                                       [&](int g, float mean, float m2) { out[(long long)g * a.splits] = make_float2(mean, m2); });
+}
+
+__device__ __forceinline__ float slice_rows(const NormArgs &a, int s) {
+    return (float)(a.rows * (s + 1) / a.splits - a.rows * s / a.splits);
+}
+// mean and 1 / sqrt(var + eps) of the chunk's groups from the slices' (n, mean, M2), a warp per group: entry s
+// of group g is part[g * gs + s * ss]
+__device__ __forceinline__ void join_stats(const NormArgs &a, const Slice &sl, const float2 *part, int gs, int ss,
+                                           float *mean, float *rstd) {
+    const int groups = sl.cc / a.cpg, lane = threadIdx.x & 31;
+    const float inv = 1.0f / (float)a.rows;
+    for (int g = threadIdx.x >> 5; g < groups; g += blockDim.x >> 5) {
+        const float2 *p = part + (long long)g * gs;
+        const float m0 = p[0].x;
+        // weights n_s / n: the mean first, then the square sums around it
+        float d = 0.f, q = 0.f;
+#pragma unroll 4
+        for (int s = lane; s < a.splits; s += 32) d = fmaf(slice_rows(a, s) * inv, p[s * ss].x - m0, d);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-        const float m = m0 + d;
-        float q = 0.f;
+        d += m0;
+#pragma unroll 4
         for (int s = lane; s < a.splits; s += 32) {
-            const float n = (float)(a.rows * (s + 1) / a.splits - a.rows * s / a.splits);
-            const float2 e = p[(long long)s * a.G];
-            q += fmaf(n * (float)a.cpg * (e.x - m), e.x - m, e.y) * (inv / (float)a.cpg);
+            const float2 e = p[s * ss];
+            const float t = e.x - d;
+            q += fmaf(slice_rows(a, s) * inv * t, t, e.y * (inv / (float)a.cpg));
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
         if (lane == 0) {
-            mean[g] = m;
-            rstd[g] = 1.0f / sqrtf(q + a.eps);
+            mean[g] = d;
+            rstd[g] = 1.0f / sqrtf((q < 0.f ? 0.f : q) + a.eps);
             if (sl.s == 0 && a.stats)
-                reinterpret_cast<float2 *>(a.stats)[(long long)sl.b * a.G + gg] = make_float2(m, rstd[g]);
+                reinterpret_cast<float2 *>(a.stats)[(long long)sl.b * a.G + sl.c0 / a.cpg + g] = make_float2(d, rstd[g]);
         }
     }
     __syncthreads();
 }
 
+// A thread's coefficients of the map: y = act((u + m) k + b), m the negative mean
+template <typename T>
+struct Map {
+    f2 m[V / 2], k[V / 2], b[V / 2];
+    __device__ __forceinline__ Map(const NormArgs &a, const Slice &sl, const float *mean, const float *rstd) {
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const int c = sl.c + min(i, sl.valid - 1), g = (c - sl.c0) / a.cpg;
+            at(m, i) = -mean[g];
+            at(k, i) = rstd[g] * (a.w ? param<T>(a.w, a.param_f32, c) : 1.f);
+            at(b, i) = a.b ? param<T>(a.b, a.param_f32, c) : 0.f;
+        }
+    }
+    __device__ __forceinline__ f2 operator()(f2 u, int i) const { return fma2(add2(u, m[i]), k[i], b[i]); }
+};
+
 // ---- forward, second launch: the map
 template <typename T, bool VEC, int PRE, int POST>
-__global__ void __launch_bounds__(MAX_T) k_gn_map(NormArgs a) {
-    constexpr int V = Vec<T>::N;
-    extern __shared__ float sm[];
-    const Slice sl(a, V);
-    float *mean = sm, *rstd = sm + a.chunk / a.cpg;
-    join_stats(a, sl, mean, rstd);
-    if (sl.valid <= 0) return;
-    float m[V], k[V], b[V], v[V];
+__global__ void __launch_bounds__(MAX_T, 2) k_gn_map(NormArgs a) {
+    constexpr int B = 2;
+    extern __shared__ __align__(16) uint8_t dsm[];
+    const Slice sl(a);
+    float *mean = reinterpret_cast<float *>(dsm + ring_bytes<T, 1, B, 4>()), *rstd = mean + a.chunk / a.cpg;
+    // from the end of the slice: L2 holds what the first launch read last
+    Feed<T, VEC, 1, B, 4> feed;
+    feed.n = sl.rows(a);
+    const long long last = sl.lo + sl.r + (long long)(feed.n - 1) * a.rl;
+    feed.p[0] = reinterpret_cast<const T *>(a.x) + sl.b * a.x_img + sl.c + last * a.x_row;
+    feed.step[0] = -a.rl * a.x_row;
+    feed.valid = sl.valid;
+    feed.ring = reinterpret_cast<uint4 *>(dsm);
+    feed.start();
+    join_stats(a, sl, reinterpret_cast<const float2 *>(a.part) + ((long long)sl.b * a.G + sl.c0 / a.cpg) * a.splits,
+               a.splits, 1, mean, rstd);
+    if (feed.n == 0) return;
+    const Map<T> map(a, sl, mean, rstd);
+    const Act<PRE> pre;
+    const Act<POST> post;
+    T *y = reinterpret_cast<T *>(a.y) + (sl.b * a.rows + last) * a.C + sl.c;
+    const long long ystep = -(long long)a.rl * a.C;
+    for (int t = 0; t * B < feed.n; t++) {
+        feed.turn(t);
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        const int c = sl.c + min(i, sl.valid - 1), g = (c - sl.c0) / a.cpg;
-        m[i] = mean[g];
-        k[i] = rstd[g] * (a.w ? param<T>(a.w, a.param_f32, c) : 1.f);
-        b[i] = a.b ? param<T>(a.b, a.param_f32, c) : 0.f;
-    }
-    const T *x = reinterpret_cast<const T *>(a.x) + sl.b * a.x_img + sl.c;
-    T *y = reinterpret_cast<T *>(a.y) + sl.b * a.rows * a.C + sl.c;
-#pragma unroll 4
-    for (long long r = sl.lo + sl.r; r < sl.hi; r += a.rl) {
-        load<T, VEC>(x + r * a.x_row, sl.valid, v);
+        for (int k = 0; k < B; k++) {
+            const int j = t * B + k;
+            if (j >= feed.n) break;
+            f2 u[V / 2];
+            unpack8<T>(feed.get(j, 0), u);
 #pragma unroll
-        for (int i = 0; i < V; i++) v[i] = gs_act<POST>(fmaf(gs_act<PRE>(v[i]) - m[i], k[i], b[i]));
-        store<T, VEC>(y + r * a.C, sl.valid, v);
+            for (int i = 0; i < V / 2; i++) u[i] = post(map(pre(u[i]), i));
+            store<T, VEC>(y + j * ystep, sl.valid, u);
+        }
     }
 }
 
-// xh, and dz from dy, of one element; w, b are read only where the activation comes after
-template <int PRE, int POST>
-__device__ __forceinline__ void grad_of(float x, float dy, float m, float rs, float w, float b, float &xh, float &dz) {
-    xh = (gs_act<PRE>(x) - m) * rs;
-    dz = POST ? dy * gs_act_slope<POST>(fmaf(xh, w, b)) : dy;
+// writes v to the place of this CTA's shared address p in rank `rank` of the cluster
+__device__ __forceinline__ void put(const float2 *p, int rank, float2 v) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                 : "=r"(a)
+                 : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(a), "f"(v.x), "f"(v.y) : "memory");
 }
 
-// ---- backward, first launch: channel sums of dz and dz xh, and their group sums weighted by w
-template <typename T, bool VEC, int PRE, int POST>
-__global__ void __launch_bounds__(MAX_T) k_gn_grad_sums(NormArgs a) {
-    constexpr int V = Vec<T>::N;
-    extern __shared__ float sm[];
-    const Slice sl(a, V);
-    const int groups = sl.cc / a.cpg, w = a.cvec * V;
-    float *buf = sm, *g0 = sm + (size_t)a.rl * w, *g1 = g0 + a.chunk / a.cpg;
-    float sz[V], sx[V];
+// ---- forward in one launch: the CTAs of a cluster hold one image's chunk of groups in shared memory,
+// activated, in fp32.  Slices are the cluster's ranks; every rank gets all ranks' (mean, M2) and joins them alike.
+template <typename T, int PRE, int POST, int W>
+__global__ void __launch_bounds__(MAX_T, 1) k_gn_fused(NormArgs a) {
+    extern __shared__ __align__(16) uint8_t dsm[];
+    const Slice sl(a, true);
+    const int gmax = a.chunk / a.cpg;
+    float4 *keep = reinterpret_cast<float4 *>(dsm + ring_bytes<T, 1, 4, 3>());
+    float *buf = reinterpret_cast<float *>(keep + 2 * a.held * MAX_T);
+    float *mean = buf + MAX_T * W + 2 * gmax, *rstd = mean + gmax;
+    float2 *all = reinterpret_cast<float2 *>(rstd + gmax);  // [ranks][gmax]
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    slice_stats<T, true, PRE, W, true>(a, sl, dsm, buf, keep, [&](int g, float m, float m2) {
+        all[sl.s * gmax + g] = make_float2(m, m2);
+    });
+    __syncthreads();
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every rank runs: its memory may be written
+    for (int t = threadIdx.x; t < gmax * a.splits; t += blockDim.x) {
+        const int rank = t / gmax, at = sl.s * gmax + t - rank * gmax;
+        if (rank != sl.s && t - rank * gmax < sl.cc / a.cpg) put(all + at, rank, all[at]);
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    join_stats(a, sl, all, 1, gmax, mean, rstd);
+    const int n = sl.rows(a);
+    if (n == 0) return;
+    const Map<T> map(a, sl, mean, rstd);
+    const Act<POST> post;
+    T *y = reinterpret_cast<T *>(a.y) + (sl.b * a.rows + sl.lo + sl.r) * a.C + sl.c;
+#pragma unroll 2
+    for (int k = 0; k < n; k++) {
+        const float4 p = keep[(2 * k) * (int)blockDim.x + (int)threadIdx.x], q = keep[(2 * k + 1) * (int)blockDim.x + (int)threadIdx.x];
+        f2 u[V / 2] = {{p.x, p.y}, {p.z, p.w}, {q.x, q.y}, {q.z, q.w}};
 #pragma unroll
-    for (int i = 0; i < V; i++) sz[i] = sx[i] = 0.f;
-    if (sl.valid > 0) {
-        float m[V], rs[V], wt[V], bs[V], v[V], d[V];
+        for (int i = 0; i < V / 2; i++) u[i] = post(map(u[i], i));
+        store<T, true>(y + (long long)k * a.rl * a.C, V, u);
+    }
+}
+
+// A thread's coefficients of the backward: statistics and parameters of its channels.  SLOPE: the first
+// activation's slope too, for dx.
+template <typename T, int PRE, int POST, bool SLOPE>
+struct Grad {
+    Act<PRE, SLOPE> pre;
+    Act<POST, true> post;
+    f2 m[V / 2], rs[V / 2], w[V / 2], b[V / 2];
+    __device__ __forceinline__ Grad(const NormArgs &a, const Slice &sl) {
 #pragma unroll
         for (int i = 0; i < V; i++) {
             const int c = sl.c + min(i, sl.valid - 1);
             const float2 st = reinterpret_cast<const float2 *>(a.stats)[(long long)sl.b * a.G + c / a.cpg];
-            m[i] = st.x;
-            rs[i] = st.y;
-            wt[i] = a.w ? param<T>(a.w, a.param_f32, c) : 1.f;
-            bs[i] = a.b ? param<T>(a.b, a.param_f32, c) : 0.f;
+            at(m, i) = -st.x;
+            at(rs, i) = st.y;
+            at(w, i) = a.w ? param<T>(a.w, a.param_f32, c) : 1.f;
+            at(b, i) = a.b ? param<T>(a.b, a.param_f32, c) : 0.f;
         }
-        const T *x = reinterpret_cast<const T *>(a.x) + sl.b * a.x_img + sl.c;
-        const T *dy = reinterpret_cast<const T *>(a.dy) + sl.b * a.dy_img + sl.c;
-#pragma unroll 2
-        for (long long r = sl.lo + sl.r; r < sl.hi; r += a.rl) {
-            load<T, VEC>(x + r * a.x_row, sl.valid, v);
-            load<T, VEC>(dy + r * a.dy_row, sl.valid, d);
+    }
+    // xh and dz of one pair
+    __device__ __forceinline__ f2 operator()(f2 x, f2 dy, int i, f2 &xh, f2 &slope) const {
+        const f2 u = SLOPE ? pre(x, slope) : pre(x);
+        xh = mul2(add2(u, m[i]), rs[i]);
+        if (POST == ACT_NONE) return dy;
+        f2 s;
+        post(fma2(xh, w[i], b[i]), s);
+        return mul2(dy, s);
+    }
+};
+
+// ---- backward, first launch: channel sums of dz and dz xh, and their group sums weighted by w
+template <typename T, bool VEC, int PRE, int POST>
+__global__ void __launch_bounds__(MAX_T, 2) k_gn_grad_sums(NormArgs a) {
+    extern __shared__ __align__(16) uint8_t dsm[];
+    const Slice sl(a);
+    const int groups = sl.cc / a.cpg;
+    float *buf = reinterpret_cast<float *>(dsm + ring_bytes<T, 2, 1, 8>()), *g0 = buf + MAX_T * V,
+          *g1 = g0 + a.chunk / a.cpg;
+    f2 sz[V / 2], sx[V / 2];
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                float xh, dz;
-                grad_of<PRE, POST>(v[i], d[i], m[i], rs[i], wt[i], bs[i], xh, dz);
-                sz[i] += dz;
-                sx[i] = fmaf(dz, xh, sx[i]);
+    for (int i = 0; i < V / 2; i++) sz[i] = sx[i] = both(0.f);
+    Feed<T, VEC, 2, 1, 8> feed;
+    feed.n = sl.rows(a);
+    feed.p[0] = reinterpret_cast<const T *>(a.x) + sl.b * a.x_img + sl.c + (sl.lo + sl.r) * a.x_row;
+    feed.p[1] = reinterpret_cast<const T *>(a.dy) + sl.b * a.dy_img + sl.c + (sl.lo + sl.r) * a.dy_row;
+    feed.step[0] = a.rl * a.x_row;
+    feed.step[1] = a.rl * a.dy_row;
+    feed.valid = sl.valid;
+    feed.ring = reinterpret_cast<uint4 *>(dsm);
+    feed.start();
+    if (feed.n > 0) {
+        const Grad<T, PRE, POST, false> grad(a, sl);
+        for (int t = 0; t < feed.n; t++) {
+            feed.turn(t);
+            f2 v[V / 2], d[V / 2];
+            unpack8<T>(feed.get(t, 0), v);
+            unpack8<T>(feed.get(t, 1), d);
+#pragma unroll
+            for (int i = 0; i < V / 2; i++) {
+                f2 xh, none;
+                const f2 dz = grad(v[i], d[i], i, xh, none);
+                sz[i] = add2(sz[i], dz);
+                sx[i] = fma2(dz, xh, sx[i]);
             }
         }
     }
     float2 *cp = reinterpret_cast<float2 *>(a.cpart) + ((long long)sl.b * a.splits + sl.s) * a.C;
-    float2 *gp = reinterpret_cast<float2 *>(a.part) + ((long long)sl.b * a.splits + sl.s) * a.G + sl.c0 / a.cpg;
+    float2 *gp = reinterpret_cast<float2 *>(a.part) + ((long long)sl.b * a.G + sl.c0 / a.cpg) * a.splits + sl.s;
     auto weight = [&](int c) { return a.w ? param<T>(a.w, a.param_f32, sl.c0 + c) : 1.f; };
-    fold_rows<V>(buf, sz, a, sl);
+    float v[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) v[i] = i < sl.valid ? at(sz, i) : 0.f;
+    fold_rows<V>(buf, v, a, sl);
     for (int c = threadIdx.x; c < sl.cc; c += blockDim.x) cp[sl.c0 + c].x = buf[c];
     fold_groups(g0, groups, a.cpg, [&](int c) { return buf[c] * weight(c); });
-    fold_rows<V>(buf, sx, a, sl);
+#pragma unroll
+    for (int i = 0; i < V; i++) v[i] = i < sl.valid ? at(sx, i) : 0.f;
+    fold_rows<V>(buf, v, a, sl);
     for (int c = threadIdx.x; c < sl.cc; c += blockDim.x) cp[sl.c0 + c].y = buf[c];
     fold_groups(g1, groups, a.cpg, [&](int c) { return buf[c] * weight(c); });
-    for (int g = threadIdx.x; g < groups; g += blockDim.x) gp[g] = make_float2(g0[g], g1[g]);
+    for (int g = threadIdx.x; g < groups; g += blockDim.x) gp[(long long)g * a.splits] = make_float2(g0[g], g1[g]);
 }
 
 // ---- backward, second launch: dx; the blocks after the slices' fold the channel sums into dw and db
 template <typename T, bool VEC, int PRE, int POST>
-__global__ void __launch_bounds__(MAX_T) k_gn_grad_map(NormArgs a) {
-    constexpr int V = Vec<T>::N;
-    extern __shared__ float sm[];
+__global__ void __launch_bounds__(MAX_T, 2) k_gn_grad_map(NormArgs a) {
+    extern __shared__ __align__(16) uint8_t dsm[];
+    float *sm = reinterpret_cast<float *>(dsm + ring_bytes<T, 2, 1, 8>());
     if ((int)blockIdx.x >= a.nslice) {
         // 32 channels per block, the (image, split) sums dealt to the warps, joined in order
         float2 *red = reinterpret_cast<float2 *>(sm);
@@ -317,7 +617,7 @@ __global__ void __launch_bounds__(MAX_T) k_gn_grad_map(NormArgs a) {
         const float2 *cp = reinterpret_cast<const float2 *>(a.cpart);
         float2 t = make_float2(0.f, 0.f);
         if (c < a.C)
-#pragma unroll 4
+#pragma unroll 8
             for (int k = threadIdx.x >> 5; k < a.B * a.splits; k += nw) {
                 const float2 e = cp[(long long)k * a.C + c];
                 t.x += e.x;
@@ -335,15 +635,27 @@ __global__ void __launch_bounds__(MAX_T) k_gn_grad_map(NormArgs a) {
         }
         return;
     }
-    const Slice sl(a, V);
+    const Slice sl(a);
     const int groups = sl.cc / a.cpg;
     float *g0 = sm, *g1 = sm + a.chunk / a.cpg;
+    // from the end of the slice, as the forward's map
+    Feed<T, VEC, 2, 1, 8> feed;
+    feed.n = sl.rows(a);
+    const long long last = sl.lo + sl.r + (long long)(feed.n - 1) * a.rl;
+    feed.p[0] = reinterpret_cast<const T *>(a.x) + sl.b * a.x_img + sl.c + last * a.x_row;
+    feed.p[1] = reinterpret_cast<const T *>(a.dy) + sl.b * a.dy_img + sl.c + last * a.dy_row;
+    feed.step[0] = -a.rl * a.x_row;
+    feed.step[1] = -a.rl * a.dy_row;
+    feed.valid = sl.valid;
+    feed.ring = reinterpret_cast<uint4 *>(dsm);
+    feed.start();
     const float inv = 1.0f / ((float)a.rows * (float)a.cpg);
     for (int g = threadIdx.x >> 5; g < groups; g += blockDim.x >> 5) {
-        const float2 *p = reinterpret_cast<const float2 *>(a.part) + (long long)sl.b * a.splits * a.G + sl.c0 / a.cpg + g;
+        const float2 *p = reinterpret_cast<const float2 *>(a.part) + ((long long)sl.b * a.G + sl.c0 / a.cpg + g) * a.splits;
         float s0 = 0.f, s1 = 0.f;
+#pragma unroll 4
         for (int s = threadIdx.x & 31; s < a.splits; s += 32) {
-            const float2 e = p[(long long)s * a.G];
+            const float2 e = p[s];
             s0 += e.x;
             s1 += e.y;
         }
@@ -358,34 +670,30 @@ __global__ void __launch_bounds__(MAX_T) k_gn_grad_map(NormArgs a) {
         }
     }
     __syncthreads();
-    if (sl.valid <= 0) return;
-    float m[V], rs[V], wt[V], bs[V], m0[V], m1[V], v[V], d[V];
+    if (feed.n == 0) return;
+    const Grad<T, PRE, POST, true> grad(a, sl);
+    f2 m0[V / 2], m1[V / 2];
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        const int c = sl.c + min(i, sl.valid - 1), g = (c - sl.c0) / a.cpg;
-        const float2 st = reinterpret_cast<const float2 *>(a.stats)[(long long)sl.b * a.G + c / a.cpg];
-        m[i] = st.x;
-        rs[i] = st.y;
-        wt[i] = a.w ? param<T>(a.w, a.param_f32, c) : 1.f;
-        bs[i] = a.b ? param<T>(a.b, a.param_f32, c) : 0.f;
-        m0[i] = g0[g];
-        m1[i] = g1[g];
+        const int g = (sl.c + min(i, sl.valid - 1) - sl.c0) / a.cpg;
+        at(m0, i) = -g0[g];
+        at(m1, i) = -g1[g];
     }
-    const T *x = reinterpret_cast<const T *>(a.x) + sl.b * a.x_img + sl.c;
-    const T *dy = reinterpret_cast<const T *>(a.dy) + sl.b * a.dy_img + sl.c;
-    T *dx = reinterpret_cast<T *>(a.dx) + sl.b * a.rows * a.C + sl.c;
-#pragma unroll 2
-    for (long long r = sl.lo + sl.r; r < sl.hi; r += a.rl) {
-        load<T, VEC>(x + r * a.x_row, sl.valid, v);
-        load<T, VEC>(dy + r * a.dy_row, sl.valid, d);
+    T *dx = reinterpret_cast<T *>(a.dx) + (sl.b * a.rows + last) * a.C + sl.c;
+    const long long ystep = -(long long)a.rl * a.C;
+    for (int t = 0; t < feed.n; t++) {
+        feed.turn(t);
+        f2 v[V / 2], d[V / 2];
+        unpack8<T>(feed.get(t, 0), v);
+        unpack8<T>(feed.get(t, 1), d);
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            float xh, dz;
-            grad_of<PRE, POST>(v[i], d[i], m[i], rs[i], wt[i], bs[i], xh, dz);
-            const float du = rs[i] * (fmaf(wt[i], dz, -m0[i]) - xh * m1[i]);
-            v[i] = PRE ? du * gs_act_slope<PRE>(v[i]) : du;
+        for (int i = 0; i < V / 2; i++) {
+            f2 xh, slope;
+            const f2 dz = grad(v[i], d[i], i, xh, slope);
+            const f2 du = mul2(grad.rs[i], fma2(xh, m1[i], fma2(grad.w[i], dz, m0[i])));
+            v[i] = PRE ? mul2(du, slope) : du;
         }
-        store<T, VEC>(dx + r * a.C, sl.valid, v);
+        store<T, VEC>(dx + t * ystep, sl.valid, v);
     }
 }
 
@@ -395,6 +703,15 @@ int elem_size(int dtype) { return dtype == GS_F32 ? 4 : 2; }
 constexpr int SMS = 148;  // of a B200: the split of the work, and with it the workspace, is a matter of sizes alone
 
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
+
+// Chunks of whole groups and whole vectors, of at least `want` channels.
+void chunks(NormArgs &a, int want) {
+    const int unit = a.cpg / gcd(a.cpg, V) * V;
+    const int n = (want + unit - 1) / unit * unit;
+    a.chunk = n < a.C ? n : a.C;
+    a.nchunk = (a.C + a.chunk - 1) / a.chunk;
+    a.cvec = (a.chunk + V - 1) / V;
+}
 
 // Fills sizes and the split of the work; false for arguments outside the operator's range.
 bool plan(const gs_norm_desc *d, NormArgs &a) {
@@ -407,29 +724,38 @@ bool plan(const gs_norm_desc *d, NormArgs &a) {
     a.x_row = d->x_row; a.x_img = d->x_img; a.dy_row = d->dy_row; a.dy_img = d->dy_img;
     a.param_f32 = d->param_dtype == GS_F32;
     a.eps = d->eps;
-    const int V = 16 / elem_size(d->dtype);
     // many groups: a block takes whole groups of about 64 channels (128 contiguous bytes a row in 16 bits), so
     // the second launch joins only those groups' sums
-    a.chunk = a.C;
-    if (a.G > 32) {
-        const int unit = a.cpg / gcd(a.cpg, V) * V;  // whole groups and whole vectors
-        const int want = (64 + unit - 1) / unit * unit;
-        if (want < a.C) a.chunk = want;
-    }
-    a.nchunk = (a.C + a.chunk - 1) / a.chunk;
-    a.cvec = (a.chunk + V - 1) / V;
-    a.rl = std::max(1, 256 / a.cvec);
-    // four blocks of 256 threads per SM, but no fewer than four rows a thread
+    chunks(a, a.G > 32 ? 64 : a.C);
+    a.rl = std::max(1, MAX_T / a.cvec);
+    // one wave of two blocks per SM, but no fewer than four rows a thread
     const long long most = std::max<long long>(1, a.rows / (4LL * a.rl));
-    const long long want = std::max<long long>(1, 4LL * SMS / std::max<long long>(1, (long long)a.B * a.nchunk));
-    a.splits = (int)std::min({most, want, 1024LL});
+    const long long want = std::max<long long>(1, 2LL * SMS / std::max<long long>(1, (long long)a.B * a.nchunk));
+    a.splits = (int)std::max(std::min(most, want), a.rows >> 30);
+    return (long long)a.B * a.splits * a.nchunk < (1LL << 30);
+}
+
+// The one-launch form's split: chunks of whole groups of at least 64 contiguous bytes a row, over a cluster of
+// as few CTAs as hold them, or as many (to 8) as find SMs idle.  False where 16 CTAs do not hold a chunk.
+bool fused_plan(const gs_norm_desc *d, NormArgs &a) {
+    if (a.C % V) return false;
+    chunks(a, 64 / elem_size(d->dtype));
+    a.rl = MAX_T / a.cvec;
+    long long n = 1;
+    while (n <= 16 && (a.rows + n - 1) / n > (long long)a.rl * FUSED_R) n *= 2;
+    if (n > 16) return false;
+    while (n < 8 && (long long)a.B * a.nchunk * n * 2 <= SMS && a.rows / (2 * n) >= a.rl) n *= 2;
+    a.splits = (int)n;
+    const int most = (int)((a.rows + n - 1) / n);
+    a.rl = std::min(a.rl, most);
+    a.held = (most + a.rl - 1) / a.rl;
     return (long long)a.B * a.splits * a.nchunk < (1LL << 30);
 }
 
 size_t al(size_t n) { return (n + 255) & ~(size_t)255; }
 size_t part_bytes(const NormArgs &a) { return al((size_t)a.B * a.splits * a.G * 8); }
 
-bool aligned(const void *p, long long row, long long img, int V) {
+bool aligned(const void *p, long long row, long long img) {
     return ((uintptr_t)p & 15) == 0 && row % V == 0 && img % V == 0;
 }
 
@@ -443,31 +769,61 @@ int done(const char *where) {
 }
 
 int threads(const NormArgs &a) { return (a.rl * a.cvec + 31) / 32 * 32; }
-// shared memory of the kernels that fold sums, and of those that only join group values
-template <typename T>
-size_t fold_smem(const NormArgs &a) {
-    return ((size_t)a.rl * a.cvec * Vec<T>::N + 2 * (size_t)(a.chunk / a.cpg)) * sizeof(float);
-}
-size_t join_smem(const NormArgs &a) {
-    return std::max<size_t>(2 * (size_t)(a.chunk / a.cpg) * sizeof(float), (size_t)MAX_T * sizeof(float2));
+template <typename K>
+int launch(K kern, unsigned grid, const NormArgs &a, size_t smem, cudaStream_t s, const char *where) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return done(where);
+    kern<<<grid, threads(a), smem, s>>>(a);
+    gs_count_launch(1);
+    return done(where);
 }
 
+constexpr const char *FWD = "gs_group_norm_act_fwd", *BWD_ = "gs_group_norm_act_bwd";
+
+template <typename T, int PRE, int POST>
+int forward_fused(const NormArgs &a, cudaStream_t s) {
+    const int W = a.cpg % V == 0 ? 1 : V;
+    auto kern = W == 1 ? k_gn_fused<T, PRE, POST, 1> : k_gn_fused<T, PRE, POST, V>;
+    if (a.splits > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+        return done(FWD);
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = a.splits;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t c;
+    memset(&c, 0, sizeof(c));
+    c.gridDim = dim3((unsigned)(a.B * a.splits * a.nchunk));
+    c.blockDim = dim3(threads(a));
+    c.dynamicSmemBytes = ring_bytes<T, 1, 4, 3>() + (size_t)2 * a.held * MAX_T * sizeof(float4) +
+                         ((size_t)MAX_T * W + (4 + 2 * (size_t)a.splits) * (a.chunk / a.cpg)) * sizeof(float);
+    c.stream = s;
+    c.attrs = at;
+    c.numAttrs = 1;
+    if (c.dynamicSmemBytes > 48 * 1024 &&
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)c.dynamicSmemBytes) != cudaSuccess)
+        return done(FWD);
+    cudaLaunchKernelEx(&c, kern, a);
+    gs_count_launch(1);
+    return done(FWD);
+}
 template <typename T, bool VEC, int PRE, int POST>
 int forward(const NormArgs &a, cudaStream_t s) {
+    if (a.fused) return forward_fused<T, PRE, POST>(a, s);
     const unsigned grid = (unsigned)(a.B * a.splits * a.nchunk);
-    k_gn_stats<T, VEC, PRE><<<grid, threads(a), fold_smem<T>(a), s>>>(a);
-    k_gn_map<T, VEC, PRE, POST><<<grid, threads(a), join_smem(a), s>>>(a);
-    gs_count_launch(2);
-    return done("gs_group_norm_act_fwd");
+    const size_t groups = 2 * (size_t)(a.chunk / a.cpg) * sizeof(float);
+    const int W = a.cpg % V == 0 ? 1 : V;
+    const int st = launch(W == 1 ? k_gn_stats<T, VEC, PRE, 1> : k_gn_stats<T, VEC, PRE, V>, grid, a,
+                          ring_bytes<T, 1, 4, 3>() + MAX_T * W * sizeof(float) + groups, s, FWD);
+    return st != GS_OK ? st : launch(k_gn_map<T, VEC, PRE, POST>, grid, a, ring_bytes<T, 1, 2, 4>() + groups, s, FWD);
 }
 template <typename T, bool VEC, int PRE, int POST>
 int backward(const NormArgs &a, cudaStream_t s) {
     const unsigned grid = (unsigned)(a.B * a.splits * a.nchunk), fold = a.dw || a.db ? (a.C + 31) / 32 : 0;
+    const size_t groups = 2 * (size_t)(a.chunk / a.cpg) * sizeof(float), ring = ring_bytes<T, 2, 1, 8>();
     if (a.nslice + fold == 0) return GS_OK;
-    k_gn_grad_sums<T, VEC, PRE, POST><<<grid, threads(a), fold_smem<T>(a), s>>>(a);
-    k_gn_grad_map<T, VEC, PRE, POST><<<a.nslice + fold, threads(a), join_smem(a), s>>>(a);
-    gs_count_launch(2);
-    return done("gs_group_norm_act_bwd");
+    const int st = launch(k_gn_grad_sums<T, VEC, PRE, POST>, grid, a, ring + MAX_T * V * sizeof(float) + groups, s, BWD_);
+    return st != GS_OK ? st
+                       : launch(k_gn_grad_map<T, VEC, PRE, POST>, a.nslice + fold, a,
+                                ring + std::max(groups, MAX_T * sizeof(float2)), s, BWD_);
 }
 
 template <bool BWD, typename T, bool VEC>
@@ -506,8 +862,12 @@ extern "C" int gs_group_norm_act_fwd(const gs_norm_desc *d, const void *x, const
     if (!workspace || workspace_bytes < gs_group_norm_act_workspace_size(d, 0)) return GS_ERR_WORKSPACE;
     a.x = x; a.w = weight; a.b = bias; a.y = y; a.stats = stats;
     a.part = reinterpret_cast<float *>(al((uintptr_t)workspace));
-    const int V = 16 / elem_size(d->dtype);
-    const bool vec = aligned(x, a.x_row, a.x_img, V) && aligned(y, a.C, 0, V);
+    const bool vec = aligned(x, a.x_row, a.x_img) && aligned(y, a.C, 0);
+    NormArgs f = a;
+    if (vec && fused_plan(d, f)) {
+        a = f;
+        a.fused = 1;
+    }
     return by_type<false>(d, a, vec, (cudaStream_t)stream);
 }
 
@@ -529,7 +889,6 @@ extern "C" int gs_group_norm_act_bwd(const gs_norm_desc *d, const void *x, const
     a.nslice = dx ? a.B * a.splits * a.nchunk : 0;
     a.part = reinterpret_cast<float *>(al((uintptr_t)workspace));
     a.cpart = reinterpret_cast<float *>(reinterpret_cast<char *>(a.part) + part_bytes(a));
-    const int V = 16 / elem_size(d->dtype);
-    const bool vec = aligned(x, a.x_row, a.x_img, V) && aligned(dy, a.dy_row, a.dy_img, V) && (!dx || aligned(dx, a.C, 0, V));
+    const bool vec = aligned(x, a.x_row, a.x_img) && aligned(dy, a.dy_row, a.dy_img) && (!dx || aligned(dx, a.C, 0));
     return by_type<true>(d, a, vec, (cudaStream_t)stream);
 }

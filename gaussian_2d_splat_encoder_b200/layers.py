@@ -25,6 +25,7 @@ from . import _lib
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTS = {"none": 0, "gelu": 1, "silu": 2}
+_NO_WORKSPACE = 256  # a linear call whose size query answers this needs none
 
 
 class _NormDesc(C.Structure):
@@ -56,20 +57,13 @@ def _dtype_code(name, t):
     return _DTYPES[t.dtype]
 
 
-def _scope(dev):
-    """The tensors' device made current; the usual case, already current, costs nothing."""
-    return _NO_SCOPE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+def _elsewhere(dev):
+    """Whether another device than the tensors' is current (the call is then repeated under a switch)."""
+    return torch.cuda.current_device() != dev.index
 
 
-class _NoScope:
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_NO_SCOPE = _NoScope()
+# the handle of a device's current stream, without the Stream object around it
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _rows_of(t, first):
@@ -111,49 +105,61 @@ def _image_layout(t):
 
 
 def _norm_forward(x, weight, bias, groups, eps, act, act_first, train):
+    dev = x.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _norm_forward(x, weight, bias, groups, eps, act, act_first, train)
     x, x_row, x_img = _image_layout(x)
+    shape = x.shape
+    B, channels = shape[0], shape[-1]
     p = weight if weight is not None else bias
-    key = (x.shape[0], x.numel() // (x.shape[0] * x.shape[-1]), x.shape[-1], groups, _DTYPES[x.dtype],
-           0 if p is None else _DTYPES[p.dtype], act, act_first, eps, x_row, x_img)
+    key = (B, x.numel() // (B * channels), channels, groups, _DTYPES[x.dtype], 0 if p is None else _DTYPES[p.dtype],
+           act, act_first, eps, x_row, x_img)
     desc, nbytes, _, _ = _norm_plan(*key, 0, 0)
     if nbytes == 0:
-        raise ValueError(f"unsupported sizes: {tuple(x.shape)} in {groups} groups")
+        raise ValueError(f"unsupported sizes: {tuple(shape)} in {groups} groups")
+    y = x.new_empty(shape)
+    # one buffer: the statistics the backward reads (8 bytes per image and group), then the workspace
+    head = (B * groups * 8 + 255) // 256 * 256 if train else 0
+    buf = x.new_empty(head + nbytes, dtype=torch.uint8)
+    at = buf.data_ptr()
+    _lib.check(_lib.load().gs_group_norm_act_fwd(desc, x.data_ptr(), None if weight is None else weight.data_ptr(),
+                                                 None if bias is None else bias.data_ptr(), y.data_ptr(),
+                                                 at if train else None, at + head, nbytes, _raw_stream(dev.index)),
+               "gs_group_norm_act_fwd")
+    return y, x, buf, key
+
+
+def _norm_backward(ctx, dy):
+    x, weight, bias, buf = ctx.saved_tensors
     dev = x.device
-    with _scope(dev):
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float32, device=dev) if train else None
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        ptr = _lib.ptr
-        _lib.check(_lib.load().gs_group_norm_act_fwd(desc, ptr(x), ptr(weight), ptr(bias), ptr(y), ptr(stats), ptr(ws),
-                                                     nbytes, _lib.stream_of(dev)), "gs_group_norm_act_fwd")
-    return y, x, stats, key
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _norm_backward(ctx, dy)
+    need = ctx.needs_input_grad
+    dy, dy_row, dy_img = _image_layout(dy)
+    desc, _, nbytes, _ = _norm_plan(*ctx.key, dy_row, dy_img)
+    dx = x.new_empty(x.shape) if need[0] else None
+    dw = weight.new_empty(weight.shape) if need[1] else None
+    db = bias.new_empty(bias.shape) if need[2] else None
+    ws = x.new_empty(nbytes, dtype=torch.uint8)
+    _lib.check(_lib.load().gs_group_norm_act_bwd(desc, x.data_ptr(), None if weight is None else weight.data_ptr(),
+                                                 None if bias is None else bias.data_ptr(), buf.data_ptr(),
+                                                 dy.data_ptr(), None if dx is None else dx.data_ptr(),
+                                                 None if dw is None else dw.data_ptr(),
+                                                 None if db is None else db.data_ptr(), ws.data_ptr(), nbytes,
+                                                 _raw_stream(dev.index)), "gs_group_norm_act_bwd")
+    return dx, dw, db, None, None, None, None
 
 
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act, act_first):
-        y, x, stats, ctx.key = _norm_forward(x, weight, bias, groups, eps, act, act_first, True)
-        ctx.save_for_backward(x, weight, bias, stats)
+        y, x, buf, ctx.key = _norm_forward(x, weight, bias, groups, eps, act, act_first, True)
+        ctx.save_for_backward(x, weight, bias, buf)
         return y
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias, stats = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dy, dy_row, dy_img = _image_layout(dy)
-        desc, _, nbytes, _ = _norm_plan(*ctx.key, dy_row, dy_img)
-        dev = x.device
-        with _scope(dev):
-            dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
-            dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if need[1] else None
-            db = torch.empty_like(bias, memory_format=torch.contiguous_format) if need[2] else None
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            ptr = _lib.ptr
-            _lib.check(_lib.load().gs_group_norm_act_bwd(desc, ptr(x), ptr(weight), ptr(bias), ptr(stats), ptr(dy),
-                                                         ptr(dx), ptr(dw), ptr(db), ptr(ws), nbytes,
-                                                         _lib.stream_of(dev)), "gs_group_norm_act_bwd")
-        return dx, dw, db, None, None, None, None
+    backward = staticmethod(once_differentiable(_norm_backward))
 
 
 def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None,
@@ -221,30 +227,61 @@ def _row_layout(t):
 
 
 def _linear_forward(x, weight, bias, residual, act, train):
+    dev = x.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _linear_forward(x, weight, bias, residual, act, train)
     x, ldx = _row_layout(x)
     weight, ldw = _row_layout(weight)
     ldr = 0
     if residual is not None:
         residual, ldr = _row_layout(residual)
     N, K = weight.shape
-    unaligned = bool(x.data_ptr() & 15) | bool(weight.data_ptr() & 15) << 1
+    px, pw = x.data_ptr(), weight.data_ptr()
+    unaligned = (1 if px & 15 else 0) | (2 if pw & 15 else 0)
     key = (x.numel() // K, N, K, _DTYPES[x.dtype], act, ldx, ldw)
     desc, nbytes, _, _ = _linear_plan(*key, ldr, 0, unaligned)
     if nbytes == 0:
         raise ValueError(f"unsupported sizes: {tuple(x.shape)} and {tuple(weight.shape)}")
-    dev = x.device
-    with _scope(dev):
-        shape = x.shape[:-1] + (N,)
-        y = torch.empty(shape, dtype=x.dtype, device=dev)
+    shape = x.shape[:-1] + (N,)
+    y = x.new_empty(shape)
+    slope = None
+    if train and act:
         # the activation's slope, as the backward takes it: fp32, or 16-bit fixed point
-        slope = torch.empty(shape, dtype=x.dtype if x.dtype == torch.float32 else torch.int16,
-                            device=dev) if train and act else None
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        ptr = _lib.ptr
-        _lib.check(_lib.load().gs_linear_act_fwd(desc, ptr(x), ptr(weight), ptr(bias), ptr(residual), ptr(y),
-                                                 ptr(slope), ptr(ws), nbytes, _lib.stream_of(dev)),
-                   "gs_linear_act_fwd")
+        slope = x.new_empty(shape, dtype=torch.float32 if x.dtype == torch.float32 else torch.int16)
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes > _NO_WORKSPACE else None
+    _lib.check(_lib.load().gs_linear_act_fwd(desc, px, pw, None if bias is None else bias.data_ptr(),
+                                             None if residual is None else residual.data_ptr(), y.data_ptr(),
+                                             None if slope is None else slope.data_ptr(),
+                                             None if ws is None else ws.data_ptr(), nbytes, _raw_stream(dev.index)),
+               "gs_linear_act_fwd")
     return y, x, weight, slope, key + (unaligned,)
+
+
+def _linear_backward(ctx, dy):
+    x, weight, slope = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    if not (need[0] or need[1] or need[2]):
+        return None, None, None, dy if need[3] else None, None
+    dev = x.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _linear_backward(ctx, dy)
+    g, ldy = _row_layout(dy)
+    *key, unaligned = ctx.key
+    pg = g.data_ptr()
+    desc, _, nbytes, _ = _linear_plan(*key, 0, ldy, unaligned | (4 if pg & 15 else 0))
+    dx = x.new_empty(x.shape) if need[0] else None
+    dw = weight.new_empty(weight.shape) if need[1] else None
+    db = weight.new_empty(weight.shape[0]) if need[2] else None
+    ws = x.new_empty(nbytes, dtype=torch.uint8)
+    _lib.check(_lib.load().gs_linear_act_bwd(desc, x.data_ptr(), weight.data_ptr(),
+                                             None if slope is None else slope.data_ptr(), pg,
+                                             None if dx is None else dx.data_ptr(),
+                                             None if dw is None else dw.data_ptr(),
+                                             None if db is None else db.data_ptr(), ws.data_ptr(), nbytes,
+                                             _raw_stream(dev.index)), "gs_linear_act_bwd")
+    return dx, dw, db, dy if need[3] else None, None
 
 
 class _LinearAct(torch.autograd.Function):
@@ -254,27 +291,7 @@ class _LinearAct(torch.autograd.Function):
         ctx.save_for_backward(x, weight, slope)
         return y
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, slope = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx = dw = db = None
-        if need[0] or need[1] or need[2]:
-            g, ldy = _row_layout(dy)
-            *key, unaligned = ctx.key
-            desc, _, nbytes, _ = _linear_plan(*key, 0, ldy, unaligned | bool(g.data_ptr() & 15) << 2)
-            dev = x.device
-            with _scope(dev):
-                dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
-                dw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if need[1] else None
-                db = torch.empty(weight.shape[0], dtype=x.dtype, device=dev) if need[2] else None
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-                ptr = _lib.ptr
-                _lib.check(_lib.load().gs_linear_act_bwd(desc, ptr(x), ptr(weight), ptr(slope), ptr(g), ptr(dx),
-                                                         ptr(dw), ptr(db), ptr(ws), nbytes, _lib.stream_of(dev)),
-                           "gs_linear_act_bwd")
-        return dx, dw, db, dy if need[3] else None, None
+    backward = staticmethod(once_differentiable(_linear_backward))
 
 
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, act: str = "none",

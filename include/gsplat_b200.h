@@ -294,7 +294,8 @@ typedef struct {
                               the workspace); a less aligned pointer without its bit is refused */
 } gs_linear_desc;
 
-/* Workspace bytes of a forward (backward = 0) or a backward (1) call; 0 for an invalid descriptor. */
+/* Workspace bytes of a forward (backward = 0) or a backward (1) call; 0 for an invalid descriptor, 256 where the
+ * call needs none (workspace may then be NULL). */
 size_t gs_linear_act_workspace_size(const gs_linear_desc *d, int backward);
 /* bias, residual and slope may be NULL; slope [M][N] (2 bytes an element for 16-bit types, else 4) receives
  * the activation's slope for the backward, in the library's own encoding; not written without an activation. */

@@ -68,7 +68,10 @@ def test_linear_workspace_and_refusals(lib, ops):
         assert lib.gs_linear_act_fwd(C.byref(d), p, p, None, p, p, None, p, 1 << 30, None) == 2, bad
     assert lib.gs_linear_act_bwd(C.byref(linear_desc(ops, ldy=31)), p, p, p, p, p, p, p, p, 1 << 30, None) == 2
     d = linear_desc(ops)
-    assert lib.gs_linear_act_fwd(C.byref(d), p, p, None, None, p, None, p, 16, None) == 5
+    need = linear_desc(ops, K=63, ldx=63)  # x is kept padded
+    assert size(C.byref(d), 0) == 256 < size(C.byref(need), 0)
+    assert lib.gs_linear_act_fwd(C.byref(need), p, p, None, None, p, None, p, 16, None) == 5
+    assert lib.gs_linear_act_fwd(C.byref(need), p, p, None, None, p, None, None, 1 << 30, None) == 5
     assert lib.gs_linear_act_bwd(C.byref(d), p, p, p, p, p, p, p, p, 16, None) == 5
     q = C.c_void_p(264)  # off 16 bytes, without the descriptor's bit
     assert lib.gs_linear_act_fwd(C.byref(d), q, p, None, None, p, None, p, 1 << 40, None) == 2
