@@ -30,34 +30,10 @@ __device__ __forceinline__ float gs_gelu(float x) {
     return 0.5f * x * (x >= 0.f ? 2.0f - q : q);
 }
 // ---- the layer kernels' forms, on pairs (fma.rn.f32x2: the FMA pipe's rate at half the issue slots)
-struct f2 {
-    float x, y;
-};
-__device__ __forceinline__ unsigned long long f2_bits(f2 v) {
-    unsigned long long r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
-    return r;
-}
-__device__ __forceinline__ f2 f2_of(unsigned long long r) {
-    f2 v;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
-    return v;
-}
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-    unsigned long long r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)), "l"(f2_bits(c)));
-    return f2_of(r);
-}
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
-    unsigned long long r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
-    return f2_of(r);
-}
-__device__ __forceinline__ f2 add2(f2 a, f2 b) {
-    unsigned long long r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
-    return f2_of(r);
-}
+using f2 = float2;
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) { return __fadd2_rn(a, b); }
 __device__ __forceinline__ f2 both(float v) { return {v, v}; }
 
 enum { ACT_NONE = 0, ACT_GELU = 1, ACT_SILU = 2 };  // gs_activation

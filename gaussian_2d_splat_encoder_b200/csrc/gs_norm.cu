@@ -38,7 +38,7 @@ namespace {
 
 constexpr int MAX_T = 256;  // threads of a block
 constexpr int V = 8;        // channels of a thread's vector
-constexpr int FUSED_R = 16; // most vectors a thread of the one-launch form holds
+constexpr int FUSED_T = 512, FUSED_R = 12;  // one-launch form: threads, most vectors a thread holds
 
 struct NormArgs {
     const void *x, *dy, *w, *b;
@@ -46,7 +46,8 @@ struct NormArgs {
     float *stats;   // [B][G][2] mean, 1 / sqrt(var + eps)
     float *part;    // forward [B][splits][G][2] mean, M2; backward the two group sums
     float *cpart;   // backward [B][splits][C][2] channel sums of dz and dz xh
-    long long rows, x_row, x_img, dy_row, dy_img;
+    long long x_row, x_img, dy_row, dy_img;
+    int rows, per;  // rows of an image, of a slice
     int B, C, G, cpg, splits;
     int chunk, nchunk, cvec, rl;  // channels per block, blocks over channels, vectors per row, rows in flight
     int nslice;                   // blocks of the backward's second launch that map slices
@@ -94,9 +95,9 @@ __device__ __forceinline__ void store(T *p, int valid, const f2 *v) {
 
 // The slice of a block and the place of a thread in it.
 struct Slice {
-    int b, s, c0, cc;   // image, split, first channel, channels of this chunk
+    int b, s, c0, cc;     // image, split, first channel, channels of this chunk
     int r, cv, c, valid;  // row lane, vector, its first channel, its channels (<= 0: idle thread)
-    long long lo, hi;   // rows
+    int lo, hi;           // rows
     __device__ Slice(const NormArgs &a, bool cluster = false) {
         int t = blockIdx.x, k;
         if (cluster) {  // the splits of a chunk are neighbours
@@ -116,14 +117,24 @@ struct Slice {
         cv = (int)threadIdx.x - r * a.cvec;
         c = c0 + cv * V;
         valid = r < a.rl ? min(V, cc - cv * V) : 0;
-        lo = a.rows * s / a.splits;
-        hi = a.rows * (s + 1) / a.splits;
+        lo = s * a.per;
+        hi = min(lo + a.per, a.rows);
     }
     // rows of this thread: lo + r, lo + r + rl, ...
-    __device__ int rows(const NormArgs &a) const {
-        return valid > 0 && lo + r < hi ? (int)((hi - 1 - lo - r) / a.rl) + 1 : 0;
-    }
+    __device__ int rows(const NormArgs &a) const { return valid > 0 && r < hi - lo ? (hi - 1 - lo - r) / a.rl + 1 : 0; }
 };
+// f(i, group of channel i) for a thread's channels, groups counted from the chunk's first
+template <typename F>
+__device__ __forceinline__ void each_channel(const NormArgs &a, const Slice &sl, F f) {
+    const int g = (sl.c - sl.c0) / a.cpg;
+    if (a.cpg % V == 0) {
+#pragma unroll
+        for (int i = 0; i < V; i++) f(i, g);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) f(i, (sl.c - sl.c0 + min(i, sl.valid - 1)) / a.cpg);
+    }
+}
 
 // A thread's rows of S tensors, fed through a ring of its own in shared memory: NB batches of B rows, cp.async
 // keeps NB - 1 of them in flight without holding registers.  Unaligned rows are read in place.
@@ -135,31 +146,48 @@ template <int N>
 __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
+// NB, a power of two, so a batch's place is a mask away and a row's an immediate offset from it
 template <typename T>
-constexpr int ring_batches(int batches) {  // fp32 rows are twice as wide
-    return sizeof(T) == 4 ? (batches + 1) / 2 : batches;
+constexpr int ring_batches() {
+    return sizeof(T) == 4 ? 2 : 4;  // fp32 rows are twice as wide
 }
-template <typename T, bool VEC, int S, int B, int BATCHES>
+template <typename T, bool VEC, int S, int B, bool KEEP = false>
 struct Feed {
-    static constexpr int NB = ring_batches<T>(BATCHES);
-    const T *p[S];
-    long long step[S];
-    int n, valid;  // rows of this thread
-    uint4 *ring;
-    __device__ __forceinline__ uint4 *slot(int j, int s, int q) const {
-        return ring + ((j % (NB * B) * S + s) * ((int)sizeof(T) / 2) + q) * (int)blockDim.x + (int)threadIdx.x;
+    // KEEP: room for all rows, as fp32
+    static constexpr int NB = KEEP ? FUSED_R / B : ring_batches<T>();
+    static constexpr int threads() { return KEEP ? FUSED_T : MAX_T; }
+    static constexpr int pieces() { return KEEP ? 2 : (int)sizeof(T) / 2; }
+    static constexpr int place(int batch) { return KEEP ? batch : batch & (NB - 1); }
+    static constexpr int row() { return S * pieces() * threads(); }  // 16-byte pieces of one row of all threads
+    const T *next[S], *here[S];  // of the next batch to issue; unaligned: of the batch to read
+    long long step[S];           // row to row
+    int n, valid;                // rows of this thread
+    uint4 *ring;                 // + this thread
+
+    __device__ __forceinline__ Feed(uint8_t *smem, int rows, int valid_) : n(rows), valid(valid_) {
+        ring = reinterpret_cast<uint4 *>(smem) + threadIdx.x;
+    }
+    __device__ __forceinline__ void tensor(int s, const T *p, long long st) {
+        next[s] = here[s] = p;
+        step[s] = st;
     }
     __device__ __forceinline__ void issue(int batch) {
         if constexpr (VEC) {
+            uint4 *const to = ring + place(batch) * (B * row());
+            const int left = n - batch * B;
 #pragma unroll
-            for (int k = 0; k < B; k++) {
-                const int j = batch * B + k;
-                if (j < n)
+            for (int s = 0; s < S; s++) {
+                const T *p = next[s];
 #pragma unroll
-                    for (int s = 0; s < S; s++)
+                for (int k = 0; k < B; k++) {
+                    if (k < left)
 #pragma unroll
                         for (int q = 0; q < (int)sizeof(T) / 2; q++)
-                            cp_async16(slot(j, s, q), reinterpret_cast<const uint4 *>(p[s] + j * step[s]) + q);
+                            cp_async16(to + k * row() + (s * pieces() + q) * threads(),
+                                       reinterpret_cast<const uint4 *>(p) + q);
+                    p += step[s];
+                }
+                next[s] = p;
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
@@ -173,57 +201,72 @@ struct Feed {
         issue(t + NB - 1);
         if (VEC) cp_async_wait<NB - 1>();
     }
-    __device__ __forceinline__ Raw8<T> get(int j, int s) const {
+    // row k of batch t
+    __device__ __forceinline__ Raw8<T> get(int t, int k, int s) const {
         if constexpr (VEC) {
+            const uint4 *const from = ring + place(t) * (B * row()) + k * row() + s * pieces() * threads();
             Raw8<T> r;
 #pragma unroll
-            for (int q = 0; q < (int)sizeof(T) / 2; q++) r.q[q] = *slot(j, s, q);
+            for (int q = 0; q < (int)sizeof(T) / 2; q++) r.q[q] = from[q * threads()];
             return r;
         } else {
-            return fetch<T, false>(p[s] + j * step[s], valid);
+            return fetch<T, false>(here[s] + (long long)(t * B + k) * step[s], valid);
         }
     }
 };
-template <typename T, int S, int B, int BATCHES>
+template <typename T, int S, int B>
 constexpr size_t ring_bytes() {
-    return (size_t)ring_batches<T>(BATCHES) * B * S * V * sizeof(T) * MAX_T;
+    return (size_t)ring_batches<T>() * B * S * V * sizeof(T) * MAX_T;
 }
 
-// Sums over the row lanes of W values per thread (0 from idle ones): buf[0..cvec*W) holds the result.  Within
-// a warp by shuffles where its lanes' vectors repeat evenly, across rows or warps in a fixed order.
+// Sums over the row lanes of W values per thread (0 from idle ones): entry cv * W + i of the returned array, in
+// buf[0..2 W threads).  Where a warp's lanes repeat the vectors evenly: by shuffles, then over the warps.  Else
+// one plane per value in shared memory, its rows dealt to as many threads as there are, their parts added in order.
 template <int W>
-__device__ __forceinline__ void fold_rows(float *buf, float *v, const NormArgs &a, const Slice &sl) {
-    const int w = a.cvec * W;
+__device__ __forceinline__ const float *fold_rows(float *buf, float *v, const NormArgs &a, const Slice &sl) {
+    const int w = a.cvec * W, T = blockDim.x;
     __syncthreads();
     if (32 % a.cvec == 0) {
         for (int o = a.cvec; o < 32; o <<= 1)
 #pragma unroll
             for (int i = 0; i < W; i++) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = T >> 5;
         if (lane < a.cvec)
 #pragma unroll
             for (int i = 0; i < W; i++) buf[warp * w + lane * W + i] = v[i];
         __syncthreads();
-        for (int k = threadIdx.x; k < w; k += blockDim.x) {
+        for (int k = threadIdx.x; k < w; k += T) {
             float s = buf[k];
             for (int q = 1; q < nw; q++) s += buf[q * w + k];
             buf[k] = s;
         }
-    } else {
-        if (sl.r < a.rl)
+        __syncthreads();
+        return buf;
+    }
+    const int plane = a.rl * a.cvec;
+    if (sl.r < a.rl)
 #pragma unroll
-            for (int i = 0; i < W; i++) buf[sl.r * w + sl.cv * W + i] = v[i];
-        int n = a.rl;
-        while (n > 1) {
-            const int h = (n + 1) >> 1;
-            __syncthreads();
-            if (sl.r < n - h)
-#pragma unroll
-                for (int i = 0; i < W; i++) buf[sl.r * w + sl.cv * W + i] += buf[(sl.r + h) * w + sl.cv * W + i];
-            n = h;
-        }
+        for (int i = 0; i < W; i++) buf[i * plane + threadIdx.x] = v[i];
+    __syncthreads();
+    float *const out = buf + W * T;
+    const int parts = max(1, min(T / w, a.rl));
+    for (int t = threadIdx.x; t < parts * w; t += T) {
+        const int part = t / w, o = t - part * w, i = o / a.cvec, cv = o - i * a.cvec;
+        float s = 0.f;
+#pragma unroll 4
+        for (int r = part; r < a.rl; r += parts) s += buf[i * plane + r * a.cvec + cv];
+        out[parts > 1 ? t : cv * W + i] = s;
     }
     __syncthreads();
+    if (parts == 1) return out;
+    for (int o = threadIdx.x; o < w; o += T) {
+        float s = out[o];
+        for (int part = 1; part < parts; part++) s += out[part * w + o];
+        const int i = o / a.cvec, cv = o - i * a.cvec;
+        buf[cv * W + i] = s;
+    }
+    __syncthreads();
+    return buf;
 }
 // Sums over each group's `per` consecutive entries, a warp per group; f gives an entry.
 template <typename F>
@@ -304,69 +347,65 @@ __device__ __forceinline__ void take(Running<W> &run, const f2 (*u)[V / 2]) {
 }
 
 // Mean and M2 of the slice's groups, W = 1 where a vector lies in one group: emit(group, mean, M2), one lane
-// per group.  KEEP: the activated values also go to `keep`, a place of the thread's own in shared memory.
+// per group.  KEEP: the ring holds all rows, and the activated values
+// replace them there.
 template <typename T, bool VEC, int PRE, int W, bool KEEP, typename Emit>
-__device__ __forceinline__ void slice_stats(const NormArgs &a, const Slice &sl, uint8_t *ring, float *buf, float4 *keep,
-                                            Emit emit) {
-    constexpr int R = 4;
+__device__ __forceinline__ void slice_stats(const NormArgs &a, const Slice &sl, uint8_t *ring, float *buf, Emit emit) {
+    constexpr int R = 2, THREADS = KEEP ? FUSED_T : MAX_T;
     const int groups = sl.cc / a.cpg, per = W == 1 ? a.cpg / V : a.cpg;
-    float *gmean = buf + MAX_T * W, *gsum = gmean + a.chunk / a.cpg;
+    float *gmean = buf + 2 * THREADS * W, *gsum = gmean + a.chunk / a.cpg;
     const Act<PRE> act;
     Running<W> run;
     run.n = 0.f;
 #pragma unroll
     for (int i = 0; i < W; i++) run.mean[i] = run.m2[i] = 0.f;
-    Feed<T, VEC, 1, R, 3> feed;
-    feed.p[0] = reinterpret_cast<const T *>(a.x) + sl.b * a.x_img + sl.c + (sl.lo + sl.r) * a.x_row;
-    feed.step[0] = a.rl * a.x_row;
-    feed.n = sl.rows(a);
-    feed.valid = sl.valid;
-    feed.ring = reinterpret_cast<uint4 *>(ring);
+    Feed<T, VEC, 1, R, KEEP> feed(ring, sl.rows(a), sl.valid);
+    feed.tensor(0, reinterpret_cast<const T *>(a.x) + sl.b * a.x_img + sl.c + (long long)(sl.lo + sl.r) * a.x_row, a.rl * a.x_row);
     feed.start();
-    for (int t = 0; t * R < feed.n; t++) {
+    auto value = [&](int t, int k, f2 *u) {
+        unpack8<T>(feed.get(t, k, 0), u);
+#pragma unroll
+        for (int i = 0; i < V / 2; i++) u[i] = act(u[i]);
+        if (KEEP) {
+            float4 *to = reinterpret_cast<float4 *>(ring) + threadIdx.x + (t * R + k) * 2 * THREADS;
+            to[0] = make_float4(u[0].x, u[0].y, u[1].x, u[1].y);
+            to[THREADS] = make_float4(u[2].x, u[2].y, u[3].x, u[3].y);
+        }
+    };
+    int t = 0;
+    f2 u[R][V / 2];
+    for (; t * R + R <= feed.n; t++) {
         feed.turn(t);
-        f2 u[R][V / 2];
 #pragma unroll
-        for (int k = 0; k < R; k++) {
-            const int j = t * R + k;
-            if (j >= feed.n) break;
-            unpack8<T>(feed.get(j, 0), u[k]);
-#pragma unroll
-            for (int i = 0; i < V / 2; i++) u[k][i] = act(u[k][i]);
-            if (KEEP) {
-                keep[(2 * j) * (int)blockDim.x + (int)threadIdx.x] = make_float4(u[k][0].x, u[k][0].y, u[k][1].x, u[k][1].y);
-                keep[(2 * j + 1) * (int)blockDim.x + (int)threadIdx.x] = make_float4(u[k][2].x, u[k][2].y, u[k][3].x, u[k][3].y);
-            }
-        }
-        if (t * R + R <= feed.n) {
-            take<W, R>(run, u);
-        } else {
-#pragma unroll
-            for (int k = 0; k < R - 1; k++)
-                if (t * R + k < feed.n) take<W, 1>(run, u + k);
-        }
+        for (int k = 0; k < R; k++) value(t, k, u[k]);
+        take<W, R>(run, u);
+    }
+    feed.turn(t);
+    for (int k = 0; t * R + k < feed.n; k++) {
+        value(t, k, u[0]);
+        take<W, 1>(run, u);
     }
     // the slice's group means, then square sums around them; the first moments correct the means' own rounding
     float v[W], m[W];
 #pragma unroll
     for (int i = 0; i < W; i++) v[i] = W == 1 || i < sl.valid ? run.n * run.mean[i] : 0.f;
     const float inv = sl.hi > sl.lo ? 1.0f / ((float)(sl.hi - sl.lo) * (float)a.cpg) : 0.f;
-    fold_rows<W>(buf, v, a, sl);
-    fold_groups(gmean, groups, per, [&](int c) { return buf[c] * inv; });
+    const float *f = fold_rows<W>(buf, v, a, sl);
+    fold_groups(gmean, groups, per, [&](int c) { return f[c] * inv; });
 #pragma unroll
     for (int i = 0; i < W; i++) {
         const bool live = W == 1 ? sl.valid > 0 : i < sl.valid;
         m[i] = live && run.n > 0.f ? run.mean[i] - gmean[(sl.cv * W + i) / per] : 0.f;
         v[i] = live ? run.n * m[i] : 0.f;
     }
-    fold_rows<W>(buf, v, a, sl);
-    fold_groups(gsum, groups, per, [&](int c) { return buf[c]; });
+    f = fold_rows<W>(buf, v, a, sl);
+    fold_groups(gsum, groups, per, [&](int c) { return f[c]; });
 #pragma unroll
     for (int i = 0; i < W; i++) v[i] = (W == 1 ? sl.valid > 0 : i < sl.valid) ? fmaf(run.n * m[i], m[i], run.m2[i]) : 0.f;
-    fold_rows<W>(buf, v, a, sl);
+    f = fold_rows<W>(buf, v, a, sl);
     for (int g = threadIdx.x >> 5; g < groups; g += blockDim.x >> 5) {
         float q = 0.f;
-        for (int c = threadIdx.x & 31; c < per; c += 32) q += buf[g * per + c];
+        for (int c = threadIdx.x & 31; c < per; c += 32) q += f[g * per + c];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
         const float d = gsum[g] * inv;
@@ -376,16 +415,16 @@ __device__ __forceinline__ void slice_stats(const NormArgs &a, const Slice &sl, 
 
 // ---- forward, first launch
 template <typename T, bool VEC, int PRE, int W>
-__global__ void __launch_bounds__(MAX_T, 2) k_gn_stats(NormArgs a) {
+__global__ void __launch_bounds__(MAX_T, W == 1 ? 3 : 2) k_gn_stats(NormArgs a) {
     extern __shared__ __align__(16) uint8_t dsm[];
     const Slice sl(a);
     float2 *out = reinterpret_cast<float2 *>(a.part) + ((long long)sl.b * a.G + sl.c0 / a.cpg) * a.splits + sl.s;
-    slice_stats<T, VEC, PRE, W, false>(a, sl, dsm, reinterpret_cast<float *>(dsm + ring_bytes<T, 1, 4, 3>()), nullptr,
+    slice_stats<T, VEC, PRE, W, false>(a, sl, dsm, reinterpret_cast<float *>(dsm + ring_bytes<T, 1, 2>()),
                                        [&](int g, float mean, float m2) { out[(long long)g * a.splits] = make_float2(mean, m2); });
 }
 
 __device__ __forceinline__ float slice_rows(const NormArgs &a, int s) {
-    return (float)(a.rows * (s + 1) / a.splits - a.rows * s / a.splits);
+    return (float)max(0, min(a.per, a.rows - s * a.per));
 }
 // mean and 1 / sqrt(var + eps) of the chunk's groups from the slices' (n, mean, M2), a warp per group: entry s
 // of group g is part[g * gs + s * ss]
@@ -426,54 +465,53 @@ template <typename T>
 struct Map {
     f2 m[V / 2], k[V / 2], b[V / 2];
     __device__ __forceinline__ Map(const NormArgs &a, const Slice &sl, const float *mean, const float *rstd) {
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-            const int c = sl.c + min(i, sl.valid - 1), g = (c - sl.c0) / a.cpg;
+        each_channel(a, sl, [&](int i, int g) {
+            const int c = sl.c + min(i, sl.valid - 1);
             at(m, i) = -mean[g];
             at(k, i) = rstd[g] * (a.w ? param<T>(a.w, a.param_f32, c) : 1.f);
             at(b, i) = a.b ? param<T>(a.b, a.param_f32, c) : 0.f;
-        }
+        });
     }
     __device__ __forceinline__ f2 operator()(f2 u, int i) const { return fma2(add2(u, m[i]), k[i], b[i]); }
 };
 
 // ---- forward, second launch: the map
 template <typename T, bool VEC, int PRE, int POST>
-__global__ void __launch_bounds__(MAX_T, 2) k_gn_map(NormArgs a) {
+__global__ void __launch_bounds__(MAX_T, 3) k_gn_map(NormArgs a) {
     constexpr int B = 2;
     extern __shared__ __align__(16) uint8_t dsm[];
     const Slice sl(a);
-    float *mean = reinterpret_cast<float *>(dsm + ring_bytes<T, 1, B, 4>()), *rstd = mean + a.chunk / a.cpg;
+    float *mean = reinterpret_cast<float *>(dsm + ring_bytes<T, 1, B>()), *rstd = mean + a.chunk / a.cpg;
     // from the end of the slice: L2 holds what the first launch read last
-    Feed<T, VEC, 1, B, 4> feed;
-    feed.n = sl.rows(a);
-    const long long last = sl.lo + sl.r + (long long)(feed.n - 1) * a.rl;
-    feed.p[0] = reinterpret_cast<const T *>(a.x) + sl.b * a.x_img + sl.c + last * a.x_row;
-    feed.step[0] = -a.rl * a.x_row;
-    feed.valid = sl.valid;
-    feed.ring = reinterpret_cast<uint4 *>(dsm);
+    const int n = sl.rows(a);
+    const long long last = sl.lo + sl.r + (long long)(n - 1) * a.rl;
+    Feed<T, VEC, 1, B> feed(dsm, n, sl.valid);
+    feed.tensor(0, reinterpret_cast<const T *>(a.x) + sl.b * a.x_img + sl.c + last * a.x_row, -a.rl * a.x_row);
     feed.start();
     join_stats(a, sl, reinterpret_cast<const float2 *>(a.part) + ((long long)sl.b * a.G + sl.c0 / a.cpg) * a.splits,
                a.splits, 1, mean, rstd);
-    if (feed.n == 0) return;
+    if (n == 0) return;
     const Map<T> map(a, sl, mean, rstd);
     const Act<PRE> pre;
     const Act<POST> post;
-    T *y = reinterpret_cast<T *>(a.y) + (sl.b * a.rows + last) * a.C + sl.c;
+    T *y = reinterpret_cast<T *>(a.y) + ((long long)sl.b * a.rows + last) * a.C + sl.c;
     const long long ystep = -(long long)a.rl * a.C;
-    for (int t = 0; t * B < feed.n; t++) {
+    auto one = [&](int t, int k) {
+        f2 u[V / 2];
+        unpack8<T>(feed.get(t, k, 0), u);
+#pragma unroll
+        for (int i = 0; i < V / 2; i++) u[i] = post(map(pre(u[i]), i));
+        store<T, VEC>(y, sl.valid, u);
+        y += ystep;
+    };
+    int t = 0;
+    for (; t * B + B <= n; t++) {
         feed.turn(t);
 #pragma unroll
-        for (int k = 0; k < B; k++) {
-            const int j = t * B + k;
-            if (j >= feed.n) break;
-            f2 u[V / 2];
-            unpack8<T>(feed.get(j, 0), u);
-#pragma unroll
-            for (int i = 0; i < V / 2; i++) u[i] = post(map(pre(u[i]), i));
-            store<T, VEC>(y + j * ystep, sl.valid, u);
-        }
+        for (int k = 0; k < B; k++) one(t, k);
     }
+    feed.turn(t);
+    for (int k = 0; t * B + k < n; k++) one(t, k);
 }
 
 // writes v to the place of this CTA's shared address p in rank `rank` of the cluster
@@ -487,19 +525,17 @@ __device__ __forceinline__ void put(const float2 *p, int rank, float2 v) {
 
 // ---- forward in one launch: the CTAs of a cluster hold one image's chunk of groups in shared memory,
 // activated, in fp32.  Slices are the cluster's ranks; every rank gets all ranks' (mean, M2) and joins them alike.
+__host__ __device__ constexpr size_t held_bytes(int rows) { return (size_t)rows * 32 * FUSED_T; }  // [row][half][thread]
 template <typename T, int PRE, int POST, int W>
-__global__ void __launch_bounds__(MAX_T, 1) k_gn_fused(NormArgs a) {
+__global__ void __launch_bounds__(FUSED_T, 1) k_gn_fused(NormArgs a) {
     extern __shared__ __align__(16) uint8_t dsm[];
     const Slice sl(a, true);
     const int gmax = a.chunk / a.cpg;
-    float4 *keep = reinterpret_cast<float4 *>(dsm + ring_bytes<T, 1, 4, 3>());
-    float *buf = reinterpret_cast<float *>(keep + 2 * a.held * MAX_T);
-    float *mean = buf + MAX_T * W + 2 * gmax, *rstd = mean + gmax;
+    float *buf = reinterpret_cast<float *>(dsm + held_bytes(a.held)), *mean = buf + 2 * FUSED_T * W + 2 * gmax, *rstd = mean + gmax;
     float2 *all = reinterpret_cast<float2 *>(rstd + gmax);  // [ranks][gmax]
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-    slice_stats<T, true, PRE, W, true>(a, sl, dsm, buf, keep, [&](int g, float m, float m2) {
-        all[sl.s * gmax + g] = make_float2(m, m2);
-    });
+    slice_stats<T, true, PRE, W, true>(a, sl, dsm, buf,
+                                       [&](int g, float m, float m2) { all[sl.s * gmax + g] = make_float2(m, m2); });
     __syncthreads();
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every rank runs: its memory may be written
     for (int t = threadIdx.x; t < gmax * a.splits; t += blockDim.x) {
@@ -512,10 +548,11 @@ __global__ void __launch_bounds__(MAX_T, 1) k_gn_fused(NormArgs a) {
     if (n == 0) return;
     const Map<T> map(a, sl, mean, rstd);
     const Act<POST> post;
-    T *y = reinterpret_cast<T *>(a.y) + (sl.b * a.rows + sl.lo + sl.r) * a.C + sl.c;
+    T *y = reinterpret_cast<T *>(a.y) + ((long long)sl.b * a.rows + sl.lo + sl.r) * a.C + sl.c;
+    const float4 *keep = reinterpret_cast<const float4 *>(dsm) + threadIdx.x;
 #pragma unroll 2
     for (int k = 0; k < n; k++) {
-        const float4 p = keep[(2 * k) * (int)blockDim.x + (int)threadIdx.x], q = keep[(2 * k + 1) * (int)blockDim.x + (int)threadIdx.x];
+        const float4 p = keep[2 * k * FUSED_T], q = keep[(2 * k + 1) * FUSED_T];
         f2 u[V / 2] = {{p.x, p.y}, {p.z, p.w}, {q.x, q.y}, {q.z, q.w}};
 #pragma unroll
         for (int i = 0; i < V / 2; i++) u[i] = post(map(u[i], i));
@@ -531,15 +568,14 @@ struct Grad {
     Act<POST, true> post;
     f2 m[V / 2], rs[V / 2], w[V / 2], b[V / 2];
     __device__ __forceinline__ Grad(const NormArgs &a, const Slice &sl) {
-#pragma unroll
-        for (int i = 0; i < V; i++) {
+        const float2 *st = reinterpret_cast<const float2 *>(a.stats) + (long long)sl.b * a.G + sl.c0 / a.cpg;
+        each_channel(a, sl, [&](int i, int g) {
             const int c = sl.c + min(i, sl.valid - 1);
-            const float2 st = reinterpret_cast<const float2 *>(a.stats)[(long long)sl.b * a.G + c / a.cpg];
-            at(m, i) = -st.x;
-            at(rs, i) = st.y;
+            at(m, i) = -st[g].x;
+            at(rs, i) = st[g].y;
             at(w, i) = a.w ? param<T>(a.w, a.param_f32, c) : 1.f;
             at(b, i) = a.b ? param<T>(a.b, a.param_f32, c) : 0.f;
-        }
+        });
     }
     // xh and dz of one pair
     __device__ __forceinline__ f2 operator()(f2 x, f2 dy, int i, f2 &xh, f2 &slope) const {
@@ -554,31 +590,29 @@ struct Grad {
 
 // ---- backward, first launch: channel sums of dz and dz xh, and their group sums weighted by w
 template <typename T, bool VEC, int PRE, int POST>
-__global__ void __launch_bounds__(MAX_T, 2) k_gn_grad_sums(NormArgs a) {
+__global__ void __launch_bounds__(MAX_T, 3) k_gn_grad_sums(NormArgs a) {
     extern __shared__ __align__(16) uint8_t dsm[];
     const Slice sl(a);
     const int groups = sl.cc / a.cpg;
-    float *buf = reinterpret_cast<float *>(dsm + ring_bytes<T, 2, 1, 8>()), *g0 = buf + MAX_T * V,
+    // (the sums fold in the ring's place, drained by then)
+    static_assert(ring_bytes<T, 2, 2>() >= 2 * MAX_T * V * sizeof(float), "room to fold");
+    float *buf = reinterpret_cast<float *>(dsm), *g0 = reinterpret_cast<float *>(dsm + ring_bytes<T, 2, 2>()),
           *g1 = g0 + a.chunk / a.cpg;
     f2 sz[V / 2], sx[V / 2];
 #pragma unroll
     for (int i = 0; i < V / 2; i++) sz[i] = sx[i] = both(0.f);
-    Feed<T, VEC, 2, 1, 8> feed;
-    feed.n = sl.rows(a);
-    feed.p[0] = reinterpret_cast<const T *>(a.x) + sl.b * a.x_img + sl.c + (sl.lo + sl.r) * a.x_row;
-    feed.p[1] = reinterpret_cast<const T *>(a.dy) + sl.b * a.dy_img + sl.c + (sl.lo + sl.r) * a.dy_row;
-    feed.step[0] = a.rl * a.x_row;
-    feed.step[1] = a.rl * a.dy_row;
-    feed.valid = sl.valid;
-    feed.ring = reinterpret_cast<uint4 *>(dsm);
+    constexpr int B = 2;
+    const int n = sl.rows(a);
+    Feed<T, VEC, 2, B> feed(dsm, n, sl.valid);
+    feed.tensor(0, reinterpret_cast<const T *>(a.x) + sl.b * a.x_img + sl.c + (long long)(sl.lo + sl.r) * a.x_row, a.rl * a.x_row);
+    feed.tensor(1, reinterpret_cast<const T *>(a.dy) + sl.b * a.dy_img + sl.c + (long long)(sl.lo + sl.r) * a.dy_row, a.rl * a.dy_row);
     feed.start();
-    if (feed.n > 0) {
+    if (n > 0) {
         const Grad<T, PRE, POST, false> grad(a, sl);
-        for (int t = 0; t < feed.n; t++) {
-            feed.turn(t);
+        auto one = [&](int t, int k) {
             f2 v[V / 2], d[V / 2];
-            unpack8<T>(feed.get(t, 0), v);
-            unpack8<T>(feed.get(t, 1), d);
+            unpack8<T>(feed.get(t, k, 0), v);
+            unpack8<T>(feed.get(t, k, 1), d);
 #pragma unroll
             for (int i = 0; i < V / 2; i++) {
                 f2 xh, none;
@@ -586,22 +620,31 @@ __global__ void __launch_bounds__(MAX_T, 2) k_gn_grad_sums(NormArgs a) {
                 sz[i] = add2(sz[i], dz);
                 sx[i] = fma2(dz, xh, sx[i]);
             }
+        };
+        int t = 0;
+        for (; t * B + B <= n; t++) {
+            feed.turn(t);
+#pragma unroll
+            for (int k = 0; k < B; k++) one(t, k);
         }
+        feed.turn(t);
+        for (int k = 0; t * B + k < n; k++) one(t, k);
     }
+    cp_async_wait<0>();
     float2 *cp = reinterpret_cast<float2 *>(a.cpart) + ((long long)sl.b * a.splits + sl.s) * a.C;
     float2 *gp = reinterpret_cast<float2 *>(a.part) + ((long long)sl.b * a.G + sl.c0 / a.cpg) * a.splits + sl.s;
     auto weight = [&](int c) { return a.w ? param<T>(a.w, a.param_f32, sl.c0 + c) : 1.f; };
     float v[V];
 #pragma unroll
     for (int i = 0; i < V; i++) v[i] = i < sl.valid ? at(sz, i) : 0.f;
-    fold_rows<V>(buf, v, a, sl);
-    for (int c = threadIdx.x; c < sl.cc; c += blockDim.x) cp[sl.c0 + c].x = buf[c];
-    fold_groups(g0, groups, a.cpg, [&](int c) { return buf[c] * weight(c); });
+    const float *f = fold_rows<V>(buf, v, a, sl);
+    for (int c = threadIdx.x; c < sl.cc; c += blockDim.x) cp[sl.c0 + c].x = f[c];
+    fold_groups(g0, groups, a.cpg, [&](int c) { return f[c] * weight(c); });
 #pragma unroll
     for (int i = 0; i < V; i++) v[i] = i < sl.valid ? at(sx, i) : 0.f;
-    fold_rows<V>(buf, v, a, sl);
-    for (int c = threadIdx.x; c < sl.cc; c += blockDim.x) cp[sl.c0 + c].y = buf[c];
-    fold_groups(g1, groups, a.cpg, [&](int c) { return buf[c] * weight(c); });
+    f = fold_rows<V>(buf, v, a, sl);
+    for (int c = threadIdx.x; c < sl.cc; c += blockDim.x) cp[sl.c0 + c].y = f[c];
+    fold_groups(g1, groups, a.cpg, [&](int c) { return f[c] * weight(c); });
     for (int g = threadIdx.x; g < groups; g += blockDim.x) gp[(long long)g * a.splits] = make_float2(g0[g], g1[g]);
 }
 
@@ -609,7 +652,7 @@ __global__ void __launch_bounds__(MAX_T, 2) k_gn_grad_sums(NormArgs a) {
 template <typename T, bool VEC, int PRE, int POST>
 __global__ void __launch_bounds__(MAX_T, 2) k_gn_grad_map(NormArgs a) {
     extern __shared__ __align__(16) uint8_t dsm[];
-    float *sm = reinterpret_cast<float *>(dsm + ring_bytes<T, 2, 1, 8>());
+    float *sm = reinterpret_cast<float *>(dsm + ring_bytes<T, 2, 2>());
     if ((int)blockIdx.x >= a.nslice) {
         // 32 channels per block, the (image, split) sums dealt to the warps, joined in order
         float2 *red = reinterpret_cast<float2 *>(sm);
@@ -639,15 +682,12 @@ __global__ void __launch_bounds__(MAX_T, 2) k_gn_grad_map(NormArgs a) {
     const int groups = sl.cc / a.cpg;
     float *g0 = sm, *g1 = sm + a.chunk / a.cpg;
     // from the end of the slice, as the forward's map
-    Feed<T, VEC, 2, 1, 8> feed;
-    feed.n = sl.rows(a);
-    const long long last = sl.lo + sl.r + (long long)(feed.n - 1) * a.rl;
-    feed.p[0] = reinterpret_cast<const T *>(a.x) + sl.b * a.x_img + sl.c + last * a.x_row;
-    feed.p[1] = reinterpret_cast<const T *>(a.dy) + sl.b * a.dy_img + sl.c + last * a.dy_row;
-    feed.step[0] = -a.rl * a.x_row;
-    feed.step[1] = -a.rl * a.dy_row;
-    feed.valid = sl.valid;
-    feed.ring = reinterpret_cast<uint4 *>(dsm);
+    constexpr int B = 2;
+    const int n = sl.rows(a);
+    const long long last = sl.lo + sl.r + (long long)(n - 1) * a.rl;
+    Feed<T, VEC, 2, B> feed(dsm, n, sl.valid);
+    feed.tensor(0, reinterpret_cast<const T *>(a.x) + sl.b * a.x_img + sl.c + last * a.x_row, -a.rl * a.x_row);
+    feed.tensor(1, reinterpret_cast<const T *>(a.dy) + sl.b * a.dy_img + sl.c + last * a.dy_row, -a.rl * a.dy_row);
     feed.start();
     const float inv = 1.0f / ((float)a.rows * (float)a.cpg);
     for (int g = threadIdx.x >> 5; g < groups; g += blockDim.x >> 5) {
@@ -670,22 +710,19 @@ __global__ void __launch_bounds__(MAX_T, 2) k_gn_grad_map(NormArgs a) {
         }
     }
     __syncthreads();
-    if (feed.n == 0) return;
+    if (n == 0) return;
     const Grad<T, PRE, POST, true> grad(a, sl);
     f2 m0[V / 2], m1[V / 2];
-#pragma unroll
-    for (int i = 0; i < V; i++) {
-        const int g = (sl.c + min(i, sl.valid - 1) - sl.c0) / a.cpg;
+    each_channel(a, sl, [&](int i, int g) {
         at(m0, i) = -g0[g];
         at(m1, i) = -g1[g];
-    }
-    T *dx = reinterpret_cast<T *>(a.dx) + (sl.b * a.rows + last) * a.C + sl.c;
+    });
+    T *dx = reinterpret_cast<T *>(a.dx) + ((long long)sl.b * a.rows + last) * a.C + sl.c;
     const long long ystep = -(long long)a.rl * a.C;
-    for (int t = 0; t < feed.n; t++) {
-        feed.turn(t);
+    auto one = [&](int t, int k) {
         f2 v[V / 2], d[V / 2];
-        unpack8<T>(feed.get(t, 0), v);
-        unpack8<T>(feed.get(t, 1), d);
+        unpack8<T>(feed.get(t, k, 0), v);
+        unpack8<T>(feed.get(t, k, 1), d);
 #pragma unroll
         for (int i = 0; i < V / 2; i++) {
             f2 xh, slope;
@@ -693,8 +730,17 @@ __global__ void __launch_bounds__(MAX_T, 2) k_gn_grad_map(NormArgs a) {
             const f2 du = mul2(grad.rs[i], fma2(xh, m1[i], fma2(grad.w[i], dz, m0[i])));
             v[i] = PRE ? mul2(du, slope) : du;
         }
-        store<T, VEC>(dx + t * ystep, sl.valid, v);
+        store<T, VEC>(dx, sl.valid, v);
+        dx += ystep;
+    };
+    int t = 0;
+    for (; t * B + B <= n; t++) {
+        feed.turn(t);
+#pragma unroll
+        for (int k = 0; k < B; k++) one(t, k);
     }
+    feed.turn(t);
+    for (int k = 0; t * B + k < n; k++) one(t, k);
 }
 
 // ---- host
@@ -703,6 +749,12 @@ int elem_size(int dtype) { return dtype == GS_F32 ? 4 : 2; }
 constexpr int SMS = 148;  // of a B200: the split of the work, and with it the workspace, is a matter of sizes alone
 
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
+
+// Slices of equal length (the last may be shorter, none is empty).
+void split(NormArgs &a, int want) {
+    a.per = std::max(1, (a.rows + want - 1) / want);
+    a.splits = std::max(1, (a.rows + a.per - 1) / a.per);
+}
 
 // Chunks of whole groups and whole vectors, of at least `want` channels.
 void chunks(NormArgs &a, int want) {
@@ -719,8 +771,9 @@ bool plan(const gs_norm_desc *d, NormArgs &a) {
     if (!d || d->B < 0 || d->rows < 0 || d->C < 1 || d->groups < 1 || d->C % d->groups) return false;
     if (d->dtype < GS_F32 || d->dtype > GS_F16 || d->act < GS_ACT_NONE || d->act > GS_ACT_SILU) return false;
     if (d->param_dtype != GS_F32 && d->param_dtype != d->dtype) return false;
-    if (!(d->eps >= 0.f) || d->C > GS_NORM_MAX_C || d->rows > (1LL << 40)) return false;
-    a.B = d->B; a.C = d->C; a.G = d->groups; a.cpg = d->C / d->groups; a.rows = d->rows;
+    if (!(d->eps >= 0.f) || d->C > GS_NORM_MAX_C || d->rows > GS_NORM_MAX_ROWS) return false;
+    a.B = d->B; a.C = d->C; a.G = d->groups; a.cpg = d->C / d->groups;
+    a.rows = (int)d->rows;
     a.x_row = d->x_row; a.x_img = d->x_img; a.dy_row = d->dy_row; a.dy_img = d->dy_img;
     a.param_f32 = d->param_dtype == GS_F32;
     a.eps = d->eps;
@@ -728,27 +781,29 @@ bool plan(const gs_norm_desc *d, NormArgs &a) {
     // the second launch joins only those groups' sums
     chunks(a, a.G > 32 ? 64 : a.C);
     a.rl = std::max(1, MAX_T / a.cvec);
-    // one wave of two blocks per SM, but no fewer than four rows a thread
+    // one wave of three blocks per SM, but no fewer than four rows a thread
     const long long most = std::max<long long>(1, a.rows / (4LL * a.rl));
-    const long long want = std::max<long long>(1, 2LL * SMS / std::max<long long>(1, (long long)a.B * a.nchunk));
-    a.splits = (int)std::max(std::min(most, want), a.rows >> 30);
+    const long long want = std::max<long long>(1, 3LL * SMS / std::max<long long>(1, (long long)a.B * a.nchunk));
+    split(a, (int)std::min(most, want));
     return (long long)a.B * a.splits * a.nchunk < (1LL << 30);
 }
 
 // The one-launch form's split: chunks of whole groups of at least 64 contiguous bytes a row, over a cluster of
-// as few CTAs as hold them, or as many (to 8) as find SMs idle.  False where 16 CTAs do not hold a chunk.
+// as few CTAs as hold them, or as many (to 8) as find SMs idle.  False where eight CTAs do not hold a chunk
+// (clusters of 16 wait for whole GPCs to be free).
 bool fused_plan(const gs_norm_desc *d, NormArgs &a) {
     if (a.C % V) return false;
     chunks(a, 64 / elem_size(d->dtype));
-    a.rl = MAX_T / a.cvec;
-    long long n = 1;
-    while (n <= 16 && (a.rows + n - 1) / n > (long long)a.rl * FUSED_R) n *= 2;
-    if (n > 16) return false;
+    if (a.cvec > FUSED_T) return false;
+    a.rl = FUSED_T / a.cvec;
+    int n = 1;
+    while (n <= 8 && (a.rows + n - 1) / n > a.rl * FUSED_R) n *= 2;
+    if (n > 8) return false;
     while (n < 8 && (long long)a.B * a.nchunk * n * 2 <= SMS && a.rows / (2 * n) >= a.rl) n *= 2;
-    a.splits = (int)n;
-    const int most = (int)((a.rows + n - 1) / n);
-    a.rl = std::min(a.rl, most);
-    a.held = (most + a.rl - 1) / a.rl;
+    a.splits = n;
+    a.per = (a.rows + n - 1) / n;
+    a.rl = std::min(a.rl, a.per);
+    a.held = (a.per + a.rl - 1) / a.rl;
     return (long long)a.B * a.splits * a.nchunk < (1LL << 30);
 }
 
@@ -783,8 +838,6 @@ template <typename T, int PRE, int POST>
 int forward_fused(const NormArgs &a, cudaStream_t s) {
     const int W = a.cpg % V == 0 ? 1 : V;
     auto kern = W == 1 ? k_gn_fused<T, PRE, POST, 1> : k_gn_fused<T, PRE, POST, V>;
-    if (a.splits > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-        return done(FWD);
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = a.splits;
@@ -793,13 +846,11 @@ int forward_fused(const NormArgs &a, cudaStream_t s) {
     memset(&c, 0, sizeof(c));
     c.gridDim = dim3((unsigned)(a.B * a.splits * a.nchunk));
     c.blockDim = dim3(threads(a));
-    c.dynamicSmemBytes = ring_bytes<T, 1, 4, 3>() + (size_t)2 * a.held * MAX_T * sizeof(float4) +
-                         ((size_t)MAX_T * W + (4 + 2 * (size_t)a.splits) * (a.chunk / a.cpg)) * sizeof(float);
+    c.dynamicSmemBytes = held_bytes(a.held) + ((size_t)2 * FUSED_T * W + (4 + 2 * (size_t)a.splits) * (a.chunk / a.cpg)) * sizeof(float);
     c.stream = s;
     c.attrs = at;
     c.numAttrs = 1;
-    if (c.dynamicSmemBytes > 48 * 1024 &&
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)c.dynamicSmemBytes) != cudaSuccess)
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)c.dynamicSmemBytes) != cudaSuccess)
         return done(FWD);
     cudaLaunchKernelEx(&c, kern, a);
     gs_count_launch(1);
@@ -812,15 +863,15 @@ int forward(const NormArgs &a, cudaStream_t s) {
     const size_t groups = 2 * (size_t)(a.chunk / a.cpg) * sizeof(float);
     const int W = a.cpg % V == 0 ? 1 : V;
     const int st = launch(W == 1 ? k_gn_stats<T, VEC, PRE, 1> : k_gn_stats<T, VEC, PRE, V>, grid, a,
-                          ring_bytes<T, 1, 4, 3>() + MAX_T * W * sizeof(float) + groups, s, FWD);
-    return st != GS_OK ? st : launch(k_gn_map<T, VEC, PRE, POST>, grid, a, ring_bytes<T, 1, 2, 4>() + groups, s, FWD);
+                          ring_bytes<T, 1, 2>() + 2 * MAX_T * W * sizeof(float) + groups, s, FWD);
+    return st != GS_OK ? st : launch(k_gn_map<T, VEC, PRE, POST>, grid, a, ring_bytes<T, 1, 2>() + groups, s, FWD);
 }
 template <typename T, bool VEC, int PRE, int POST>
 int backward(const NormArgs &a, cudaStream_t s) {
     const unsigned grid = (unsigned)(a.B * a.splits * a.nchunk), fold = a.dw || a.db ? (a.C + 31) / 32 : 0;
-    const size_t groups = 2 * (size_t)(a.chunk / a.cpg) * sizeof(float), ring = ring_bytes<T, 2, 1, 8>();
+    const size_t groups = 2 * (size_t)(a.chunk / a.cpg) * sizeof(float), ring = ring_bytes<T, 2, 2>();
     if (a.nslice + fold == 0) return GS_OK;
-    const int st = launch(k_gn_grad_sums<T, VEC, PRE, POST>, grid, a, ring + MAX_T * V * sizeof(float) + groups, s, BWD_);
+    const int st = launch(k_gn_grad_sums<T, VEC, PRE, POST>, grid, a, ring + groups, s, BWD_);
     return st != GS_OK ? st
                        : launch(k_gn_grad_map<T, VEC, PRE, POST>, a.nslice + fold, a,
                                 ring + std::max(groups, MAX_T * sizeof(float2)), s, BWD_);

@@ -251,8 +251,10 @@ typedef enum {
  * elements; channels adjacent), C / groups channels per group, statistics per (image, group) in fp32.
  * act_first 0: y = act(w xh + b); act_first 1: xh is normalised act(x), y = w xh + b (the order of the
  * encoder's stages, efficient_encoder.py:53-58).  The stages of gs_encoder_fwd keep their own fused form;
- * this one stands alone, for any group count, and has a backward.  C <= GS_NORM_MAX_C. */
+ * this one stands alone, for any group count, and has a backward.  C <= GS_NORM_MAX_C,
+ * rows <= GS_NORM_MAX_ROWS. */
 #define GS_NORM_MAX_C 2048
+#define GS_NORM_MAX_ROWS (1 << 30)
 typedef struct {
     int32_t B, C, groups;
     int32_t dtype;       /* gs_dtype of x, y, dy, dx */

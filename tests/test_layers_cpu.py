@@ -40,7 +40,7 @@ def test_norm_workspace_and_refusals(lib, ops):
     size = lib.gs_group_norm_act_workspace_size
     assert 0 < size(C.byref(norm_desc(ops)), 0) < size(C.byref(norm_desc(ops)), 1) < 1 << 24
     for bad in (dict(B=-1), dict(C=0), dict(groups=0), dict(groups=7), dict(dtype=3), dict(param_dtype=2), dict(act=3),
-                dict(act=-1), dict(eps=-1.0), dict(eps=float("nan")), dict(rows=-1), dict(C=2056)):
+                dict(act=-1), dict(eps=-1.0), dict(eps=float("nan")), dict(rows=-1), dict(C=2056), dict(rows=(1 << 30) + 1)):
         d = norm_desc(ops, **bad)
         assert size(C.byref(d), 0) == 0, bad
         assert lib.gs_group_norm_act_fwd(C.byref(d), *[None] * 6, 0, None) == 2, bad
