@@ -53,27 +53,6 @@ __device__ __forceinline__ float slope_of(uint32_t c) {
     return c == 65535u ? __int_as_float(0x7fffffff) : s;
 }
 
-// activation, and with `slope` its slope, of n pairs
-template <int N>
-__device__ __forceinline__ void activate(f2 *v, int act, const Act<ACT_GELU, true> &gelu, const Act<ACT_SILU, true> &silu) {
-    if (act == ACT_GELU)
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] = gelu(v[i]);
-    else if (act == ACT_SILU)
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] = silu(v[i]);
-}
-template <int N>
-__device__ __forceinline__ void activate(f2 *v, f2 *slope, int act, const Act<ACT_GELU, true> &gelu,
-                                         const Act<ACT_SILU, true> &silu) {
-    if (act == ACT_GELU)
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] = gelu(v[i], slope[i]);
-    else
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] = silu(v[i], slope[i]);
-}
-
 struct GemmArgs {
     long long I;          // rows of D
     int J;                // columns of D
@@ -84,7 +63,6 @@ struct GemmArgs {
     int tiles_i, tiles_j;
     // epilogue
     int out_f16;          // 16-bit output type
-    int act;
     int out_tma, res_tma; // whole 16-byte rows: TMA boxes, else element by element
     const void *bias, *residual;
     void *out, *slope;
@@ -94,203 +72,123 @@ struct GemmArgs {
 // term products of fp32 operands, small ones first: (a term, b term), 0 = high
 __constant__ const unsigned char PAIR_A[6] = {2, 0, 1, 1, 0, 0}, PAIR_B[6] = {0, 2, 1, 0, 1, 0};
 
-// Persistent and warp-specialised.  Work item = a 128 x BN tile of D times a k split; CTAs stride over
-// the items, neighbouring CTAs on neighbouring columns of the same rows (A from L2).
+// What an epilogue does with z = acc + bias: nothing, an activation, or an activation and its slope.
+enum { EPI_NONE = 0, EPI_GELU = 1, EPI_SILU = 2, EPI_GELU_SLOPE = 3, EPI_SILU_SLOPE = 4 };
+
+// Persistent and warp-specialised, one CTA per SM.  Work item = a tile of D times a k split; CTAs (or pairs)
+// stride over the items, neighbours on neighbouring columns of the same rows (A from L2).
 //   warp 0   TMA producer: A and B k-blocks into a STAGES-deep ring of 128-byte-swizzled tiles
 //   warp 1   TMEM owner, MMA issuer; accumulators double-buffered, so the epilogue runs under the next item
-//   warps 2..9  epilogue: quarter warp % 4 of the rows; BN >= 128: half of the columns each, BN = 64: every
-//            second item.  A unit is 32 rows x 128 bytes of the output, staged in shared memory in the
+//   warps 2..9  epilogue: quarter warp % 4 of the CTA's 128 rows; half of the columns each (BN = 64: every
+//            second item).  A unit is 32 rows x 128 bytes of the output, staged in shared memory in the
 //            128-byte swizzle (a thread writes its row without bank conflicts) and moved by TMA; the residual
-//            comes by TMA into the same place and is added in registers before the only rounding.
+//            comes by TMA into the same place, a unit ahead, and is added in registers before the only rounding.
+// PAIR: two CTAs share a 256 x 256 tile (cta_group::2): each loads its 128 rows of A and half of B's rows, so an
+// output costs two thirds of the L2 reads of a 128 x 256 tile; that traffic, not the tensor cores, bounds large
+// products (a 128 x 256 tile read 13 TB/s from L2 at 1130 TFLOP/s).  The leader issues all MMAs.
 // Every wait is bounded; one that gives up records a code in g_wait_error and raises the CTA's abort flag.
-template <int BN, bool OUT32>
+template <int BN, bool PAIR, bool OUT32>
 struct Shape {
-    static constexpr uint32_t A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = BN == 256 ? 3 : BN == 128 ? 5 : 6;
+    static constexpr int BROWS = PAIR ? BN / 2 : BN;  // rows of B in this CTA
+    static constexpr uint32_t A_BYTES = BM * BK * 2, B_BYTES = BROWS * BK * 2, STAGE = A_BYTES + B_BYTES;
+    static constexpr int STAGES = BROWS >= 128 ? 4 : 5;
     static constexpr int CS = BN >= 128 ? 2 : 1;  // warps sharing a row quarter's columns
     static constexpr int EC = OUT32 ? 32 : 64;    // columns of a unit
     static constexpr int UNITS = BN / CS / EC;
-    static constexpr uint32_t EPI = 8 * 2 * 4096;  // two units per epilogue warp
-    static constexpr size_t SMEM = 1024 + STAGES * STAGE + EPI;
+    static constexpr uint32_t SLOTS = 3 * 4096;  // per epilogue warp: two for outputs and residuals, one for slopes
+    static constexpr size_t SMEM = 1024 + STAGES * STAGE + 8 * SLOTS;
+    static constexpr int TILE_I = PAIR ? 2 * BM : BM;
 };
 
-template <int BN, bool OUT32>
-__global__ void __launch_bounds__(320, 1)
-    k_gemm(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-           const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmS,
-           const __grid_constant__ CUtensorMap tmR, const GemmArgs a) {
-    using S = Shape<BN, OUT32>;
-    constexpr int STAGES = S::STAGES, EC = S::EC;
-    extern __shared__ uint8_t dsmem[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], tfull[2], tempty[2], mdone, rbar[8][2];
-    __shared__ uint32_t tmem_base;
-    __shared__ volatile int abort_flag;
-    __shared__ int issued, consumed;
-    __shared__ __align__(16) float sbias[8][32];
+struct Pipe {  // one CTA's barriers
+    uint64_t full[5], empty[5], tfull[2], tempty[2], mdone, rbar[8][2];
+    uint32_t tmem_base;
+    volatile int abort_flag;
+    int issued, consumed;
+    __align__(16) float bias[8][32];  // read as float4
+};
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int kbt = a.kb * a.npair;
-    const int n_items = a.tiles_i * a.tiles_j * a.splits;
-
-    if (warp == 1) {
-        tmem_alloc(&tmem_base, 2 * BN);
-        tmem_relinquish();
+// row tile, column tile, split of an item
+struct Item {
+    int i, j, s;
+    __device__ __forceinline__ Item(const GemmArgs &a, int item) {
+        j = item % a.tiles_j;
+        item /= a.tiles_j;
+        i = item % a.tiles_i;
+        s = item / a.tiles_i;
     }
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; s++) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
-        }
-        for (int j = 0; j < 2; j++) {
-            mbar_init(&tfull[j], 1);
-            mbar_init(&tempty[j], 4 * S::CS);
-        }
-        for (int w = 0; w < 8; w++)
-            for (int j = 0; j < 2; j++) mbar_init(&rbar[w][j], 1);
-        mbar_init(&mdone, 1);
-        abort_flag = 0;
-        issued = 0;
-        consumed = 0;
-        fence_barrier_init();
-        prefetch_tensormap(&tmA);
-        prefetch_tensormap(&tmB);
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tbase = tmem_base;
+};
 
-    if (warp == 0) {
-        if (lane == 0) {
-            int it = 0;
-            for (int item = blockIdx.x; item < n_items && !abort_flag; item += gridDim.x) {
-                int t = item;
-                const int j0 = t % a.tiles_j * BN;
-                t /= a.tiles_j;
-                const int i0 = t % a.tiles_i * BM;
-                const int s = t / a.tiles_i;
-                const int k1 = (int)((long long)kbt * (s + 1) / a.splits);
-                for (int k = (int)((long long)kbt * s / a.splits); k < k1; k++, it++) {
-                    const int st = it % STAGES;
-                    if (it >= STAGES && !mbar_wait_or_abort(&empty[st], ((it / STAGES) - 1) & 1, &abort_flag,
-                                                            &g_wait_error, 1))
-                        break;
-                    if (abort_flag) break;
-                    mbar_arrive_expect_tx(&full[st], S::STAGE);
-                    uint8_t *sa = smem + st * S::STAGE, *sb = sa + S::A_BYTES;
-                    const int p = k / a.kb, kk = (k - p * a.kb) * BK;
-                    const int ta = a.npair > 1 ? PAIR_A[p] : 0, tb = a.npair > 1 ? PAIR_B[p] : 0;
-                    if (a.a_mn) {
-#pragma unroll
-                        for (int c = 0; c < BM / 64; c++)
-                            tma_load_3d(sa + c * 64 * 128, &tmA, &full[st], i0 + 64 * c, kk, ta);
-                    } else {
-                        tma_load_3d(sa, &tmA, &full[st], kk, i0, ta);
-                    }
-                    if (a.b_mn) {
-#pragma unroll
-                        for (int c = 0; c < BN / 64; c++)
-                            tma_load_3d(sb + c * 64 * 128, &tmB, &full[st], j0 + 64 * c, kk, tb);
-                    } else {
-                        tma_load_3d(sb, &tmB, &full[st], kk, j0, tb);
-                    }
-                    issued = it + 1;
-                }
-            }
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t fmt = a.f16 ? 0u : 1u;
-            const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)a.a_mn << 15) |
-                                   ((uint32_t)a.b_mn << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
-            // per 16 of k: 32 bytes inside the swizzled row (K-major), two 8-row groups (MN-major)
-            const uint32_t stepA = a.a_mn ? 2048u : 32u, stepB = a.b_mn ? 2048u : 32u;
-            int it = 0, tc = 0;
-            for (int item = blockIdx.x; item < n_items && !abort_flag; item += gridDim.x, tc++) {
-                const int s = item / (a.tiles_j * a.tiles_i);
-                const int k0 = (int)((long long)kbt * s / a.splits), k1 = (int)((long long)kbt * (s + 1) / a.splits);
-                const int buf = tc & 1;
-                if (tc >= 2 && !mbar_wait_or_abort(&tempty[buf], ((tc >> 1) - 1) & 1, &abort_flag, &g_wait_error, 2))
-                    break;
-                tc_fence_after();
-                const uint32_t dcol = tbase + (uint32_t)buf * BN;
-                bool ok = true;
-                for (int k = k0; k < k1; k++, it++) {
-                    const int st = it % STAGES;
-                    if (!mbar_wait_or_abort(&full[st], (it / STAGES) & 1, &abort_flag, &g_wait_error, 3)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t sa = smem_u32(smem + st * S::STAGE), sb = sa + S::A_BYTES;
-#pragma unroll
-                    for (int q = 0; q < BK / 16; q++) {
-                        const uint64_t ad = a.a_mn ? sdesc_mn(sa + stepA * q, 8192, 1024) : sdesc(sa + stepA * q, 1024, 2);
-                        const uint64_t bd = a.b_mn ? sdesc_mn(sb + stepB * q, 8192, 1024) : sdesc(sb + stepB * q, 1024, 2);
-                        mma_bf16(dcol, ad, bd, idesc, (k > k0 || q) ? 1u : 0u);
-                    }
-                    mma_commit(&empty[st]);
-                    consumed = it + 1;
-                }
-                if (!ok) break;
-                mma_commit(&tfull[buf]);
-            }
-            // all MMAs of this CTA (also those of an aborted item) have finished once mdone flips
-            mma_commit(&mdone);
-            mbar_wait(&mdone, 0, &g_wait_error, 4);
-        }
-    } else {
-        const int e = warp - 2, q = warp & 3, half = e >> 2;
-        uint8_t *const slots = smem + STAGES * S::STAGE + e * 8192;
-        const bool has_res = a.residual != nullptr, has_slope = a.slope != nullptr;
-        const Act<ACT_GELU, true> gelu;
-        const Act<ACT_SILU, true> silu;
-        int tc = 0, use = 0, rphase[2] = {0, 0};
-        for (int item = blockIdx.x; item < n_items; item += gridDim.x, tc++) {
-            const int buf = tc & 1;
-            if (S::CS == 1 && half != buf) continue;
-            int t = item;
-            const int jt = t % a.tiles_j * BN;
-            t /= a.tiles_j;
-            const long long row0 = (long long)(t % a.tiles_i) * BM + q * 32;
-            const int sp = t / a.tiles_i;
-            bool ready = false, dead = false;
-#pragma unroll
-            for (int u = 0; u < S::UNITS; u++) {
-                const int lc = (S::CS == 2 ? half * (BN / 2) : 0) + u * EC;  // column inside the tile
-                const int col0 = jt + lc;
-                const bool live = col0 < a.J && row0 < a.I;
-                // the slot: alternating, or with a slope always the first (the second is the slope's)
-                const int sl = has_slope ? 0 : use & 1;
-                uint8_t *const out = slots + sl * 4096, *const slo = slots + 4096;
-                if (live) {
-                    use++;
+template <int BN, bool PAIR, bool OUT32, int EPI>
+__device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ring_end, const CUtensorMap *tmO,
+                                         const CUtensorMap *tmS, const CUtensorMap *tmR, int first, int stride, int n_items,
+                                         int rank) {
+    using S = Shape<BN, PAIR, OUT32>;
+    constexpr int EC = S::EC;
+    constexpr bool SLOPE = EPI >= EPI_GELU_SLOPE;
+    constexpr int ACT = EPI == EPI_NONE ? ACT_NONE : EPI == EPI_GELU || EPI == EPI_GELU_SLOPE ? ACT_GELU : ACT_SILU;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e = warp - 2, q = warp & 3, half = e >> 2;
+    uint8_t *const slots = ring_end + e * S::SLOTS, *const slo = slots + 2 * 4096;
+    const uint32_t tbase = p.tmem_base + ((uint32_t)(q * 32) << 16);
+    const bool has_res = a.residual != nullptr, res_tma = has_res && a.res_tma;
+    const Act<ACT, SLOPE> act;
+    // this warp's items: all, or (BN = 64) those of its accumulator buffer
+    const int step = S::CS == 1 ? 2 * stride : stride;
+    int item = S::CS == 1 ? first + half * stride : first, tc = S::CS == 1 ? half : 0, use = 0;
+
+    auto place = [&](int it, int u, int &col0, long long &row0) {
+        const Item t(a, it);
+        col0 = t.j * BN + (S::CS == 2 ? half * (BN / 2) : 0) + u * EC;
+        row0 = (long long)t.i * S::TILE_I + rank * BM + q * 32;
+        return col0 < a.J && row0 < a.I;
+    };
+    // the residual of the first live unit from (it, u) on goes to slot s
+    auto prefetch = [&](int it, int u, int s) {
+        int col0;
+        long long row0;
+        for (; it < n_items; it += step, u = 0)
+            for (; u < S::UNITS; u++)
+                if (place(it, u, col0, row0)) {
                     if (lane == 0) {
-                        if (has_slope) bulk_wait_read<0>();
-                        else bulk_wait_read<1>();
+                        mbar_arrive_expect_tx(&p.rbar[e][s], 4096);
+                        tma_load_3d(slots + s * 4096, tmR, &p.rbar[e][s], col0, (int)row0, 0);
                     }
-                    __syncwarp();
-                    if (has_res && a.res_tma) {
-                        if (lane == 0) {
-                            mbar_arrive_expect_tx(&rbar[e][sl], 4096);
-                            tma_load_3d(out, &tmR, &rbar[e][sl], col0, (int)row0, 0);
-                        }
-                    } else if (has_res) {
-                        for (int r = 0; r < 32 && row0 + r < a.I; r++)
-#pragma unroll
-                            for (int c = lane; c < EC; c += 32)
-                                if (col0 + c < a.J) {
-                                    const long long at = (row0 + r) * a.ldr + col0 + c;
-                                    const int b = c * (128 / EC);
-                                    uint8_t *d = out + r * 128 + ((b & ~15) ^ ((r & 7) << 4)) + (b & 15);
-                                    if (OUT32) *reinterpret_cast<float *>(d) = reinterpret_cast<const float *>(a.residual)[at];
-                                    else *reinterpret_cast<uint16_t *>(d) = reinterpret_cast<const uint16_t *>(a.residual)[at];
-                                }
-                        __syncwarp();
-                    }
+                    return true;
                 }
-                float bias[EC / 32];
+        return false;
+    };
+    bool pending = res_tma && prefetch(item, 0, 0);  // a residual is on its way to slot use & 1
+    bool dead = false;
+    for (; item < n_items && !dead; item += step, tc += S::CS == 1 ? 2 : 1) {
+        const int buf = tc & 1;
+        const int sp = Item(a, item).s;
+#pragma unroll 1
+        for (int u = 0; u < S::UNITS && !dead; u++) {
+            int col0;
+            long long row0;
+            const bool live = place(item, u, col0, row0);
+            uint8_t *const out = slots + (use & 1) * 4096;
+            float bias[EC / 32];
+            if (live) {
+                // the slots this unit writes are no longer read by their stores
+                if (lane == 0) {
+                    if (SLOPE) bulk_wait_read<0>();
+                    else bulk_wait_read<1>();
+                }
+                __syncwarp();
+                if (has_res && !res_tma) {
+                    for (int r = 0; r < 32 && row0 + r < a.I; r++)
+#pragma unroll
+                        for (int c = lane; c < EC; c += 32)
+                            if (col0 + c < a.J) {
+                                const long long at = (row0 + r) * a.ldr + col0 + c;
+                                const int b = c * (128 / EC);
+                                uint8_t *d = out + r * 128 + ((b & ~15) ^ ((r & 7) << 4)) + (b & 15);
+                                if (OUT32) *reinterpret_cast<float *>(d) = reinterpret_cast<const float *>(a.residual)[at];
+                                else *reinterpret_cast<uint16_t *>(d) = reinterpret_cast<const uint16_t *>(a.residual)[at];
+                            }
+                    __syncwarp();
+                }
 #pragma unroll
                 for (int h = 0; h < EC / 32; h++) {
                     const int c = col0 + 32 * h + lane;
@@ -300,114 +198,290 @@ __global__ void __launch_bounds__(320, 1)
                                   : a.out_f16 ? to_f32(reinterpret_cast<const __half *>(a.bias)[c])
                                               : to_f32(reinterpret_cast<const __nv_bfloat16 *>(a.bias)[c]);
                 }
-                if (!ready) {
-                    if (!mbar_wait_or_abort(&tfull[buf], (tc >> 1) & 1, &abort_flag, &g_wait_error, 5)) dead = true;
-                    tc_fence_after();
-                    ready = true;
+            }
+            if (u == 0) {
+                if (!mbar_wait_or_abort(&p.tfull[buf], (tc >> 1) & 1, &p.abort_flag, &g_wait_error, 5)) dead = true;
+                tc_fence_after();
+            }
+            if (live && pending) {
+                // (after an abort too: the copy lands in this CTA's shared memory)
+                if (!mbar_wait(&p.rbar[e][use & 1], (use >> 1) & 1, &g_wait_error, 6)) {
+                    p.abort_flag = 1;
+                    dead = true;
                 }
-                if (live && has_res && a.res_tma) {
-                    // (after an abort too: the copy lands in this CTA's shared memory)
-                    if (!mbar_wait(&rbar[e][sl], rphase[sl] & 1, &g_wait_error, 6)) {
-                        abort_flag = 1;
-                        dead = true;
-                    }
-                    rphase[sl]++;
-                }
+                pending = false;
+            }
 #pragma unroll
-                for (int h = 0; h < EC / 32; h++) {
+            for (int h = 0; h < EC / 32; h++) {
+                f2 v[16];
+                if (live && !dead) {
                     uint32_t r[32];
+                    const int lc = (S::CS == 2 ? half * (BN / 2) : 0) + u * EC + 32 * h;
+                    tmem_ld32(tbase + (uint32_t)(buf * BN + lc), r);
                     __syncwarp();
-                    sbias[e][lane] = bias[h];
+                    p.bias[e][lane] = bias[h];
                     __syncwarp();
-                    if (live && !dead) {
-                        tmem_ld32(tbase + ((uint32_t)(q * 32) << 16) + (uint32_t)buf * BN + (uint32_t)(lc + 32 * h), r);
-                        tmem_wait_ld();
+                    tmem_wait_ld32(r);
+                    const float4 *b = reinterpret_cast<const float4 *>(p.bias[e]);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float4 f = b[i];
+                        v[2 * i] = add2({__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])}, {f.x, f.y});
+                        v[2 * i + 1] = add2({__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3])}, {f.z, f.w});
                     }
-                    if (u == S::UNITS - 1 && h == EC / 32 - 1) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&tempty[buf]);
-                    }
-                    if (!live || dead) continue;
-                    // 16 bytes of output at a time: 8 columns (16 bit) or 4 (fp32)
-                    constexpr int W = OUT32 ? 4 : 8;
-#pragma unroll
-                    for (int g = 0; g < 32 / W; g++) {
-                        f2 v[W / 2];
-                        const uint32_t at = (uint32_t)lane * 128u + ((uint32_t)(((OUT32 ? 0 : 4 * h) + g) ^ (lane & 7)) << 4);
-#pragma unroll
-                        for (int i = 0; i < W / 2; i++) {
-                            const float2 b = *reinterpret_cast<const float2 *>(&sbias[e][g * W + 2 * i]);
-                            v[i] = add2({__uint_as_float(r[g * W + 2 * i]), __uint_as_float(r[g * W + 2 * i + 1])}, {b.x, b.y});
-                        }
-                        if (has_slope) {
-                            f2 sv[W / 2];
-                            activate<W / 2>(v, sv, a.act, gelu, silu);
-                            *reinterpret_cast<uint4 *>(slo + at) =
-                                OUT32 ? pack16<float>(sv)
-                                      : make_uint4(slope_codes(sv[0]), slope_codes(sv[1]), slope_codes(sv[2 % (W / 2)]),
-                                                   slope_codes(sv[3 % (W / 2)]));
-                        } else {
-                            activate<W / 2>(v, a.act, gelu, silu);
-                        }
-                        if (has_res) {
-                            const uint4 p = *reinterpret_cast<const uint4 *>(out + at);
-                            f2 f[4];
-                            if (OUT32) unpack16<float>(p, f);
-                            else if (a.out_f16) unpack16<__half>(p, f);
-                            else unpack16<__nv_bfloat16>(p, f);
-#pragma unroll
-                            for (int i = 0; i < W / 2; i++) v[i] = add2(v[i], f[i]);
-                        }
-                        if (OUT32) *reinterpret_cast<uint4 *>(out + at) = pack16<float>(v);
-                        else *reinterpret_cast<uint4 *>(out + at) = a.out_f16 ? pack16<__half>(v) : pack16<__nv_bfloat16>(v);
+                }
+                if (u == S::UNITS - 1 && h == EC / 32 - 1) {  // the accumulator is drained
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (PAIR && rank) mbar_arrive_cluster(in_rank(&p.tempty[buf], 0));
+                        else mbar_arrive(&p.tempty[buf]);
                     }
                 }
                 if (!live || dead) continue;
-                if (a.out_tma) {
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) {
-                        tma_store_3d(&tmO, out, col0, (int)row0, sp);
-                        if (has_slope) tma_store_3d(&tmS, slo, col0, (int)row0, 0);
-                        bulk_commit();
+                // 16 bytes of a row: chunk c of the unit, in the 128-byte swizzle
+                auto chunk = [&](uint8_t *base, int c) {
+                    return reinterpret_cast<uint4 *>(base + lane * 128 + ((c ^ (lane & 7)) << 4));
+                };
+                if (SLOPE) {
+#pragma unroll
+                    for (int g = 0; g < 2; g++) {
+                        f2 s[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) v[8 * g + i] = act(v[8 * g + i], s[i]);
+                        if (OUT32) {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) *chunk(slo, 4 * g + i) = pack16<float>(s + 2 * i);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 2; i++)
+                                *chunk(slo, 4 * h + 2 * g + i) = make_uint4(slope_codes(s[4 * i]), slope_codes(s[4 * i + 1]),
+                                                                            slope_codes(s[4 * i + 2]), slope_codes(s[4 * i + 3]));
+                        }
+                    }
+                } else if (ACT != ACT_NONE) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) v[i] = act(v[i]);
+                }
+                if (OUT32) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        uint4 *c = chunk(out, i);
+                        if (has_res) {
+                            f2 f[2];
+                            unpack16<float>(*c, f);
+                            v[2 * i] = add2(v[2 * i], f[0]);
+                            v[2 * i + 1] = add2(v[2 * i + 1], f[1]);
+                        }
+                        *c = pack16<float>(v + 2 * i);
                     }
                 } else {
-                    __syncwarp();
-                    constexpr int ES = 128 / EC;  // bytes of an element
-                    for (int r = 0; r < 32 && row0 + r < a.I; r++)
 #pragma unroll
-                        for (int c = lane; c < EC; c += 32)
-                            if (col0 + c < a.J) {
-                                const long long at = (row0 + r) * a.J + col0 + c;
-                                const int b = c * ES, off = r * 128 + ((b & ~15) ^ ((r & 7) << 4)) + (b & 15);
-                                if (OUT32) {
-                                    reinterpret_cast<float *>(a.out)[at] = *reinterpret_cast<const float *>(out + off);
-                                    if (has_slope)
-                                        reinterpret_cast<float *>(a.slope)[at] = *reinterpret_cast<const float *>(slo + off);
-                                } else {
-                                    reinterpret_cast<uint16_t *>(a.out)[at] = *reinterpret_cast<const uint16_t *>(out + off);
-                                    if (has_slope)
-                                        reinterpret_cast<uint16_t *>(a.slope)[at] = *reinterpret_cast<const uint16_t *>(slo + off);
-                                }
-                            }
-                    fence_proxy_async();  // the next residual's copy overwrites what was just read
-                    __syncwarp();
+                    for (int i = 0; i < 4; i++) {
+                        uint4 *c = chunk(out, 4 * h + i);
+                        if (has_res) {
+                            f2 f[4];
+                            if (a.out_f16) unpack16<__half>(*c, f);
+                            else unpack16<__nv_bfloat16>(*c, f);
+#pragma unroll
+                            for (int k = 0; k < 4; k++) v[4 * i + k] = add2(v[4 * i + k], f[k]);
+                        }
+                        *c = a.out_f16 ? pack16<__half>(v + 4 * i) : pack16<__nv_bfloat16>(v + 4 * i);
+                    }
                 }
             }
-            if (dead) break;
+            if (!live || dead) continue;
+            fence_proxy_async();
+            __syncwarp();
+            if (res_tma) {
+                if (lane == 0) bulk_wait_read<0>();  // the other slot's store, a unit ago
+                pending = prefetch(item, u + 1, (use + 1) & 1);
+            }
+            if (a.out_tma) {
+                if (lane == 0) {
+                    tma_store_3d(tmO, out, col0, (int)row0, sp);
+                    if (SLOPE) tma_store_3d(tmS, slo, col0, (int)row0, 0);
+                    bulk_commit();
+                }
+            } else {
+                constexpr int ES = 128 / EC;  // bytes of an element
+                for (int r = 0; r < 32 && row0 + r < a.I; r++)
+#pragma unroll
+                    for (int c = lane; c < EC; c += 32)
+                        if (col0 + c < a.J) {
+                            const long long at = (row0 + r) * a.J + col0 + c;
+                            const int b = c * ES, off = r * 128 + ((b & ~15) ^ ((r & 7) << 4)) + (b & 15);
+                            if (OUT32) {
+                                reinterpret_cast<float *>(a.out)[at] = *reinterpret_cast<const float *>(out + off);
+                                if (SLOPE) reinterpret_cast<float *>(a.slope)[at] = *reinterpret_cast<const float *>(slo + off);
+                            } else {
+                                reinterpret_cast<uint16_t *>(a.out)[at] = *reinterpret_cast<const uint16_t *>(out + off);
+                                if (SLOPE)
+                                    reinterpret_cast<uint16_t *>(a.slope)[at] = *reinterpret_cast<const uint16_t *>(slo + off);
+                            }
+                        }
+                fence_proxy_async();  // the next residual's copy overwrites what was just read
+                __syncwarp();
+            }
+            use++;
         }
-        if (lane == 0) bulk_wait<0>();
+    }
+    if (pending) mbar_wait(&p.rbar[e][use & 1], (use >> 1) & 1, &g_wait_error, 8);
+    if (lane == 0) bulk_wait<0>();
+    __syncwarp();
+}
+
+template <int BN, bool PAIR, bool OUT32, int EPI>
+__global__ void __launch_bounds__(320, 1)
+    k_gemm(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+           const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmS,
+           const __grid_constant__ CUtensorMap tmR, const GemmArgs a) {
+    using S = Shape<BN, PAIR, OUT32>;
+    constexpr int STAGES = S::STAGES;
+    extern __shared__ uint8_t dsmem[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~(uintptr_t)1023);
+    __shared__ __align__(16) Pipe p;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = PAIR ? (int)cluster_rank() : 0;
+    const int first = PAIR ? blockIdx.x / 2 : blockIdx.x, stride = PAIR ? gridDim.x / 2 : gridDim.x;
+    const int kbt = a.kb * a.npair;
+    const int n_items = a.tiles_i * a.tiles_j * a.splits;
+
+    if (warp == 1) {
+        if (PAIR) {
+            tmem_alloc_pair(&p.tmem_base, 2 * BN);
+        } else {
+            tmem_alloc(&p.tmem_base, 2 * BN);
+            tmem_relinquish();
+        }
+    }
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(&p.full[s], 1);
+            mbar_init(&p.empty[s], 1);
+        }
+        for (int j = 0; j < 2; j++) {
+            mbar_init(&p.tfull[j], 1);
+            mbar_init(&p.tempty[j], 4 * S::CS * (PAIR ? 2 : 1));
+        }
+        for (int w = 0; w < 8; w++)
+            for (int j = 0; j < 2; j++) mbar_init(&p.rbar[w][j], 1);
+        mbar_init(&p.mdone, 1);
+        p.abort_flag = 0;
+        p.issued = 0;
+        p.consumed = 0;
+        fence_barrier_init();
+        prefetch_tensormap(&tmA);
+        prefetch_tensormap(&tmB);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (PAIR) cluster_arrive_wait();  // both CTAs' barriers exist
+    tc_fence_after();
+    const uint32_t tbase = p.tmem_base;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            for (int item = first; item < n_items && !p.abort_flag; item += stride) {
+                const Item t(a, item);
+                const int j0 = t.j * BN + (PAIR ? rank * S::BROWS : 0), i0 = t.i * S::TILE_I + rank * BM;
+                const int k1 = (int)((long long)kbt * (t.s + 1) / a.splits);
+                for (int k = (int)((long long)kbt * t.s / a.splits); k < k1; k++, it++) {
+                    const int st = it % STAGES;
+                    if (it >= STAGES && !mbar_wait_or_abort(&p.empty[st], ((it / STAGES) - 1) & 1, &p.abort_flag,
+                                                            &g_wait_error, 1))
+                        break;
+                    if (p.abort_flag) break;
+                    uint8_t *sa = smem + st * S::STAGE, *sb = sa + S::A_BYTES;
+                    const int pr = k / a.kb, kk = (k - pr * a.kb) * BK;
+                    const int ta = a.npair > 1 ? PAIR_A[pr] : 0, tb = a.npair > 1 ? PAIR_B[pr] : 0;
+                    // both CTAs' copies complete on the leader's barrier
+                    if (rank == 0) mbar_arrive_expect_tx(&p.full[st], S::STAGE * (PAIR ? 2 : 1));
+                    const uint32_t bar = PAIR ? in_rank(&p.full[st], 0) : 0;
+                    auto load = [&](uint8_t *dst, const CUtensorMap *tm, int c0, int c1, int c2) {
+                        if (PAIR) tma_load_3d_pair(dst, tm, bar, c0, c1, c2);
+                        else tma_load_3d(dst, tm, &p.full[st], c0, c1, c2);
+                    };
+                    if (a.a_mn) {
+#pragma unroll
+                        for (int c = 0; c < BM / 64; c++) load(sa + c * 64 * 128, &tmA, i0 + 64 * c, kk, ta);
+                    } else {
+                        load(sa, &tmA, kk, i0, ta);
+                    }
+                    if (a.b_mn) {
+#pragma unroll
+                        for (int c = 0; c < S::BROWS / 64; c++) load(sb + c * 64 * 128, &tmB, j0 + 64 * c, kk, tb);
+                    } else {
+                        load(sb, &tmB, kk, j0, tb);
+                    }
+                    p.issued = it + 1;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            const uint32_t fmt = a.f16 ? 0u : 1u;
+            const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)a.a_mn << 15) |
+                                   ((uint32_t)a.b_mn << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(S::TILE_I >> 4) << 24);
+            // per 16 of k: 32 bytes inside the swizzled row (K-major), two 8-row groups (MN-major)
+            const uint32_t stepA = a.a_mn ? 2048u : 32u, stepB = a.b_mn ? 2048u : 32u;
+            int it = 0, tc = 0;
+            for (int item = first; item < n_items && !p.abort_flag; item += stride, tc++) {
+                const int s = Item(a, item).s;
+                const int k0 = (int)((long long)kbt * s / a.splits), k1 = (int)((long long)kbt * (s + 1) / a.splits);
+                const int buf = tc & 1;
+                if (tc >= 2 && !mbar_wait_or_abort(&p.tempty[buf], ((tc >> 1) - 1) & 1, &p.abort_flag, &g_wait_error, 2))
+                    break;
+                tc_fence_after();
+                const uint32_t dcol = tbase + (uint32_t)buf * BN;
+                bool ok = true;
+                for (int k = k0; k < k1; k++, it++) {
+                    const int st = it % STAGES;
+                    if (!mbar_wait_or_abort(&p.full[st], (it / STAGES) & 1, &p.abort_flag, &g_wait_error, 3)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t sa = smem_u32(smem + st * S::STAGE), sb = sa + S::A_BYTES;
+#pragma unroll
+                    for (int q = 0; q < BK / 16; q++) {
+                        const uint64_t ad = a.a_mn ? sdesc_mn(sa + stepA * q, 8192, 1024) : sdesc(sa + stepA * q, 1024, 2);
+                        const uint64_t bd = a.b_mn ? sdesc_mn(sb + stepB * q, 8192, 1024) : sdesc(sb + stepB * q, 1024, 2);
+                        if (PAIR) mma_pair(dcol, ad, bd, idesc, (k > k0 || q) ? 1u : 0u);
+                        else mma_bf16(dcol, ad, bd, idesc, (k > k0 || q) ? 1u : 0u);
+                    }
+                    if (PAIR) mma_commit_pair(&p.empty[st]);
+                    else mma_commit(&p.empty[st]);
+                    p.consumed = it + 1;
+                }
+                if (!ok) break;
+                if (PAIR) mma_commit_pair(&p.tfull[buf]);
+                else mma_commit(&p.tfull[buf]);
+            }
+            // all MMAs of this CTA or pair (also those of an aborted item) have finished once mdone flips
+            if (PAIR) mma_commit_pair(&p.mdone);
+            else mma_commit(&p.mdone);
+            mbar_wait(&p.mdone, 0, &g_wait_error, 4);
+        }
+    } else {
+        epilogue<BN, PAIR, OUT32, EPI>(a, p, smem + STAGES * S::STAGE, &tmO, &tmS, &tmR, first, stride, n_items, rank);
     }
 
     tc_fence_before();
     __syncthreads();
-    if (abort_flag && threadIdx.x == 0)
+    if (PAIR) cluster_arrive_wait();  // no CTA leaves while its peer's copies, MMAs or arrivals may reach it
+    if (p.abort_flag && threadIdx.x == 0 && rank == 0)
         // copies that were issued but never consumed still land in shared memory: wait for them
-        for (int j = consumed; j < issued; j++) mbar_wait(&full[j % STAGES], (j / STAGES) & 1, &g_wait_error, 7);
+        for (int j = p.consumed; j < p.issued; j++) mbar_wait(&p.full[j % STAGES], (j / STAGES) & 1, &g_wait_error, 7);
     __syncthreads();
+    if (PAIR) cluster_arrive_wait();
     tc_fence_after();
-    if (warp == 1) tmem_dealloc(tbase, 2 * BN);
+    if (warp == 1) {
+        if (PAIR) tmem_dealloc_pair(tbase, 2 * BN);
+        else tmem_dealloc(tbase, 2 * BN);
+    }
 }
 
 // ---- operands that TMA cannot read in place (rows not on 16 bytes, fp32): rows padded to a multiple of eight
@@ -593,8 +667,13 @@ __global__ void __launch_bounds__(256) k_join(JoinArgs a) {
             v[0] = add2(v[0], {to_f32(b[0]), n > 1 ? to_f32(b[1]) : 0.f});
             v[1] = add2(v[1], {n > 2 ? to_f32(b[2]) : 0.f, n > 3 ? to_f32(b[3]) : 0.f});
         }
-        if (a.slope) activate<2>(v, sl, a.act, gelu, silu);
-        else activate<2>(v, a.act, gelu, silu);
+        if (a.act == ACT_GELU) {
+            v[0] = gelu(v[0], sl[0]);
+            v[1] = gelu(v[1], sl[1]);
+        } else if (a.act == ACT_SILU) {
+            v[0] = silu(v[0], sl[0]);
+            v[1] = silu(v[1], sl[1]);
+        }
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             if (k >= n) break;
@@ -623,25 +702,28 @@ bool valid(const gs_linear_desc *d) {
            d->ldy <= GS_LINEAR_MAX_LD && d->M * std::max(d->N, d->K) <= 1LL << 40;
 }
 
-// The tile of one product: the columns whose waves over the SMs cost least (a tile's cost: its columns of
-// MMA and epilogue work and a fixed part), then k splits while SMs are left over and a part keeps at least
-// four k-blocks.
+// The tile of one product: pairs on 256 x 256, single CTAs on 128 x 128 or 128 x 64, whichever its waves cost
+// least, in SM cycles.  A k-block costs its L2 reads at 64 bytes a cycle (512 cycles for the wide two, the
+// pair's MMAs take as long), an output about 0.2 cycles of epilogue, overlapped but for the last; k splits
+// while SMs are left over and a part keeps at least four k-blocks.
 struct Tiling {
-    int bn, tiles_i, tiles_j, splits;
+    int bn, pair, tiles_i, tiles_j, splits;
 };
 Tiling tiling(long long I, int J, long long kbt) {
-    Tiling best{64, 0, 0, 1};
+    Tiling best{64, 0, 0, 0, 1};
     double least = 0;
     for (int bn : {256, 128, 64}) {
+        const int pair = bn == 256, ti = pair ? 256 : 128, units = pair ? SMS / 2 : SMS;
         if (bn > 64 && J <= bn / 2) continue;
-        const long long tiles = cdiv(I, BM) * cdiv(J, bn);
+        const long long tiles = cdiv(I, ti) * cdiv(J, bn);
         long long s = 1;
-        if (tiles < SMS) s = std::max<long long>(1, std::min<long long>(SMS / tiles, kbt / 4));
-        const double waves = (double)cdiv(tiles * s, SMS);
-        const double cost = waves * ((double)cdiv(kbt, s) * (bn + 32) + 3.0 * bn + 200);
+        if (tiles < units) s = std::max<long long>(1, std::min<long long>(units / tiles, kbt / 4));
+        const double waves = (double)cdiv(tiles * s, units);
+        const double k = (double)cdiv(kbt, s) * (bn == 64 ? 384 : 512), epi = 0.2 * 128 * bn;
+        const double cost = waves * std::max(k, epi) + std::min(k, epi) + 2000 + (s > 1 ? 4000 : 0);
         if (least == 0 || cost < least) {
             least = cost;
-            best = Tiling{bn, (int)cdiv(I, BM), (int)cdiv(J, bn), (int)s};
+            best = Tiling{bn, pair, (int)cdiv(I, ti), (int)cdiv(J, bn), (int)s};
         }
     }
     return best;
@@ -737,15 +819,44 @@ bool make_map(CUtensorMap *tm, CUtensorMapDataType type, int es, const void *bas
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int BN, bool OUT32>
+template <int BN, bool PAIR, bool OUT32, int EPI>
 int launch(const CUtensorMap *m, const GemmArgs &a, cudaStream_t s) {
-    using S = Shape<BN, OUT32>;
-    auto kern = k_gemm<BN, OUT32>;
+    using S = Shape<BN, PAIR, OUT32>;
+    auto kern = k_gemm<BN, PAIR, OUT32, EPI>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM) != cudaSuccess)
         return done("gs_linear_act");
     const int items = a.tiles_i * a.tiles_j * a.splits;
-    kern<<<std::min(items, SMS), 320, S::SMEM, s>>>(m[0], m[1], m[2], m[3], m[4], a);
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = PAIR ? 2 : 1;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t c;
+    memset(&c, 0, sizeof(c));
+    c.gridDim = dim3(PAIR ? 2 * std::min(items, SMS / 2) : std::min(items, SMS));
+    c.blockDim = dim3(320);
+    c.dynamicSmemBytes = S::SMEM;
+    c.stream = s;
+    c.attrs = at;
+    c.numAttrs = PAIR ? 1 : 0;
+    cudaLaunchKernelEx(&c, kern, m[0], m[1], m[2], m[3], m[4], a);
+    gs_count_launch(1);
     return GS_OK;
+}
+template <bool OUT32, int EPI>
+int launch_tile(int bn, const CUtensorMap *m, const GemmArgs &a, cudaStream_t s) {
+    return bn == 256   ? launch<256, true, OUT32, EPI>(m, a, s)
+           : bn == 128 ? launch<128, false, OUT32, EPI>(m, a, s)
+                       : launch<64, false, OUT32, EPI>(m, a, s);
+}
+template <bool OUT32>
+int launch_epi(int epi, int bn, const CUtensorMap *m, const GemmArgs &a, cudaStream_t s) {
+    switch (epi) {
+        case EPI_NONE: return launch_tile<OUT32, EPI_NONE>(bn, m, a, s);
+        case EPI_GELU: return launch_tile<OUT32, EPI_GELU>(bn, m, a, s);
+        case EPI_SILU: return launch_tile<OUT32, EPI_SILU>(bn, m, a, s);
+        case EPI_GELU_SLOPE: return launch_tile<OUT32, EPI_GELU_SLOPE>(bn, m, a, s);
+        default: return launch_tile<OUT32, EPI_SILU_SLOPE>(bn, m, a, s);
+    }
 }
 
 // one operand of a product: [terms][rows][cols], row stride ld
@@ -777,7 +888,7 @@ int product(const gs_linear_desc *d, const Plan &p, const Tiling &t, long long I
     CUtensorMap m[5];
     const CUtensorMapDataType in = a.f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     bool ok = make_map(&m[0], in, 2, A.p, A.cols, A.rows, A.ld, p.terms, 64, A.mn ? BK : BM) &&
-              make_map(&m[1], in, 2, B.p, B.cols, B.rows, B.ld, p.terms, 64, B.mn ? BK : t.bn);
+              make_map(&m[1], in, 2, B.p, B.cols, B.rows, B.ld, p.terms, 64, B.mn ? BK : t.pair ? t.bn / 2 : t.bn);
     m[2] = m[3] = m[4] = m[0];
     if (raw) {
         a.out_tma = 1;
@@ -785,7 +896,7 @@ int product(const gs_linear_desc *d, const Plan &p, const Tiling &t, long long I
     } else {
         const int es = f32 ? 4 : 2, ec = f32 ? 32 : 64;
         const CUtensorMapDataType ty = f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
-        a.bias = e.bias; a.residual = e.residual; a.ldr = e.ldr; a.act = e.act; a.out = e.out; a.slope = e.slope;
+        a.bias = e.bias; a.residual = e.residual; a.ldr = e.ldr; a.out = e.out; a.slope = e.slope;
         const auto whole = [&](const void *q, long long ld) { return ((uintptr_t)q & 15) == 0 && ld * es % 16 == 0; };
         a.out_tma = whole(e.out, J) && (!e.slope || whole(e.slope, J));
         a.res_tma = e.residual && whole(e.residual, e.ldr);
@@ -794,10 +905,9 @@ int product(const gs_linear_desc *d, const Plan &p, const Tiling &t, long long I
         if (a.res_tma) ok = ok && make_map(&m[4], ty, es, e.residual, J, I, e.ldr, 1, ec, 32);
     }
     if (!ok) return cuda_error("gs_linear_act", "cuTensorMapEncodeTiled refused a tensor");
-    gs_count_launch(1);
-    if (out32)
-        return t.bn == 256 ? launch<256, true>(m, a, s) : t.bn == 128 ? launch<128, true>(m, a, s) : launch<64, true>(m, a, s);
-    return t.bn == 256 ? launch<256, false>(m, a, s) : t.bn == 128 ? launch<128, false>(m, a, s) : launch<64, false>(m, a, s);
+    const int epi = raw || e.act == GS_ACT_NONE ? EPI_NONE : e.act == GS_ACT_GELU ? (e.slope ? EPI_GELU_SLOPE : EPI_GELU)
+                                                                                   : (e.slope ? EPI_SILU_SLOPE : EPI_SILU);
+    return out32 ? launch_epi<true>(epi, t.bn, m, a, s) : launch_epi<false>(epi, t.bn, m, a, s);
 }
 
 template <typename T>
