@@ -73,39 +73,44 @@ struct GemmArgs {
 __constant__ const unsigned char PAIR_A[6] = {2, 0, 1, 1, 0, 0}, PAIR_B[6] = {0, 2, 1, 0, 1, 0};
 
 // What an epilogue does with z = acc + bias: nothing, an activation, or an activation and its slope.
+constexpr int EPI_WARPS = 16, UNIT = 2048, GEMM_THREADS = 64 + 32 * EPI_WARPS;
 enum { EPI_NONE = 0, EPI_GELU = 1, EPI_SILU = 2, EPI_GELU_SLOPE = 3, EPI_SILU_SLOPE = 4 };
 
 // Persistent and warp-specialised, one CTA per SM.  Work item = a tile of D times a k split; CTAs (or pairs)
 // stride over the items, neighbours on neighbouring columns of the same rows (A from L2).
 //   warp 0   TMA producer: A and B k-blocks into a STAGES-deep ring of 128-byte-swizzled tiles
 //   warp 1   TMEM owner, MMA issuer; accumulators double-buffered, so the epilogue runs under the next item
-//   warps 2..9  epilogue: quarter warp % 4 of the CTA's 128 rows; half of the columns each (BN = 64: every
-//            second item).  A unit is 32 rows x 128 bytes of the output, staged in shared memory in the
-//            128-byte swizzle (a thread writes its row without bank conflicts) and moved by TMA; the residual
+//   warps 2..17 epilogue: quarter warp % 4 of the CTA's 128 rows; a quarter (BN = 256) or half (128) of the
+//            columns, and every second (128) or fourth (64) item.  16 warps, because two per scheduler left
+//            it idle 60 % of the time.  A unit is 32 rows x 64 bytes of the output, staged in shared memory in the
+//            64-byte swizzle (a thread writes its row without bank conflicts) and moved by TMA; the residual
 //            comes by TMA into the same place, a unit ahead, and is added in registers before the only rounding.
 // PAIR: two CTAs share a 256 x 256 tile (cta_group::2): each loads its 128 rows of A and half of B's rows, so an
 // output costs two thirds of the L2 reads of a 128 x 256 tile; that traffic, not the tensor cores, bounds large
 // products (a 128 x 256 tile read 13 TB/s from L2 at 1130 TFLOP/s).  The leader issues all MMAs.
 // Every wait is bounded; one that gives up records a code in g_wait_error and raises the CTA's abort flag.
-template <int BN, bool PAIR, bool OUT32>
+template <int BN, bool PAIR, bool OUT32, int EPI>
 struct Shape {
     static constexpr int BROWS = PAIR ? BN / 2 : BN;  // rows of B in this CTA
     static constexpr uint32_t A_BYTES = BM * BK * 2, B_BYTES = BROWS * BK * 2, STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = BROWS >= 128 ? 4 : 5;
-    static constexpr int CS = BN >= 128 ? 2 : 1;  // warps sharing a row quarter's columns
-    static constexpr int EC = OUT32 ? 32 : 64;    // columns of a unit
-    static constexpr int UNITS = BN / CS / EC;
-    static constexpr uint32_t SLOTS = 3 * 4096;  // per epilogue warp: two for outputs and residuals, one for slopes
-    static constexpr size_t SMEM = 1024 + STAGES * STAGE + 8 * SLOTS;
+    static constexpr int CS = BN / 64;                // warps sharing a row quarter's columns
+    static constexpr int PAR = 4 / CS;                // groups of warps taking turns at the items
+    static constexpr int NBUF = PAR > 2 ? PAR : 2;    // accumulators
+    static constexpr int EC = OUT32 ? 16 : 32;        // columns of a unit
+    static constexpr int UNITS = 64 / EC;
+    static constexpr bool SLOPE = EPI >= EPI_GELU_SLOPE;
+    static constexpr uint32_t SLOTS = (2 + SLOPE) * UNIT;  // per epilogue warp: two for outputs and residuals
+    static constexpr int STAGES = (229376 - EPI_WARPS * SLOTS) / STAGE;  // 4 to 6
+    static constexpr size_t SMEM = 1024 + STAGES * STAGE + EPI_WARPS * SLOTS;
     static constexpr int TILE_I = PAIR ? 2 * BM : BM;
 };
 
 struct Pipe {  // one CTA's barriers
-    uint64_t full[5], empty[5], tfull[2], tempty[2], mdone, rbar[8][2];
+    uint64_t full[6], empty[6], tfull[4], tempty[4], mdone, rbar[EPI_WARPS][2];
     uint32_t tmem_base;
     volatile int abort_flag;
     int issued, consumed;
-    __align__(16) float bias[8][32];  // read as float4
+    __align__(16) float bias[EPI_WARPS][16];  // read as float4
 };
 
 // row tile, column tile, split of an item
@@ -123,22 +128,27 @@ template <int BN, bool PAIR, bool OUT32, int EPI>
 __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ring_end, const CUtensorMap *tmO,
                                          const CUtensorMap *tmS, const CUtensorMap *tmR, int first, int stride, int n_items,
                                          int rank) {
-    using S = Shape<BN, PAIR, OUT32>;
+    using S = Shape<BN, PAIR, OUT32, EPI>;
     constexpr int EC = S::EC;
-    constexpr bool SLOPE = EPI >= EPI_GELU_SLOPE;
+    constexpr bool SLOPE = S::SLOPE;
     constexpr int ACT = EPI == EPI_NONE ? ACT_NONE : EPI == EPI_GELU || EPI == EPI_GELU_SLOPE ? ACT_GELU : ACT_SILU;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e = warp - 2, q = warp & 3, half = e >> 2;
-    uint8_t *const slots = ring_end + e * S::SLOTS, *const slo = slots + 2 * 4096;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e = warp - 2, q = warp & 3;
+    const int part = (e >> 2) % S::CS, turn = (e >> 2) / S::CS;
+    uint8_t *const slots = ring_end + e * S::SLOTS, *const slo = slots + 2 * UNIT;
     const uint32_t tbase = p.tmem_base + ((uint32_t)(q * 32) << 16);
     const bool has_res = a.residual != nullptr, res_tma = has_res && a.res_tma;
     const Act<ACT, SLOPE> act;
-    // this warp's items: all, or (BN = 64) those of its accumulator buffer
-    const int step = S::CS == 1 ? 2 * stride : stride;
-    int item = S::CS == 1 ? first + half * stride : first, tc = S::CS == 1 ? half : 0, use = 0;
+    const int step = S::PAR * stride;
+    int item = first + turn * stride, tc = turn, use = 0;
 
+    // byte of row r, column c in a unit: rows of 64 bytes, 16-byte chunks exchanged by the 64-byte swizzle
+    auto place_of = [](int r, int c) {
+        const int b = c * (OUT32 ? 4 : 2);
+        return r * 64 + (((b >> 4) ^ ((r >> 1) & 3)) << 4) + (b & 15);
+    };
     auto place = [&](int it, int u, int &col0, long long &row0) {
         const Item t(a, it);
-        col0 = t.j * BN + (S::CS == 2 ? half * (BN / 2) : 0) + u * EC;
+        col0 = t.j * BN + part * 64 + u * EC;
         row0 = (long long)t.i * S::TILE_I + rank * BM + q * 32;
         return col0 < a.J && row0 < a.I;
     };
@@ -150,25 +160,26 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ri
             for (; u < S::UNITS; u++)
                 if (place(it, u, col0, row0)) {
                     if (lane == 0) {
-                        mbar_arrive_expect_tx(&p.rbar[e][s], 4096);
-                        tma_load_3d(slots + s * 4096, tmR, &p.rbar[e][s], col0, (int)row0, 0);
+                        mbar_arrive_expect_tx(&p.rbar[e][s], UNIT);
+                        tma_load_3d(slots + s * UNIT, tmR, &p.rbar[e][s], col0, (int)row0, 0);
                     }
                     return true;
                 }
         return false;
     };
-    bool pending = res_tma && prefetch(item, 0, 0);  // a residual is on its way to slot use & 1
+    bool pending = res_tma && prefetch(item, 0, 0);  // a residual is on its way to the next unit's place
     bool dead = false;
-    for (; item < n_items && !dead; item += step, tc += S::CS == 1 ? 2 : 1) {
-        const int buf = tc & 1;
+    for (; item < n_items && !dead; item += step, tc += S::PAR) {
+        const int buf = tc % S::NBUF;
         const int sp = Item(a, item).s;
 #pragma unroll 1
         for (int u = 0; u < S::UNITS && !dead; u++) {
             int col0;
             long long row0;
             const bool live = place(item, u, col0, row0);
-            uint8_t *const out = slots + (use & 1) * 4096;
-            float bias[EC / 32];
+            const int sl = use & 1;
+            uint8_t *const out = slots + sl * UNIT;
+            float bias = 0.f;
             if (live) {
                 // the slots this unit writes are no longer read by their stores
                 if (lane == 0) {
@@ -177,60 +188,52 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ri
                 }
                 __syncwarp();
                 if (has_res && !res_tma) {
-                    for (int r = 0; r < 32 && row0 + r < a.I; r++)
-#pragma unroll
-                        for (int c = lane; c < EC; c += 32)
-                            if (col0 + c < a.J) {
+                    for (int r = lane / EC; r < 32 && row0 + r < a.I; r += 32 / EC)
+                        if (const int c = lane % EC; col0 + c < a.J) {
                                 const long long at = (row0 + r) * a.ldr + col0 + c;
-                                const int b = c * (128 / EC);
-                                uint8_t *d = out + r * 128 + ((b & ~15) ^ ((r & 7) << 4)) + (b & 15);
+                                uint8_t *d = out + place_of(r, c);
                                 if (OUT32) *reinterpret_cast<float *>(d) = reinterpret_cast<const float *>(a.residual)[at];
                                 else *reinterpret_cast<uint16_t *>(d) = reinterpret_cast<const uint16_t *>(a.residual)[at];
                             }
                     __syncwarp();
                 }
-#pragma unroll
-                for (int h = 0; h < EC / 32; h++) {
-                    const int c = col0 + 32 * h + lane;
-                    bias[h] = 0.f;
-                    if (a.bias && c < a.J)
-                        bias[h] = OUT32       ? reinterpret_cast<const float *>(a.bias)[c]
-                                  : a.out_f16 ? to_f32(reinterpret_cast<const __half *>(a.bias)[c])
-                                              : to_f32(reinterpret_cast<const __nv_bfloat16 *>(a.bias)[c]);
-                }
+                if (const int c = col0 + lane; a.bias && lane < EC && c < a.J)
+                    bias = OUT32       ? reinterpret_cast<const float *>(a.bias)[c]
+                               : a.out_f16 ? to_f32(reinterpret_cast<const __half *>(a.bias)[c])
+                                           : to_f32(reinterpret_cast<const __nv_bfloat16 *>(a.bias)[c]);
             }
             if (u == 0) {
-                if (!mbar_wait_or_abort(&p.tfull[buf], (tc >> 1) & 1, &p.abort_flag, &g_wait_error, 5)) dead = true;
+                if (!mbar_wait_or_abort(&p.tfull[buf], (tc / S::NBUF) & 1, &p.abort_flag, &g_wait_error, 5)) dead = true;
                 tc_fence_after();
             }
             if (live && pending) {
                 // (after an abort too: the copy lands in this CTA's shared memory)
-                if (!mbar_wait(&p.rbar[e][use & 1], (use >> 1) & 1, &g_wait_error, 6)) {
+                if (!mbar_wait(&p.rbar[e][sl], (use >> 1) & 1, &g_wait_error, 6)) {
                     p.abort_flag = 1;
                     dead = true;
                 }
                 pending = false;
             }
+            // 16 columns at a time
 #pragma unroll
-            for (int h = 0; h < EC / 32; h++) {
-                f2 v[16];
+            for (int h = 0; h < EC / 16; h++) {
+                f2 v[8];
                 if (live && !dead) {
-                    uint32_t r[32];
-                    const int lc = (S::CS == 2 ? half * (BN / 2) : 0) + u * EC + 32 * h;
-                    tmem_ld32(tbase + (uint32_t)(buf * BN + lc), r);
+                    uint32_t r[16];
+                    tmem_issue16(tbase + (uint32_t)(buf * BN + part * 64 + u * EC + 16 * h), r);
                     __syncwarp();
-                    p.bias[e][lane] = bias[h];
+                    if (lane >> 4 == h) p.bias[e][lane & 15] = bias;
                     __syncwarp();
-                    tmem_wait_ld32(r);
+                    tmem_wait16(r);
                     const float4 *b = reinterpret_cast<const float4 *>(p.bias[e]);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
+                    for (int i = 0; i < 4; i++) {
                         const float4 f = b[i];
                         v[2 * i] = add2({__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])}, {f.x, f.y});
                         v[2 * i + 1] = add2({__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3])}, {f.z, f.w});
                     }
                 }
-                if (u == S::UNITS - 1 && h == EC / 32 - 1) {  // the accumulator is drained
+                if (u == S::UNITS - 1 && h == EC / 16 - 1) {  // this warp's part of the accumulator is drained
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
@@ -239,33 +242,30 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ri
                     }
                 }
                 if (!live || dead) continue;
-                // 16 bytes of a row: chunk c of the unit, in the 128-byte swizzle
+                // 16 bytes of a row: chunk c of the unit
                 auto chunk = [&](uint8_t *base, int c) {
-                    return reinterpret_cast<uint4 *>(base + lane * 128 + ((c ^ (lane & 7)) << 4));
+                    return reinterpret_cast<uint4 *>(base + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4));
                 };
                 if (SLOPE) {
+                    f2 s[8];
 #pragma unroll
-                    for (int g = 0; g < 2; g++) {
-                        f2 s[8];
+                    for (int i = 0; i < 8; i++) v[i] = act(v[i], s[i]);
+                    if (OUT32) {
 #pragma unroll
-                        for (int i = 0; i < 8; i++) v[8 * g + i] = act(v[8 * g + i], s[i]);
-                        if (OUT32) {
+                        for (int i = 0; i < 4; i++) *chunk(slo, i) = pack16<float>(s + 2 * i);
+                    } else {
 #pragma unroll
-                            for (int i = 0; i < 4; i++) *chunk(slo, 4 * g + i) = pack16<float>(s + 2 * i);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 2; i++)
-                                *chunk(slo, 4 * h + 2 * g + i) = make_uint4(slope_codes(s[4 * i]), slope_codes(s[4 * i + 1]),
-                                                                            slope_codes(s[4 * i + 2]), slope_codes(s[4 * i + 3]));
-                        }
+                        for (int i = 0; i < 2; i++)
+                            *chunk(slo, 2 * h + i) = make_uint4(slope_codes(s[4 * i]), slope_codes(s[4 * i + 1]),
+                                                                slope_codes(s[4 * i + 2]), slope_codes(s[4 * i + 3]));
                     }
                 } else if (ACT != ACT_NONE) {
 #pragma unroll
-                    for (int i = 0; i < 16; i++) v[i] = act(v[i]);
+                    for (int i = 0; i < 8; i++) v[i] = act(v[i]);
                 }
                 if (OUT32) {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
+                    for (int i = 0; i < 4; i++) {
                         uint4 *c = chunk(out, i);
                         if (has_res) {
                             f2 f[2];
@@ -277,8 +277,8 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ri
                     }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        uint4 *c = chunk(out, 4 * h + i);
+                    for (int i = 0; i < 2; i++) {
+                        uint4 *c = chunk(out, 2 * h + i);
                         if (has_res) {
                             f2 f[4];
                             if (a.out_f16) unpack16<__half>(*c, f);
@@ -304,22 +304,19 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ri
                     bulk_commit();
                 }
             } else {
-                constexpr int ES = 128 / EC;  // bytes of an element
-                for (int r = 0; r < 32 && row0 + r < a.I; r++)
-#pragma unroll
-                    for (int c = lane; c < EC; c += 32)
-                        if (col0 + c < a.J) {
-                            const long long at = (row0 + r) * a.J + col0 + c;
-                            const int b = c * ES, off = r * 128 + ((b & ~15) ^ ((r & 7) << 4)) + (b & 15);
-                            if (OUT32) {
-                                reinterpret_cast<float *>(a.out)[at] = *reinterpret_cast<const float *>(out + off);
-                                if (SLOPE) reinterpret_cast<float *>(a.slope)[at] = *reinterpret_cast<const float *>(slo + off);
-                            } else {
-                                reinterpret_cast<uint16_t *>(a.out)[at] = *reinterpret_cast<const uint16_t *>(out + off);
-                                if (SLOPE)
-                                    reinterpret_cast<uint16_t *>(a.slope)[at] = *reinterpret_cast<const uint16_t *>(slo + off);
-                            }
+                for (int r = lane / EC; r < 32 && row0 + r < a.I; r += 32 / EC)
+                    if (const int c = lane % EC; col0 + c < a.J) {
+                        const long long at = (row0 + r) * a.J + col0 + c;
+                        const int off = place_of(r, c);
+                        if (OUT32) {
+                            reinterpret_cast<float *>(a.out)[at] = *reinterpret_cast<const float *>(out + off);
+                            if (SLOPE) reinterpret_cast<float *>(a.slope)[at] = *reinterpret_cast<const float *>(slo + off);
+                        } else {
+                            reinterpret_cast<uint16_t *>(a.out)[at] = *reinterpret_cast<const uint16_t *>(out + off);
+                            if (SLOPE)
+                                reinterpret_cast<uint16_t *>(a.slope)[at] = *reinterpret_cast<const uint16_t *>(slo + off);
                         }
+                    }
                 fence_proxy_async();  // the next residual's copy overwrites what was just read
                 __syncwarp();
             }
@@ -332,11 +329,11 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ri
 }
 
 template <int BN, bool PAIR, bool OUT32, int EPI>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(GEMM_THREADS, 1)
     k_gemm(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
            const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmS,
            const __grid_constant__ CUtensorMap tmR, const GemmArgs a) {
-    using S = Shape<BN, PAIR, OUT32>;
+    using S = Shape<BN, PAIR, OUT32, EPI>;
     constexpr int STAGES = S::STAGES;
     extern __shared__ uint8_t dsmem[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~(uintptr_t)1023);
@@ -350,9 +347,9 @@ __global__ void __launch_bounds__(320, 1)
 
     if (warp == 1) {
         if (PAIR) {
-            tmem_alloc_pair(&p.tmem_base, 2 * BN);
+            tmem_alloc_pair(&p.tmem_base, S::NBUF * BN);
         } else {
-            tmem_alloc(&p.tmem_base, 2 * BN);
+            tmem_alloc(&p.tmem_base, S::NBUF * BN);
             tmem_relinquish();
         }
     }
@@ -361,11 +358,11 @@ __global__ void __launch_bounds__(320, 1)
             mbar_init(&p.full[s], 1);
             mbar_init(&p.empty[s], 1);
         }
-        for (int j = 0; j < 2; j++) {
+        for (int j = 0; j < S::NBUF; j++) {
             mbar_init(&p.tfull[j], 1);
             mbar_init(&p.tempty[j], 4 * S::CS * (PAIR ? 2 : 1));
         }
-        for (int w = 0; w < 8; w++)
+        for (int w = 0; w < EPI_WARPS; w++)
             for (int j = 0; j < 2; j++) mbar_init(&p.rbar[w][j], 1);
         mbar_init(&p.mdone, 1);
         p.abort_flag = 0;
@@ -381,22 +378,20 @@ __global__ void __launch_bounds__(320, 1)
     tc_fence_after();
     const uint32_t tbase = p.tmem_base;
 
+    // (these two loops run in one thread each, and an instruction of theirs costs a few cycles: a stage's place,
+    // phase and descriptors are stepped, not computed)
     if (warp == 0) {
         if (lane == 0) {
-            int it = 0;
+            int it = 0, st = 0, parity = 1;  // of the ring's previous round; the first finds it complete
             for (int item = first; item < n_items && !p.abort_flag; item += stride) {
                 const Item t(a, item);
                 const int j0 = t.j * BN + (PAIR ? rank * S::BROWS : 0), i0 = t.i * S::TILE_I + rank * BM;
-                const int k1 = (int)((long long)kbt * (t.s + 1) / a.splits);
-                for (int k = (int)((long long)kbt * t.s / a.splits); k < k1; k++, it++) {
-                    const int st = it % STAGES;
-                    if (it >= STAGES && !mbar_wait_or_abort(&p.empty[st], ((it / STAGES) - 1) & 1, &p.abort_flag,
-                                                            &g_wait_error, 1))
-                        break;
-                    if (p.abort_flag) break;
+                int k = (int)((long long)kbt * t.s / a.splits), left = (int)((long long)kbt * (t.s + 1) / a.splits) - k;
+                int pr = k / a.kb, kk = (k - pr * a.kb) * BK;
+                int ta = a.npair > 1 ? PAIR_A[pr] : 0, tb = a.npair > 1 ? PAIR_B[pr] : 0;
+                for (; left > 0; left--, it++) {
+                    if (!mbar_wait_or_abort(&p.empty[st], parity, &p.abort_flag, &g_wait_error, 1)) break;
                     uint8_t *sa = smem + st * S::STAGE, *sb = sa + S::A_BYTES;
-                    const int pr = k / a.kb, kk = (k - pr * a.kb) * BK;
-                    const int ta = a.npair > 1 ? PAIR_A[pr] : 0, tb = a.npair > 1 ? PAIR_B[pr] : 0;
                     // both CTAs' copies complete on the leader's barrier
                     if (rank == 0) mbar_arrive_expect_tx(&p.full[st], S::STAGE * (PAIR ? 2 : 1));
                     const uint32_t bar = PAIR ? in_rank(&p.full[st], 0) : 0;
@@ -417,6 +412,17 @@ __global__ void __launch_bounds__(320, 1)
                         load(sb, &tmB, kk, j0, tb);
                     }
                     p.issued = it + 1;
+                    if (++st == STAGES) {
+                        st = 0;
+                        parity ^= 1;
+                    }
+                    kk += BK;
+                    if (kk == a.kb * BK && left > 1) {  // the next term product
+                        kk = 0;
+                        pr++;
+                        ta = PAIR_A[pr];
+                        tb = PAIR_B[pr];
+                    }
                 }
             }
         }
@@ -425,36 +431,46 @@ __global__ void __launch_bounds__(320, 1)
             const uint32_t fmt = a.f16 ? 0u : 1u;
             const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)a.a_mn << 15) |
                                    ((uint32_t)a.b_mn << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(S::TILE_I >> 4) << 24);
-            // per 16 of k: 32 bytes inside the swizzled row (K-major), two 8-row groups (MN-major)
-            const uint32_t stepA = a.a_mn ? 2048u : 32u, stepB = a.b_mn ? 2048u : 32u;
-            int it = 0, tc = 0;
+            // per 16 of k: 32 bytes inside the swizzled row (K-major), two 8-row groups (MN-major); in a
+            // descriptor's units of 16 bytes, whose low word holds the address
+            const uint64_t stepA = a.a_mn ? 128u : 2u, stepB = a.b_mn ? 128u : 2u;
+            const uint32_t s0 = smem_u32(smem);
+            const uint64_t descA = a.a_mn ? sdesc_mn(s0, 8192, 1024) : sdesc(s0, 1024, 2);
+            const uint64_t descB = a.b_mn ? sdesc_mn(s0 + S::A_BYTES, 8192, 1024) : sdesc(s0 + S::A_BYTES, 1024, 2);
+            int it = 0, tc = 0, st = 0, parity = 0;
             for (int item = first; item < n_items && !p.abort_flag; item += stride, tc++) {
                 const int s = Item(a, item).s;
-                const int k0 = (int)((long long)kbt * s / a.splits), k1 = (int)((long long)kbt * (s + 1) / a.splits);
-                const int buf = tc & 1;
-                if (tc >= 2 && !mbar_wait_or_abort(&p.tempty[buf], ((tc >> 1) - 1) & 1, &p.abort_flag, &g_wait_error, 2))
+                int left = (int)((long long)kbt * (s + 1) / a.splits) - (int)((long long)kbt * s / a.splits);
+                const int buf = tc % S::NBUF;
+                if (tc >= S::NBUF && !mbar_wait_or_abort(&p.tempty[buf], (tc / S::NBUF - 1) & 1, &p.abort_flag,
+                                                         &g_wait_error, 2))
                     break;
                 tc_fence_after();
                 const uint32_t dcol = tbase + (uint32_t)buf * BN;
                 bool ok = true;
-                for (int k = k0; k < k1; k++, it++) {
-                    const int st = it % STAGES;
-                    if (!mbar_wait_or_abort(&p.full[st], (it / STAGES) & 1, &p.abort_flag, &g_wait_error, 3)) {
+                uint32_t more = 0;
+                for (; left > 0; left--, it++) {
+                    if (!mbar_wait_or_abort(&p.full[st], parity, &p.abort_flag, &g_wait_error, 3)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t sa = smem_u32(smem + st * S::STAGE), sb = sa + S::A_BYTES;
+                    uint64_t ad = descA + (uint32_t)st * (S::STAGE >> 4), bd = descB + (uint32_t)st * (S::STAGE >> 4);
 #pragma unroll
                     for (int q = 0; q < BK / 16; q++) {
-                        const uint64_t ad = a.a_mn ? sdesc_mn(sa + stepA * q, 8192, 1024) : sdesc(sa + stepA * q, 1024, 2);
-                        const uint64_t bd = a.b_mn ? sdesc_mn(sb + stepB * q, 8192, 1024) : sdesc(sb + stepB * q, 1024, 2);
-                        if (PAIR) mma_pair(dcol, ad, bd, idesc, (k > k0 || q) ? 1u : 0u);
-                        else mma_bf16(dcol, ad, bd, idesc, (k > k0 || q) ? 1u : 0u);
+                        if (PAIR) mma_pair(dcol, ad, bd, idesc, more);
+                        else mma_bf16(dcol, ad, bd, idesc, more);
+                        more = 1;
+                        ad += stepA;
+                        bd += stepB;
                     }
                     if (PAIR) mma_commit_pair(&p.empty[st]);
                     else mma_commit(&p.empty[st]);
                     p.consumed = it + 1;
+                    if (++st == STAGES) {
+                        st = 0;
+                        parity ^= 1;
+                    }
                 }
                 if (!ok) break;
                 if (PAIR) mma_commit_pair(&p.tfull[buf]);
@@ -479,8 +495,8 @@ __global__ void __launch_bounds__(320, 1)
     if (PAIR) cluster_arrive_wait();
     tc_fence_after();
     if (warp == 1) {
-        if (PAIR) tmem_dealloc_pair(tbase, 2 * BN);
-        else tmem_dealloc(tbase, 2 * BN);
+        if (PAIR) tmem_dealloc_pair(tbase, S::NBUF * BN);
+        else tmem_dealloc(tbase, S::NBUF * BN);
     }
 }
 
@@ -539,61 +555,77 @@ struct DzArgs {
     float *colsum;  // [blocks][N], or NULL
     long long M, ldy;
     int N, ldp, cvec, rl;  // vectors of eight columns per block, row lanes
-    int vec;               // dy and slope rows lie on 16 bytes
 };
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_dz(DzArgs a) {
     __shared__ float buf[256 * 8];
     const int r = threadIdx.x / a.cvec, cv = threadIdx.x - r * a.cvec;
     const int c = (blockIdx.y * a.cvec + cv) * 8;
     const bool live = r < a.rl && c < a.ldp;
     const long long lo = a.M * blockIdx.x / gridDim.x, hi = a.M * (blockIdx.x + 1LL) / gridDim.x;
+    const T *dy = reinterpret_cast<const T *>(a.dy) + c, *slope = reinterpret_cast<const T *>(a.slope) + c;
     f2 s[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
-    if (live)
-#pragma unroll 2
-        for (long long m = lo + r; m < hi; m += a.rl) {
-            const T *p = reinterpret_cast<const T *>(a.dy) + m * a.ldy + c;
-            f2 v[4];
-            if (a.vec) {
-                unpack8<T>(*reinterpret_cast<const Raw8<T> *>(p), v);
+    // dy and its slope g (as the forward packed it), in row m
+    auto one = [&](long long m, const Raw8<T> &d, const Raw8<T> &g) {
+        f2 v[4];
+        unpack8<T>(d, v);
+        if (a.slope) {
+            f2 f[4];
+            if (sizeof(T) == 4) {
+                unpack8<T>(g, f);
             } else {
+                const uint32_t x[4] = {g.q[0].x, g.q[0].y, g.q[0].z, g.q[0].w};
 #pragma unroll
-                for (int i = 0; i < 8; i++) at(v, i) = c + i < a.N ? to_f32(p[i]) : 0.f;
-            }
-            if (a.slope) {
-                f2 g[4];
-                if (sizeof(T) == 4) {
-                    const float *q = reinterpret_cast<const float *>(a.slope) + m * a.N + c;
-                    if (a.vec) {
-                        unpack8<float>(*reinterpret_cast<const Raw8<float> *>(q), g);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) at(g, i) = c + i < a.N ? q[i] : 0.f;
-                    }
-                } else {
-                    const uint16_t *q = reinterpret_cast<const uint16_t *>(a.slope) + m * a.N + c;
-                    if (a.vec) {
-                        const uint4 w = *reinterpret_cast<const uint4 *>(q);
-                        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                        for (int i = 0; i < 8; i++) at(g, i) = slope_of(i & 1 ? x[i >> 1] >> 16 : x[i >> 1] & 0xffffu);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) at(g, i) = c + i < a.N ? slope_of(q[i]) : 0.f;
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) v[i] = mul2(v[i], g[i]);
+                for (int i = 0; i < 4; i++) f[i] = {slope_of(x[i] & 0xffffu), slope_of(x[i] >> 16)};
             }
 #pragma unroll
-            for (int i = 0; i < 4; i++) s[i] = add2(s[i], v[i]);
-            if (a.dz) {
-                if (sizeof(T) == 4)
-                    store_terms(v, reinterpret_cast<__nv_bfloat16 *>(a.dz) + m * a.ldp + c, a.M * a.ldp);
-                else
-                    *reinterpret_cast<Raw8<T> *>(reinterpret_cast<T *>(a.dz) + m * a.ldp + c) = pack8<T>(v);
-            }
+            for (int i = 0; i < 4; i++) v[i] = mul2(v[i], f[i]);  // (rounded: db's bits do not depend on dz being written)
         }
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[i] = add2(s[i], v[i]);
+        if (a.dz) {
+            if (sizeof(T) == 4)
+                store_terms(v, reinterpret_cast<__nv_bfloat16 *>(a.dz) + m * a.ldp + c, a.M * a.ldp);
+            else
+                *reinterpret_cast<Raw8<T> *>(reinterpret_cast<T *>(a.dz) + m * a.ldp + c) = pack8<T>(v);
+        }
+    };
+    auto fetch = [&](const T *p, Raw8<T> &o) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int k = 0; k < (int)sizeof(T) / 2; k++) o.q[k] = __ldcs(reinterpret_cast<const uint4 *>(p) + k);  // read once
+        } else {
+            union {
+                Raw8<T> q;
+                T e[8];
+            } u;
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (c + i < a.N) u.e[i] = p[i];
+                else from_f32(0.f, u.e[i]);  // (and 0 codes a finite slope)
+            o = u.q;
+        }
+    };
+    if (live) {
+        long long m = lo + r;
+        constexpr int R = 4;  // rows in flight
+        for (; m + (R - 1) * a.rl < hi; m += R * a.rl) {
+            Raw8<T> d[R], g[R];
+#pragma unroll
+            for (int k = 0; k < R; k++) {
+                fetch(dy + (m + k * a.rl) * a.ldy, d[k]);
+                if (a.slope) fetch(slope + (m + k * a.rl) * a.N, g[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < R; k++) one(m + k * a.rl, d[k], g[k]);
+        }
+        for (; m < hi; m += a.rl) {
+            Raw8<T> d, g;
+            fetch(dy + m * a.ldy, d);
+            if (a.slope) fetch(slope + m * a.N, g);
+            one(m, d, g);
+        }
+    }
     if (!a.colsum) return;
     const int w = a.cvec * 8;
     if (r < a.rl)
@@ -633,7 +665,7 @@ __global__ void __launch_bounds__(256) k_join(JoinArgs a) {
         const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = ((int)blockIdx.x - a.sum_blocks) * 32 + lane;
         float t = 0.f;
         if (c < a.ncol)
-#pragma unroll 4
+#pragma unroll 16
             for (int k = w; k < a.nsum; k += 8) t += a.colsum[(long long)k * a.ncol + c];
         red[w][lane] = t;
         __syncthreads();
@@ -652,7 +684,7 @@ __global__ void __launch_bounds__(256) k_join(JoinArgs a) {
         const int c = (int)(t - i * nv) * 4;
         const float *p = a.part + i * a.ldp + c;
         float4 s = *reinterpret_cast<const float4 *>(p);
-#pragma unroll 4
+#pragma unroll 8
         for (int k = 1; k < a.splits; k++) {
             const float4 e = *reinterpret_cast<const float4 *>(p + k * a.part_stride);
             s.x += e.x;
@@ -703,24 +735,27 @@ bool valid(const gs_linear_desc *d) {
 }
 
 // The tile of one product: pairs on 256 x 256, single CTAs on 128 x 128 or 128 x 64, whichever its waves cost
-// least, in SM cycles.  A k-block costs its L2 reads at 64 bytes a cycle (512 cycles for the wide two, the
-// pair's MMAs take as long), an output about 0.2 cycles of epilogue, overlapped but for the last; k splits
-// while SMs are left over and a part keeps at least four k-blocks.
+// least, in SM cycles as measured: a k-block 720, 600 and 590 (16384x4096->4096: 387, 569, 1099 us), a tile's
+// epilogue with GELU 12000, 5500 and 3700 (36864x128->512: 25.6, 23.3, 31.5 us), the shorter of the two
+// exposed once.  k splits while SMs are left over and a part keeps at least four k-blocks; their join costs a
+// launch and the parts' bytes.
 struct Tiling {
     int bn, pair, tiles_i, tiles_j, splits;
 };
 Tiling tiling(long long I, int J, long long kbt) {
     Tiling best{64, 0, 0, 0, 1};
     double least = 0;
-    for (int bn : {256, 128, 64}) {
-        const int pair = bn == 256, ti = pair ? 256 : 128, units = pair ? SMS / 2 : SMS;
+    const int widths[3] = {256, 128, 64};
+    const double block[3] = {720, 600, 590}, epi[3] = {12000, 5500, 3700};
+    for (int w = 0; w < 3; w++) {
+        const int bn = widths[w], pair = bn == 256, ti = pair ? 256 : 128, units = pair ? SMS / 2 : SMS;
         if (bn > 64 && J <= bn / 2) continue;
         const long long tiles = cdiv(I, ti) * cdiv(J, bn);
         long long s = 1;
         if (tiles < units) s = std::max<long long>(1, std::min<long long>(units / tiles, kbt / 4));
-        const double waves = (double)cdiv(tiles * s, units);
-        const double k = (double)cdiv(kbt, s) * (bn == 64 ? 384 : 512), epi = 0.2 * 128 * bn;
-        const double cost = waves * std::max(k, epi) + std::min(k, epi) + 2000 + (s > 1 ? 4000 : 0);
+        const double waves = (double)cdiv(tiles * s, units), k = (double)cdiv(kbt, s) * block[w];
+        const double join = s > 1 ? 3000 + (double)s * I * J * 8 / 3000 : 0;
+        const double cost = waves * std::max(k, epi[w]) + std::min(k, epi[w]) + join;
         if (least == 0 || cost < least) {
             least = cost;
             best = Tiling{bn, pair, (int)cdiv(I, ti), (int)cdiv(J, bn), (int)s};
@@ -807,21 +842,23 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     }();
     return fn;
 }
-// [terms][rows][cols] elements of es bytes with row stride ld: boxes of box_cols x box_rows, 128-byte swizzle
+// [terms][rows][cols] elements of es bytes with row stride ld: boxes of box_cols x box_rows, swizzled
 bool make_map(CUtensorMap *tm, CUtensorMapDataType type, int es, const void *base, long long cols, long long rows,
               long long ld, int terms, int box_cols, int box_rows) {
+    // rows of operand boxes are 128 bytes, of output and residual units 64
     const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)terms};
     const cuuint64_t str[2] = {(cuuint64_t)ld * es, (cuuint64_t)(terms > 1 ? rows : 1) * ld * es};
     const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1}, one[3] = {1, 1, 1};
     auto fn = encode_fn();
     return fn && fn(tm, type, 3, const_cast<void *>(base), dims, str, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    box_cols * es == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int BN, bool PAIR, bool OUT32, int EPI>
 int launch(const CUtensorMap *m, const GemmArgs &a, cudaStream_t s) {
-    using S = Shape<BN, PAIR, OUT32>;
+    using S = Shape<BN, PAIR, OUT32, EPI>;
     auto kern = k_gemm<BN, PAIR, OUT32, EPI>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM) != cudaSuccess)
         return done("gs_linear_act");
@@ -833,7 +870,7 @@ int launch(const CUtensorMap *m, const GemmArgs &a, cudaStream_t s) {
     cudaLaunchConfig_t c;
     memset(&c, 0, sizeof(c));
     c.gridDim = dim3(PAIR ? 2 * std::min(items, SMS / 2) : std::min(items, SMS));
-    c.blockDim = dim3(320);
+    c.blockDim = dim3(GEMM_THREADS);
     c.dynamicSmemBytes = S::SMEM;
     c.stream = s;
     c.attrs = at;
@@ -892,9 +929,9 @@ int product(const gs_linear_desc *d, const Plan &p, const Tiling &t, long long I
     m[2] = m[3] = m[4] = m[0];
     if (raw) {
         a.out_tma = 1;
-        ok = ok && make_map(&m[2], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, part, J, I, (J + 3) & ~3, t.splits, 32, 32);
+        ok = ok && make_map(&m[2], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, part, J, I, (J + 3) & ~3, t.splits, 16, 32);
     } else {
-        const int es = f32 ? 4 : 2, ec = f32 ? 32 : 64;
+        const int es = f32 ? 4 : 2, ec = f32 ? 16 : 32;
         const CUtensorMapDataType ty = f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
         a.bias = e.bias; a.residual = e.residual; a.ldr = e.ldr; a.out = e.out; a.slope = e.slope;
         const auto whole = [&](const void *q, long long ld) { return ((uintptr_t)q & 15) == 0 && ld * es % 16 == 0; };
@@ -985,9 +1022,12 @@ int backward(const gs_linear_desc *d, const Plan &p, const void *x, const void *
         Z.ld = p.ldn;
     }
     if (make_dz || db) {
-        DzArgs a{dy, slope, make_dz ? ws + p.o_dz : nullptr, colsum, d->M, d->ldy, d->N, p.ldn, p.dz_cvec, p.dz_rl, 0};
-        a.vec = !ragged(d->ldy, d->unaligned & 4) && d->N % 8 == 0 && ((uintptr_t)slope & 15) == 0;
-        k_dz<T><<<dim3((unsigned)p.dz_rows, (unsigned)p.dz_cols), 256, 0, s>>>(a);
+        const DzArgs a{dy, slope, make_dz ? ws + p.o_dz : nullptr, colsum, d->M, d->ldy, d->N, p.ldn, p.dz_cvec, p.dz_rl};
+        // whole 16-byte vectors of dy and of the kept slope
+        const bool vec = !ragged(d->ldy, d->unaligned & 4) && d->N % 8 == 0 && ((uintptr_t)slope & 15) == 0;
+        const dim3 grid((unsigned)p.dz_rows, (unsigned)p.dz_cols);
+        if (vec) k_dz<T, true><<<grid, 256, 0, s>>>(a);
+        else k_dz<T, false><<<grid, 256, 0, s>>>(a);
         gs_count_launch(1);
     }
     int st = GS_OK;
