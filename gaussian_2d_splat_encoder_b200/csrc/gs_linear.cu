@@ -122,6 +122,10 @@ struct Item {
         i = item % a.tiles_i;
         s = item / a.tiles_i;
     }
+    // its k-blocks, and how many it multiplies over all term products
+    __device__ __forceinline__ int from(const GemmArgs &a) const { return (int)((long long)a.kb * s / a.splits); }
+    __device__ __forceinline__ int to(const GemmArgs &a) const { return (int)((long long)a.kb * (s + 1) / a.splits); }
+    __device__ __forceinline__ int blocks(const GemmArgs &a) const { return (to(a) - from(a)) * a.npair; }
 };
 
 template <int BN, bool PAIR, bool OUT32, int EPI>
@@ -342,7 +346,6 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = PAIR ? (int)cluster_rank() : 0;
     const int first = PAIR ? blockIdx.x / 2 : blockIdx.x, stride = PAIR ? gridDim.x / 2 : gridDim.x;
-    const int kbt = a.kb * a.npair;
     const int n_items = a.tiles_i * a.tiles_j * a.splits;
 
     if (warp == 1) {
@@ -386,9 +389,9 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
             for (int item = first; item < n_items && !p.abort_flag; item += stride) {
                 const Item t(a, item);
                 const int j0 = t.j * BN + (PAIR ? rank * S::BROWS : 0), i0 = t.i * S::TILE_I + rank * BM;
-                int k = (int)((long long)kbt * t.s / a.splits), left = (int)((long long)kbt * (t.s + 1) / a.splits) - k;
-                int pr = k / a.kb, kk = (k - pr * a.kb) * BK;
-                int ta = a.npair > 1 ? PAIR_A[pr] : 0, tb = a.npair > 1 ? PAIR_B[pr] : 0;
+                const int k0 = t.from(a) * BK, k1 = t.to(a) * BK;
+                int kk = k0, pr = 0, left = t.blocks(a);
+                int ta = a.npair > 1 ? PAIR_A[0] : 0, tb = a.npair > 1 ? PAIR_B[0] : 0;
                 for (; left > 0; left--, it++) {
                     if (!mbar_wait_or_abort(&p.empty[st], parity, &p.abort_flag, &g_wait_error, 1)) break;
                     uint8_t *sa = smem + st * S::STAGE, *sb = sa + S::A_BYTES;
@@ -417,8 +420,8 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
                         parity ^= 1;
                     }
                     kk += BK;
-                    if (kk == a.kb * BK && left > 1) {  // the next term product
-                        kk = 0;
+                    if (kk == k1 && left > 1) {  // the next term product
+                        kk = k0;
                         pr++;
                         ta = PAIR_A[pr];
                         tb = PAIR_B[pr];
@@ -439,8 +442,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
             const uint64_t descB = a.b_mn ? sdesc_mn(s0 + S::A_BYTES, 8192, 1024) : sdesc(s0 + S::A_BYTES, 1024, 2);
             int it = 0, tc = 0, st = 0, parity = 0;
             for (int item = first; item < n_items && !p.abort_flag; item += stride, tc++) {
-                const int s = Item(a, item).s;
-                int left = (int)((long long)kbt * (s + 1) / a.splits) - (int)((long long)kbt * s / a.splits);
+                int left = Item(a, item).blocks(a);
                 const int buf = tc % S::NBUF;
                 if (tc >= S::NBUF && !mbar_wait_or_abort(&p.tempty[buf], (tc / S::NBUF - 1) & 1, &p.abort_flag,
                                                          &g_wait_error, 2))
@@ -524,11 +526,10 @@ __device__ __forceinline__ void store_terms(const f2 *v, __nv_bfloat16 *dst, lon
     *reinterpret_cast<uint4 *>(dst + 2 * term_stride) = pack16<__nv_bfloat16>(l);
 }
 template <typename T>
-__global__ void __launch_bounds__(256) k_prep_operand(PrepJob a, PrepJob b) {
-    const PrepJob &j = blockIdx.y ? b : a;
+__device__ __forceinline__ void prep_operand(const PrepJob &j, int block, int blocks) {
     const int nv = j.ldp / 8;
     const long long n = j.rows * nv;
-    for (long long t = blockIdx.x * 256LL + threadIdx.x; t < n; t += gridDim.x * 256LL) {
+    for (long long t = block * 256LL + threadIdx.x; t < n; t += blocks * 256LL) {
         const long long r = t / nv;
         const int c = (int)(t - r * nv) * 8;
         const T *p = reinterpret_cast<const T *>(j.src) + r * j.ld + c;
@@ -547,22 +548,38 @@ __global__ void __launch_bounds__(256) k_prep_operand(PrepJob a, PrepJob b) {
         }
     }
 }
+// the operands of one call that need it, x and W
+struct PrepJobs {
+    PrepJob job[2];
+    int n, blocks;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) k_prep_operands(const __grid_constant__ PrepJobs p) {
+    prep_operand<T>(p.job[blockIdx.y], blockIdx.x, gridDim.x);
+}
 
-// ---- dz = dy slope as an operand (dz NULL: not written, dy serves), and its column sums per block of rows
+// ---- dz = dy slope as an operand (dz NULL: not written, dy serves), and its column sums per block of rows.
+// Blocks from `rows` on prepare x and W for the backward's products: a launch less.
 struct DzArgs {
     const void *dy, *slope;
     void *dz;
     float *colsum;  // [blocks][N], or NULL
     long long M, ldy;
     int N, ldp, cvec, rl;  // vectors of eight columns per block, row lanes
+    int rows;              // blocks over the rows
+    PrepJobs prep;
 };
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) k_dz(DzArgs a) {
+__global__ void __launch_bounds__(256) k_dz(const __grid_constant__ DzArgs a) {
     __shared__ float buf[256 * 8];
+    if ((int)blockIdx.x >= a.rows) {
+        for (int k = blockIdx.y; k < a.prep.n; k += gridDim.y) prep_operand<T>(a.prep.job[k], blockIdx.x - a.rows, a.prep.blocks);
+        return;
+    }
     const int r = threadIdx.x / a.cvec, cv = threadIdx.x - r * a.cvec;
     const int c = (blockIdx.y * a.cvec + cv) * 8;
     const bool live = r < a.rl && c < a.ldp;
-    const long long lo = a.M * blockIdx.x / gridDim.x, hi = a.M * (blockIdx.x + 1LL) / gridDim.x;
+    const long long lo = a.M * blockIdx.x / a.rows, hi = a.M * (blockIdx.x + 1LL) / a.rows;
     const T *dy = reinterpret_cast<const T *>(a.dy) + c, *slope = reinterpret_cast<const T *>(a.slope) + c;
     f2 s[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
     // dy and its slope g (as the forward packed it), in row m
@@ -738,11 +755,13 @@ bool valid(const gs_linear_desc *d) {
 // least, in SM cycles as measured: a k-block 720, 600 and 590 (16384x4096->4096: 387, 569, 1099 us), a tile's
 // epilogue with GELU 12000, 5500 and 3700 (36864x128->512: 25.6, 23.3, 31.5 us), the shorter of the two
 // exposed once.  k splits while SMs are left over and a part keeps at least four k-blocks; their join costs a
-// launch and the parts' bytes.
+// launch and the parts' bytes.  In fp32 a part has at most FP32_CHAIN k-blocks: the accumulators cut what they
+// add up rather than round it (1.7e-6 of the result over 1536 terms, growing with their number); the join rounds.
+constexpr int FP32_CHAIN = 8;
 struct Tiling {
     int bn, pair, tiles_i, tiles_j, splits;
 };
-Tiling tiling(long long I, int J, long long kbt) {
+Tiling tiling(long long I, int J, long long kb, int npair) {
     Tiling best{64, 0, 0, 0, 1};
     double least = 0;
     const int widths[3] = {256, 128, 64};
@@ -752,8 +771,9 @@ Tiling tiling(long long I, int J, long long kbt) {
         if (bn > 64 && J <= bn / 2) continue;
         const long long tiles = cdiv(I, ti) * cdiv(J, bn);
         long long s = 1;
-        if (tiles < units) s = std::max<long long>(1, std::min<long long>(units / tiles, kbt / 4));
-        const double waves = (double)cdiv(tiles * s, units), k = (double)cdiv(kbt, s) * block[w];
+        if (tiles < units) s = std::max<long long>(1, std::min({units / tiles, kb * npair / 4, kb}));
+        if (npair > 1) s = std::max(s, cdiv(kb, FP32_CHAIN));
+        const double waves = (double)cdiv(tiles * s, units), k = (double)cdiv(kb, s) * npair * block[w];
         const double join = s > 1 ? 3000 + (double)s * I * J * 8 / 3000 : 0;
         const double cost = waves * std::max(k, epi[w]) + std::min(k, epi[w]) + join;
         if (least == 0 || cost < least) {
@@ -800,13 +820,13 @@ Plan plan(const gs_linear_desc *d, bool bwd) {
     p.o_x = take(p.prep_x ? (size_t)d->M * p.ldx * 2 * p.terms : 0);
     p.o_w = take(p.prep_w ? (size_t)d->N * p.ldw * 2 * p.terms : 0);
     if (!bwd) {
-        p.fwd = tiling(d->M, d->N, cdiv(d->K, BK) * p.npair);
+        p.fwd = tiling(d->M, d->N, cdiv(d->K, BK), p.npair);
         p.o_part = take(parts(p.fwd, d->M, d->N));
     } else {
         p.need_dz = f32 || d->act != GS_ACT_NONE || ragged(d->ldy, d->unaligned & 4);
         p.o_dz = take(p.need_dz ? (size_t)d->M * p.ldn * 2 * p.terms : 0);
-        p.gx = tiling(d->M, d->K, cdiv(d->N, BK) * p.npair);
-        p.gw = tiling(d->N, d->K, cdiv(d->M, BK) * p.npair);
+        p.gx = tiling(d->M, d->K, cdiv(d->N, BK), p.npair);
+        p.gw = tiling(d->N, d->K, cdiv(d->M, BK), p.npair);
         p.o_part = take(std::max(parts(p.gx, d->M, d->K), parts(p.gw, d->N, d->K)));
         // dz: blocks of 256 threads, up to 256 column vectors each, about four blocks per SM
         const int nv = p.ldn / 8;
@@ -948,14 +968,6 @@ int product(const gs_linear_desc *d, const Plan &p, const Tiling &t, long long I
 }
 
 template <typename T>
-void prep(const PrepJob *jobs, int n, cudaStream_t s) {
-    if (!n) return;
-    long long most = 0;
-    for (int k = 0; k < n; k++) most = std::max(most, jobs[k].rows * (jobs[k].ldp / 8));
-    k_prep_operand<T><<<dim3((unsigned)std::min<long long>(cdiv(most, 256), 16 * SMS), n), 256, 0, s>>>(jobs[0], jobs[n - 1]);
-    gs_count_launch(1);
-}
-template <typename T>
 void join(const Tiling *t, long long I, int J, const Epilogue &e, const void *part, const float *colsum, int ncol, int nsum,
           void *db, cudaStream_t s) {
     JoinArgs a;
@@ -975,25 +987,27 @@ void join(const Tiling *t, long long I, int J, const Epilogue &e, const void *pa
 
 char *base_of(void *ws) { return reinterpret_cast<char *>(al((uintptr_t)ws)); }
 
-// x and W as the products read them: in place, or prepared in the workspace
-template <typename T>
-void operands(const gs_linear_desc *d, const Plan &p, const void *x, const void *w, char *ws, bool want_x, bool want_w,
-              Operand &X, Operand &W, cudaStream_t s) {
-    PrepJob jobs[2];
-    int n = 0;
+// x and W as the products read them: in place, or prepared in the workspace by the jobs
+PrepJobs operands(const gs_linear_desc *d, const Plan &p, const void *x, const void *w, char *ws, bool want_x, bool want_w,
+                  Operand &X, Operand &W) {
+    PrepJobs jobs;
+    memset(&jobs, 0, sizeof(jobs));
     X = Operand{x, d->M, d->K, d->ldx, 0};
     W = Operand{w, d->N, d->K, d->ldw, 0};
     if (want_x && p.prep_x) {
-        jobs[n++] = PrepJob{x, ws + p.o_x, d->M, d->ldx, d->K, p.ldx};
+        jobs.job[jobs.n++] = PrepJob{x, ws + p.o_x, d->M, d->ldx, d->K, p.ldx};
         X.p = ws + p.o_x;
         X.ld = p.ldx;
     }
     if (want_w && p.prep_w) {
-        jobs[n++] = PrepJob{w, ws + p.o_w, d->N, d->ldw, d->K, p.ldw};
+        jobs.job[jobs.n++] = PrepJob{w, ws + p.o_w, d->N, d->ldw, d->K, p.ldw};
         W.p = ws + p.o_w;
         W.ld = p.ldw;
     }
-    prep<T>(jobs, n, s);
+    long long most = 0;
+    for (int k = 0; k < jobs.n; k++) most = std::max(most, jobs.job[k].rows * (jobs.job[k].ldp / 8));
+    jobs.blocks = (int)std::min<long long>(cdiv(most, 256), 8 * SMS);
+    return jobs;
 }
 
 template <typename T>
@@ -1001,7 +1015,11 @@ int forward(const gs_linear_desc *d, const Plan &p, const void *x, const void *w
             cudaStream_t s) {
     char *ws = base_of(workspace);
     Operand X, W;
-    operands<T>(d, p, x, w, ws, true, true, X, W, s);
+    const PrepJobs jobs = operands(d, p, x, w, ws, true, true, X, W);
+    if (jobs.n) {
+        k_prep_operands<T><<<dim3((unsigned)jobs.blocks, (unsigned)jobs.n), 256, 0, s>>>(jobs);
+        gs_count_launch(1);
+    }
     const int st = product(d, p, p.fwd, d->M, d->N, d->K, X, W, e, ws + p.o_part, s);
     if (st != GS_OK) return st;
     if (p.fwd.splits > 1) join<T>(&p.fwd, d->M, d->N, e, ws + p.o_part, nullptr, 0, 0, nullptr, s);
@@ -1013,7 +1031,7 @@ int backward(const gs_linear_desc *d, const Plan &p, const void *x, const void *
              void *dx, void *dw, void *db, void *workspace, cudaStream_t s) {
     char *ws = base_of(workspace);
     Operand X, W;
-    operands<T>(d, p, x, w, ws, dw != nullptr, dx != nullptr, X, W, s);
+    const PrepJobs jobs = operands(d, p, x, w, ws, dw != nullptr, dx != nullptr, X, W);
     Operand Z{dy, d->M, d->N, d->ldy, 0};
     const bool make_dz = p.need_dz && (dx || dw);
     float *colsum = db ? reinterpret_cast<float *>(ws + p.o_col) : nullptr;
@@ -1021,11 +1039,13 @@ int backward(const gs_linear_desc *d, const Plan &p, const void *x, const void *
         Z.p = ws + p.o_dz;
         Z.ld = p.ldn;
     }
-    if (make_dz || db) {
-        const DzArgs a{dy, slope, make_dz ? ws + p.o_dz : nullptr, colsum, d->M, d->ldy, d->N, p.ldn, p.dz_cvec, p.dz_rl};
+    const bool rows = make_dz || db;
+    if (rows || jobs.n) {
+        const DzArgs a{dy, slope, make_dz ? ws + p.o_dz : nullptr, colsum, d->M, d->ldy, d->N, p.ldn, p.dz_cvec, p.dz_rl,
+                       rows ? p.dz_rows : 0, jobs};
         // whole 16-byte vectors of dy and of the kept slope
         const bool vec = !ragged(d->ldy, d->unaligned & 4) && d->N % 8 == 0 && ((uintptr_t)slope & 15) == 0;
-        const dim3 grid((unsigned)p.dz_rows, (unsigned)p.dz_cols);
+        const dim3 grid((unsigned)(a.rows + jobs.blocks), (unsigned)(rows ? p.dz_cols : 1));
         if (vec) k_dz<T, true><<<grid, 256, 0, s>>>(a);
         else k_dz<T, false><<<grid, 256, 0, s>>>(a);
         gs_count_launch(1);

@@ -201,6 +201,23 @@ def test_linear_long_sums(ops):
         linear_case(ops, x, w, rand(20, seed=58, dtype=dtype), None, "gelu", rand(70001, 20, seed=59, dtype=dtype, shift=0.1))
 
 
+@pytest.mark.parametrize("M,K,N", [(70000, 200, 300), (300, 4096, 130), (600, 150, 4096)])
+def test_linear_fp32_keeps_fp32_accuracy(ops, M, K, N):
+    """Long sums in each of the three products: in norm within 2e-6, 32 roundings' worth (u = 2^-24), however
+    long the sum."""
+    x, w, b = rand(M, K, seed=300), rand(N, K, seed=301, scale=K ** -0.5), rand(N, seed=302)
+    dy = rand(M, N, seed=303)
+    ts = [t.requires_grad_(True) for t in (x, w, b)]
+    y = ops.linear_act(*ts, act="gelu")
+    grads = torch.autograd.grad(y, ts, dy)
+    ds = [t.detach().double().requires_grad_(True) for t in ts]
+    Y = torch.nn.functional.gelu(ds[0] @ ds[1].t() + ds[2])
+    ref = torch.autograd.grad(Y, ds, dy.double())
+    for name, a, e in zip(("y", "dx", "dw", "db"), (y.detach(), *grads), (Y.detach(), *ref)):
+        rel = float((a.double() - e).norm() / e.norm())
+        assert rel <= 2e-6, (name, rel)
+
+
 def test_linear_nan_stays_in_its_row(ops):
     for dtype in TYPES:
         x, w, b = rand(300, 72, seed=60, dtype=dtype), rand(40, 72, seed=61, dtype=dtype), rand(40, seed=62, dtype=dtype)
