@@ -162,6 +162,13 @@ class _GroupNormAct(torch.autograd.Function):
     backward = staticmethod(once_differentiable(_norm_backward))
 
 
+def _check_param(name, p, x, channels):
+    if p.dim() != 1 or p.shape[0] != channels:
+        raise ValueError(f"{name} must be [{channels}], got {tuple(p.shape)}")
+    if p.dtype != torch.float32 and p.dtype != x.dtype:
+        raise ValueError(f"{name} must be float32 or {x.dtype}, got {p.dtype}")
+
+
 def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None,
                    bias: torch.Tensor | None = None, eps: float = 1e-5, *, act: str = "none",
                    act_first: bool = False) -> torch.Tensor:
@@ -187,23 +194,21 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
         raise ValueError(f"at most 2048 channels, got {channels}")
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    for name, p in (("weight", weight), ("bias", bias)):
-        if p is None:
-            continue
-        if p.shape != (channels,):
-            raise ValueError(f"{name} must be [{channels}], got {tuple(p.shape)}")
-        if p.dtype != x.dtype and p.dtype != torch.float32:
-            raise ValueError(f"{name} must be float32 or {x.dtype}, got {p.dtype}")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise ValueError(f"weight and bias must be of one type, got {weight.dtype} and {bias.dtype}")
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
+    grad = x.requires_grad
+    if weight is not None:
+        _check_param("weight", weight, x, channels)
+        grad, weight = grad or weight.requires_grad, weight.contiguous()
+    if bias is not None:
+        _check_param("bias", bias, x, channels)
+        grad, bias = grad or bias.requires_grad, bias.contiguous()
+        if weight is not None and weight.dtype != bias.dtype:
+            raise ValueError(f"weight and bias must be of one type, got {weight.dtype} and {bias.dtype}")
     args = (x, weight, bias, num_groups, float(eps), code, int(bool(act_first)))
     if x.numel() == 0:
         # nothing to normalise; the graph stays connected, with zero gradients
         y = torch.empty(x.shape, dtype=x.dtype, device=dev)
         return y + sum((p.sum() * 0).to(x.dtype) for p in (x, weight, bias) if p is not None)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if grad and torch.is_grad_enabled():
         return _GroupNormAct.apply(*args)
     return _norm_forward(*args, False)[0]
 
@@ -315,10 +320,13 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
         raise ValueError(f"bias must be [{N}], got {tuple(bias.shape)}")
     if residual is not None and residual.shape != x.shape[:-1] + (N,):
         raise ValueError(f"residual must be {tuple(x.shape[:-1] + (N,))}, got {tuple(residual.shape)}")
+    grad = x.requires_grad or weight.requires_grad
     for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):
-        if t is not None and t.dtype != x.dtype:
-            raise ValueError(f"{name} must be {x.dtype} like x, got {t.dtype}")
+        if t is not None:
+            if t.dtype != x.dtype:
+                raise ValueError(f"{name} must be {x.dtype} like x, got {t.dtype}")
+            grad = grad or t.requires_grad
     bias = None if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if grad and torch.is_grad_enabled():
         return _LinearAct.apply(x, weight, bias, residual, code)
     return _linear_forward(x, weight, bias, residual, code, False)[0]

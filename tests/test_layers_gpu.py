@@ -33,7 +33,8 @@ def norm_case(ops, x, G, w, b, act, first, dy, eps=1e-5):
 
 NORM_SHAPES = [((1, 16, 16, 256), 8), ((2, 7, 5, 24), 3), ((3, 61, 47, 120), 6), ((1, 1, 8), 8), ((1, 1, 1), 1),
                ((2, 3, 33), 11), ((1, 40, 2048), 1), ((1, 100, 512), 512), ((5, 1, 1, 64), 8), ((3, 64), 4),
-               ((70, 9, 16), 16), ((1, 3001, 7), 7), ((1, 33, 1000), 40), ((2, 50, 2047), 23), ((1, 2500, 2), 1)]
+               ((70, 9, 16), 16), ((1, 3001, 7), 7), ((1, 33, 1000), 40), ((2, 50, 2047), 23), ((1, 2500, 2), 1),
+               ((2, 30, 72), 9), ((1, 5000, 40), 5)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
