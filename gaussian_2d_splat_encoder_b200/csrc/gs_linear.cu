@@ -755,7 +755,7 @@ bool valid(const gs_linear_desc *d) {
 // least, in SM cycles as measured: a k-block 720, 600 and 590 (16384x4096->4096: 387, 569, 1099 us), a tile's
 // epilogue with GELU 12000, 5500 and 3700 (36864x128->512: 25.6, 23.3, 31.5 us), the shorter of the two
 // exposed once.  k splits while SMs are left over and a part keeps at least four k-blocks; their join costs a
-// launch and the parts' bytes.  In fp32 a part has at most FP32_CHAIN k-blocks: the accumulators cut what they
+// launch, 5 us of the host's time, and the parts' bytes.  In fp32 a part has at most FP32_CHAIN k-blocks: the accumulators cut what they
 // add up rather than round it (1.7e-6 of the result over 1536 terms, growing with their number); the join rounds.
 constexpr int FP32_CHAIN = 8;
 struct Tiling {
@@ -770,15 +770,17 @@ Tiling tiling(long long I, int J, long long kb, int npair) {
         const int bn = widths[w], pair = bn == 256, ti = pair ? 256 : 128, units = pair ? SMS / 2 : SMS;
         if (bn > 64 && J <= bn / 2) continue;
         const long long tiles = cdiv(I, ti) * cdiv(J, bn);
-        long long s = 1;
-        if (tiles < units) s = std::max<long long>(1, std::min({units / tiles, kb * npair / 4, kb}));
-        if (npair > 1) s = std::max(s, cdiv(kb, FP32_CHAIN));
-        const double waves = (double)cdiv(tiles * s, units), k = (double)cdiv(kb, s) * npair * block[w];
-        const double join = s > 1 ? 3000 + (double)s * I * J * 8 / 3000 : 0;
-        const double cost = waves * std::max(k, epi[w]) + std::min(k, epi[w]) + join;
-        if (least == 0 || cost < least) {
-            least = cost;
-            best = Tiling{bn, pair, (int)cdiv(I, ti), (int)cdiv(J, bn), (int)s};
+        // unsplit (in fp32 as few parts as the chain allows), or one part for every idle SM
+        const long long few = npair > 1 ? cdiv(kb, FP32_CHAIN) : 1;
+        const long long many = tiles < units ? std::min({units / tiles, kb * npair / 4, kb}) : 1;
+        for (long long s : {few, std::max(few, many)}) {
+            const double waves = (double)cdiv(tiles * s, units), k = (double)cdiv(kb, s) * npair * block[w];
+            const double join = s > 1 ? 9000 + (double)s * I * J * 8 / 3000 : 0;
+            const double cost = waves * std::max(k, epi[w]) + std::min(k, epi[w]) + join;
+            if (least == 0 || cost < least) {
+                least = cost;
+                best = Tiling{bn, pair, (int)cdiv(I, ti), (int)cdiv(J, bn), (int)s};
+            }
         }
     }
     return best;
