@@ -386,6 +386,38 @@ def test_captured_and_replayed(ops):
             assert all(torch.equal(u, v) for u, v in zip(out, ref))
 
 
+def test_offsets_past_32_bits(ops):
+    """Maps of more than 2^31 elements: the last rows against a call on those rows alone (both within one bf16
+    rounding of the same value, so at most a step of 2^-7 apart)."""
+    x = torch.empty(3, 1 << 20, 704, device="cuda", dtype=torch.bfloat16)
+    x[:2].fill_(0.5)
+    x[2] = rand(1 << 20, 704, seed=120, dtype=torch.bfloat16)
+    w = rand(704, seed=121, shift=1.0)
+    xr = x.requires_grad_(True)
+    y = ops.group_norm_act(xr, 8, w, act="gelu")
+    (dx,) = torch.autograd.grad(y, xr, y.detach())
+    tail = x.detach()[2:].clone().requires_grad_(True)
+    yt = ops.group_norm_act(tail, 8, w, act="gelu")
+    (dt,) = torch.autograd.grad(yt, tail, yt.detach())
+    for a, e in ((y[2, -99999:], yt[0, -99999:]), (dx[2, -99999:], dt[0, -99999:])):
+        assert torch.allclose(a.float(), e.float(), rtol=2 ** -6, atol=2 ** -6)
+    del y, dx, yt, dt, tail, xr, x
+    torch.cuda.empty_cache()
+    M = (1 << 21) + 77
+    x, w = rand(M, 16, seed=122, dtype=torch.bfloat16), rand(1048, 16, seed=123, dtype=torch.bfloat16)
+    xr = x.requires_grad_(True)
+    y = ops.linear_act(xr, w, act="silu")
+    (dx,) = torch.autograd.grad(y, xr, y.detach())
+    tail = x.detach()[-1000:].clone().requires_grad_(True)
+    yt = ops.linear_act(tail, w, act="silu")
+    (dt,) = torch.autograd.grad(yt, tail, yt.detach())
+    assert torch.equal(y[-1000:], yt)
+    # the same rounded dz in both; fp32 sums of 1048 terms of some 10 in another order, then one rounding each
+    assert torch.allclose(dx[-1000:].float(), dt.float(), rtol=2 ** -6, atol=0.05)
+    del y, dx, x, xr
+    torch.cuda.empty_cache()
+
+
 def test_refusals_on_the_device(ops):
     x = rand(2, 4, 16, seed=110)
     with pytest.raises(ValueError, match="divide"):
