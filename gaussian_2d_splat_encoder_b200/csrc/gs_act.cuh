@@ -196,3 +196,33 @@ __device__ __forceinline__ Raw8<T> pack8(const f2 *v) {
 // element i of a vector of pairs
 __device__ __forceinline__ float &at(f2 *v, int i) { return i & 1 ? v[i >> 1].y : v[i >> 1].x; }
 __device__ __forceinline__ float at(const f2 *v, int i) { return i & 1 ? v[i >> 1].y : v[i >> 1].x; }
+
+// ---- launches of one call that follow each other (programmatic dependent launch): the first lets its follower
+// be set up early, the follower waits here until the kernel before it has finished and its writes are visible.
+// Every block of a follower waits, so a chain's end implies its beginning.
+__device__ __forceinline__ void gs_let_follow() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void gs_wait_leader() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// launches kern; follows: as the follower of the launch before it on the stream; cluster: CTAs per cluster
+template <typename K, typename... A>
+inline void gs_launch(K kern, dim3 grid, int threads, size_t smem, cudaStream_t s, bool follows, int cluster,
+                      const A &...args) {
+    cudaLaunchAttribute at[2];
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid;
+    c.blockDim = dim3((unsigned)threads);
+    c.dynamicSmemBytes = smem;
+    c.stream = s;
+    c.attrs = at;
+    if (follows) {
+        at[c.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[c.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        at[c.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        at[c.numAttrs].val.clusterDim.x = (unsigned)cluster;
+        at[c.numAttrs].val.clusterDim.y = at[c.numAttrs].val.clusterDim.z = 1;
+        c.numAttrs++;
+    }
+    cudaLaunchKernelEx(&c, kern, args...);
+}

@@ -175,12 +175,13 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ri
     bool dead = false;
     for (; item < n_items && !dead; item += step, tc += S::PAR) {
         const int buf = tc % S::NBUF;
-        const int sp = Item(a, item).s;
+        const Item tile(a, item);
+        const int sp = tile.s, base = tile.j * BN + part * 64;
+        const long long row0 = (long long)tile.i * S::TILE_I + rank * BM + q * 32;
 #pragma unroll 1
         for (int u = 0; u < S::UNITS && !dead; u++) {
-            int col0;
-            long long row0;
-            const bool live = place(item, u, col0, row0);
+            const int col0 = base + u * EC;
+            const bool live = col0 < a.J && row0 < a.I;
             const int sl = use & 1;
             uint8_t *const out = slots + sl * UNIT;
             float bias = 0.f;
@@ -375,6 +376,8 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
         prefetch_tensormap(&tmA);
         prefetch_tensormap(&tmB);
     }
+    gs_let_follow();
+    gs_wait_leader();  // operands and residents of the workspace come from the launch before
     tc_fence_before();
     __syncthreads();
     if (PAIR) cluster_arrive_wait();  // both CTAs' barriers exist
@@ -555,6 +558,7 @@ struct PrepJobs {
 };
 template <typename T>
 __global__ void __launch_bounds__(256) k_prep_operands(const __grid_constant__ PrepJobs p) {
+    gs_let_follow();
     prep_operand<T>(p.job[blockIdx.y], blockIdx.x, gridDim.x);
 }
 
@@ -572,6 +576,7 @@ struct DzArgs {
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_dz(const __grid_constant__ DzArgs a) {
     __shared__ float buf[256 * 8];
+    gs_let_follow();
     if ((int)blockIdx.x >= a.rows) {
         for (int k = blockIdx.y; k < a.prep.n; k += gridDim.y) prep_operand<T>(a.prep.job[k], blockIdx.x - a.rows, a.prep.blocks);
         return;
@@ -677,6 +682,8 @@ struct JoinArgs {
 };
 template <typename T>
 __global__ void __launch_bounds__(256) k_join(JoinArgs a) {
+    gs_let_follow();
+    gs_wait_leader();
     if ((int)blockIdx.x >= a.sum_blocks) {
         __shared__ float red[8][33];
         const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = ((int)blockIdx.x - a.sum_blocks) * 32 + lane;
@@ -879,42 +886,31 @@ bool make_map(CUtensorMap *tm, CUtensorMapDataType type, int es, const void *bas
 }
 
 template <int BN, bool PAIR, bool OUT32, int EPI>
-int launch(const CUtensorMap *m, const GemmArgs &a, cudaStream_t s) {
+int launch(const CUtensorMap *m, const GemmArgs &a, bool follows, cudaStream_t s) {
     using S = Shape<BN, PAIR, OUT32, EPI>;
     auto kern = k_gemm<BN, PAIR, OUT32, EPI>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM) != cudaSuccess)
         return done("gs_linear_act");
     const int items = a.tiles_i * a.tiles_j * a.splits;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = PAIR ? 2 : 1;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cudaLaunchConfig_t c;
-    memset(&c, 0, sizeof(c));
-    c.gridDim = dim3(PAIR ? 2 * std::min(items, SMS / 2) : std::min(items, SMS));
-    c.blockDim = dim3(GEMM_THREADS);
-    c.dynamicSmemBytes = S::SMEM;
-    c.stream = s;
-    c.attrs = at;
-    c.numAttrs = PAIR ? 1 : 0;
-    cudaLaunchKernelEx(&c, kern, m[0], m[1], m[2], m[3], m[4], a);
+    gs_launch(kern, dim3(PAIR ? 2 * std::min(items, SMS / 2) : std::min(items, SMS)), GEMM_THREADS, S::SMEM, s, follows,
+              PAIR ? 2 : 1, m[0], m[1], m[2], m[3], m[4], a);
     gs_count_launch(1);
     return GS_OK;
 }
 template <bool OUT32, int EPI>
-int launch_tile(int bn, const CUtensorMap *m, const GemmArgs &a, cudaStream_t s) {
-    return bn == 256   ? launch<256, true, OUT32, EPI>(m, a, s)
-           : bn == 128 ? launch<128, false, OUT32, EPI>(m, a, s)
-                       : launch<64, false, OUT32, EPI>(m, a, s);
+int launch_tile(int bn, const CUtensorMap *m, const GemmArgs &a, bool follows, cudaStream_t s) {
+    return bn == 256   ? launch<256, true, OUT32, EPI>(m, a, follows, s)
+           : bn == 128 ? launch<128, false, OUT32, EPI>(m, a, follows, s)
+                       : launch<64, false, OUT32, EPI>(m, a, follows, s);
 }
 template <bool OUT32>
-int launch_epi(int epi, int bn, const CUtensorMap *m, const GemmArgs &a, cudaStream_t s) {
+int launch_epi(int epi, int bn, const CUtensorMap *m, const GemmArgs &a, bool follows, cudaStream_t s) {
     switch (epi) {
-        case EPI_NONE: return launch_tile<OUT32, EPI_NONE>(bn, m, a, s);
-        case EPI_GELU: return launch_tile<OUT32, EPI_GELU>(bn, m, a, s);
-        case EPI_SILU: return launch_tile<OUT32, EPI_SILU>(bn, m, a, s);
-        case EPI_GELU_SLOPE: return launch_tile<OUT32, EPI_GELU_SLOPE>(bn, m, a, s);
-        default: return launch_tile<OUT32, EPI_SILU_SLOPE>(bn, m, a, s);
+        case EPI_NONE: return launch_tile<OUT32, EPI_NONE>(bn, m, a, follows, s);
+        case EPI_GELU: return launch_tile<OUT32, EPI_GELU>(bn, m, a, follows, s);
+        case EPI_SILU: return launch_tile<OUT32, EPI_SILU>(bn, m, a, follows, s);
+        case EPI_GELU_SLOPE: return launch_tile<OUT32, EPI_GELU_SLOPE>(bn, m, a, follows, s);
+        default: return launch_tile<OUT32, EPI_SILU_SLOPE>(bn, m, a, follows, s);
     }
 }
 
@@ -933,7 +929,7 @@ struct Epilogue {
 
 // D [I][J] over k = K; with splits the parts go to `part` and the caller joins them
 int product(const gs_linear_desc *d, const Plan &p, const Tiling &t, long long I, int J, long long K, const Operand &A,
-            const Operand &B, const Epilogue &e, void *part, cudaStream_t s) {
+            const Operand &B, const Epilogue &e, void *part, bool follows, cudaStream_t s) {
     GemmArgs a;
     memset(&a, 0, sizeof(a));
     const bool f32 = d->dtype == GS_F32, raw = t.splits > 1, out32 = f32 || raw;
@@ -966,7 +962,7 @@ int product(const gs_linear_desc *d, const Plan &p, const Tiling &t, long long I
     if (!ok) return cuda_error("gs_linear_act", "cuTensorMapEncodeTiled refused a tensor");
     const int epi = raw || e.act == GS_ACT_NONE ? EPI_NONE : e.act == GS_ACT_GELU ? (e.slope ? EPI_GELU_SLOPE : EPI_GELU)
                                                                                    : (e.slope ? EPI_SILU_SLOPE : EPI_SILU);
-    return out32 ? launch_epi<true>(epi, t.bn, m, a, s) : launch_epi<false>(epi, t.bn, m, a, s);
+    return out32 ? launch_epi<true>(epi, t.bn, m, a, follows, s) : launch_epi<false>(epi, t.bn, m, a, follows, s);
 }
 
 template <typename T>
@@ -983,7 +979,7 @@ void join(const Tiling *t, long long I, int J, const Epilogue &e, const void *pa
     a.colsum = colsum; a.ncol = ncol; a.nsum = nsum; a.db = db;
     const int fold = db ? (int)cdiv(ncol, 32) : 0;
     if (a.sum_blocks + fold == 0) return;
-    k_join<T><<<a.sum_blocks + fold, 256, 0, s>>>(a);
+    gs_launch(k_join<T>, dim3((unsigned)(a.sum_blocks + fold)), 256, 0, s, true, 1, a);  // (a product or dz came before)
     gs_count_launch(1);
 }
 
@@ -1022,7 +1018,7 @@ int forward(const gs_linear_desc *d, const Plan &p, const void *x, const void *w
         k_prep_operands<T><<<dim3((unsigned)jobs.blocks, (unsigned)jobs.n), 256, 0, s>>>(jobs);
         gs_count_launch(1);
     }
-    const int st = product(d, p, p.fwd, d->M, d->N, d->K, X, W, e, ws + p.o_part, s);
+    const int st = product(d, p, p.fwd, d->M, d->N, d->K, X, W, e, ws + p.o_part, jobs.n > 0, s);
     if (st != GS_OK) return st;
     if (p.fwd.splits > 1) join<T>(&p.fwd, d->M, d->N, e, ws + p.o_part, nullptr, 0, 0, nullptr, s);
     return done("gs_linear_act_fwd");
@@ -1052,12 +1048,13 @@ int backward(const gs_linear_desc *d, const Plan &p, const void *x, const void *
         else k_dz<T, false><<<grid, 256, 0, s>>>(a);
         gs_count_launch(1);
     }
+    const bool first = rows || jobs.n;  // a launch of this call came before the products
     int st = GS_OK;
     if (dx) {
         Operand B = W;
         B.mn = 1;
         const Epilogue e{nullptr, nullptr, 0, 0, dx, nullptr};
-        st = product(d, p, p.gx, d->M, d->K, d->N, Z, B, e, ws + p.o_part, s);
+        st = product(d, p, p.gx, d->M, d->K, d->N, Z, B, e, ws + p.o_part, first, s);
         if (st != GS_OK) return st;
         if (p.gx.splits > 1) join<T>(&p.gx, d->M, d->K, e, ws + p.o_part, nullptr, 0, 0, nullptr, s);
     }
@@ -1065,7 +1062,7 @@ int backward(const gs_linear_desc *d, const Plan &p, const void *x, const void *
     if (dw) {
         Operand A = Z, B = X;
         A.mn = B.mn = 1;
-        st = product(d, p, p.gw, d->N, d->K, d->M, A, B, e, ws + p.o_part, s);
+        st = product(d, p, p.gw, d->N, d->K, d->M, A, B, e, ws + p.o_part, first || dx, s);
         if (st != GS_OK) return st;
     }
     join<T>(dw && p.gw.splits > 1 ? &p.gw : nullptr, d->N, d->K, e, ws + p.o_part, colsum, d->N, p.dz_rows, db, s);

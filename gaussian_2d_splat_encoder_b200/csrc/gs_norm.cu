@@ -417,6 +417,7 @@ __device__ __forceinline__ void slice_stats(const NormArgs &a, const Slice &sl, 
 template <typename T, bool VEC, int PRE, int W>
 __global__ void __launch_bounds__(MAX_T, W == 1 ? 3 : 2) k_gn_stats(NormArgs a) {
     extern __shared__ __align__(16) uint8_t dsm[];
+    gs_let_follow();
     const Slice sl(a);
     float2 *out = reinterpret_cast<float2 *>(a.part) + ((long long)sl.b * a.G + sl.c0 / a.cpg) * a.splits + sl.s;
     slice_stats<T, VEC, PRE, W, false>(a, sl, dsm, reinterpret_cast<float *>(dsm + ring_bytes<T, 1, 2>()),
@@ -487,7 +488,8 @@ __global__ void __launch_bounds__(MAX_T, 3) k_gn_map(NormArgs a) {
     const long long last = sl.lo + sl.r + (long long)(n - 1) * a.rl;
     Feed<T, VEC, 1, B> feed(dsm, n, sl.valid);
     feed.tensor(0, reinterpret_cast<const T *>(a.x) + sl.b * a.x_img + sl.c + last * a.x_row, -a.rl * a.x_row);
-    feed.start();
+    feed.start();  // (x does not come from the first launch)
+    gs_wait_leader();
     join_stats(a, sl, reinterpret_cast<const float2 *>(a.part) + ((long long)sl.b * a.G + sl.c0 / a.cpg) * a.splits,
                a.splits, 1, mean, rstd);
     if (n == 0) return;
@@ -592,6 +594,7 @@ struct Grad {
 template <typename T, bool VEC, int PRE, int POST>
 __global__ void __launch_bounds__(MAX_T, 3) k_gn_grad_sums(NormArgs a) {
     extern __shared__ __align__(16) uint8_t dsm[];
+    gs_let_follow();
     const Slice sl(a);
     const int groups = sl.cc / a.cpg;
     // (the sums fold in the ring's place, drained by then)
@@ -654,6 +657,7 @@ __global__ void __launch_bounds__(MAX_T, 2) k_gn_grad_map(NormArgs a) {
     extern __shared__ __align__(16) uint8_t dsm[];
     float *sm = reinterpret_cast<float *>(dsm + ring_bytes<T, 2, 2>());
     if ((int)blockIdx.x >= a.nslice) {
+        gs_wait_leader();
         // 32 channels per block, the (image, split) sums dealt to the warps, joined in order
         float2 *red = reinterpret_cast<float2 *>(sm);
         const int lane = threadIdx.x & 31, nw = blockDim.x >> 5, c = ((int)blockIdx.x - a.nslice) * 32 + lane;
@@ -689,6 +693,7 @@ __global__ void __launch_bounds__(MAX_T, 2) k_gn_grad_map(NormArgs a) {
     feed.tensor(0, reinterpret_cast<const T *>(a.x) + sl.b * a.x_img + sl.c + last * a.x_row, -a.rl * a.x_row);
     feed.tensor(1, reinterpret_cast<const T *>(a.dy) + sl.b * a.dy_img + sl.c + last * a.dy_row, -a.rl * a.dy_row);
     feed.start();
+    gs_wait_leader();
     const float inv = 1.0f / ((float)a.rows * (float)a.cpg);
     for (int g = threadIdx.x >> 5; g < groups; g += blockDim.x >> 5) {
         const float2 *p = reinterpret_cast<const float2 *>(a.part) + ((long long)sl.b * a.G + sl.c0 / a.cpg + g) * a.splits;
@@ -825,9 +830,9 @@ int done(const char *where) {
 
 int threads(const NormArgs &a) { return (a.rl * a.cvec + 31) / 32 * 32; }
 template <typename K>
-int launch(K kern, unsigned grid, const NormArgs &a, size_t smem, cudaStream_t s, const char *where) {
+int launch(K kern, unsigned grid, const NormArgs &a, size_t smem, cudaStream_t s, bool follows, const char *where) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return done(where);
-    kern<<<grid, threads(a), smem, s>>>(a);
+    gs_launch(kern, dim3(grid), threads(a), smem, s, follows, 1, a);
     gs_count_launch(1);
     return done(where);
 }
@@ -838,21 +843,9 @@ template <typename T, int PRE, int POST>
 int forward_fused(const NormArgs &a, cudaStream_t s) {
     const int W = a.cpg % V == 0 ? 1 : V;
     auto kern = W == 1 ? k_gn_fused<T, PRE, POST, 1> : k_gn_fused<T, PRE, POST, V>;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = a.splits;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cudaLaunchConfig_t c;
-    memset(&c, 0, sizeof(c));
-    c.gridDim = dim3((unsigned)(a.B * a.splits * a.nchunk));
-    c.blockDim = dim3(threads(a));
-    c.dynamicSmemBytes = held_bytes(a.held) + ((size_t)2 * FUSED_T * W + (4 + 2 * (size_t)a.splits) * (a.chunk / a.cpg)) * sizeof(float);
-    c.stream = s;
-    c.attrs = at;
-    c.numAttrs = 1;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)c.dynamicSmemBytes) != cudaSuccess)
-        return done(FWD);
-    cudaLaunchKernelEx(&c, kern, a);
+    const size_t smem = held_bytes(a.held) + ((size_t)2 * FUSED_T * W + (4 + 2 * (size_t)a.splits) * (a.chunk / a.cpg)) * sizeof(float);
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return done(FWD);
+    gs_launch(kern, dim3((unsigned)(a.B * a.splits * a.nchunk)), threads(a), smem, s, false, a.splits, a);
     gs_count_launch(1);
     return done(FWD);
 }
@@ -863,18 +856,18 @@ int forward(const NormArgs &a, cudaStream_t s) {
     const size_t groups = 2 * (size_t)(a.chunk / a.cpg) * sizeof(float);
     const int W = a.cpg % V == 0 ? 1 : V;
     const int st = launch(W == 1 ? k_gn_stats<T, VEC, PRE, 1> : k_gn_stats<T, VEC, PRE, V>, grid, a,
-                          ring_bytes<T, 1, 2>() + 2 * MAX_T * W * sizeof(float) + groups, s, FWD);
-    return st != GS_OK ? st : launch(k_gn_map<T, VEC, PRE, POST>, grid, a, ring_bytes<T, 1, 2>() + groups, s, FWD);
+                          ring_bytes<T, 1, 2>() + 2 * MAX_T * W * sizeof(float) + groups, s, false, FWD);
+    return st != GS_OK ? st : launch(k_gn_map<T, VEC, PRE, POST>, grid, a, ring_bytes<T, 1, 2>() + groups, s, true, FWD);
 }
 template <typename T, bool VEC, int PRE, int POST>
 int backward(const NormArgs &a, cudaStream_t s) {
     const unsigned grid = (unsigned)(a.B * a.splits * a.nchunk), fold = a.dw || a.db ? (a.C + 31) / 32 : 0;
     const size_t groups = 2 * (size_t)(a.chunk / a.cpg) * sizeof(float), ring = ring_bytes<T, 2, 2>();
     if (a.nslice + fold == 0) return GS_OK;
-    const int st = launch(k_gn_grad_sums<T, VEC, PRE, POST>, grid, a, ring + groups, s, BWD_);
+    const int st = launch(k_gn_grad_sums<T, VEC, PRE, POST>, grid, a, ring + groups, s, false, BWD_);
     return st != GS_OK ? st
                        : launch(k_gn_grad_map<T, VEC, PRE, POST>, a.nslice + fold, a,
-                                ring + std::max(groups, MAX_T * sizeof(float2)), s, BWD_);
+                                ring + std::max(groups, MAX_T * sizeof(float2)), s, true, BWD_);
 }
 
 template <bool BWD, typename T, bool VEC>
