@@ -172,9 +172,26 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ri
         return false;
     };
     bool pending = res_tma && prefetch(item, 0, 0);  // a residual is on its way to the next unit's place
+    // bias of this warp's 64 columns of an item, two a lane, loaded an item ahead
+    float ahead[2] = {0.f, 0.f};
+    auto load_bias = [&](int it) {
+        if (!a.bias || it >= n_items) return;
+        const int c = Item(a, it).j * BN + part * 64 + lane;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int cc = c + 32 * k;
+            ahead[k] = cc >= a.J   ? 0.f
+                       : OUT32     ? reinterpret_cast<const float *>(a.bias)[cc]
+                       : a.out_f16 ? to_f32(reinterpret_cast<const __half *>(a.bias)[cc])
+                                   : to_f32(reinterpret_cast<const __nv_bfloat16 *>(a.bias)[cc]);
+        }
+    };
+    load_bias(item);
     bool dead = false;
     for (; item < n_items && !dead; item += step, tc += S::PAR) {
         const int buf = tc % S::NBUF;
+        const float bias[2] = {ahead[0], ahead[1]};
+        load_bias(item + step);
         const Item tile(a, item);
         const int sp = tile.s, base = tile.j * BN + part * 64;
         const long long row0 = (long long)tile.i * S::TILE_I + rank * BM + q * 32;
@@ -184,7 +201,6 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ri
             const bool live = col0 < a.J && row0 < a.I;
             const int sl = use & 1;
             uint8_t *const out = slots + sl * UNIT;
-            float bias = 0.f;
             if (live) {
                 // the slots this unit writes are no longer read by their stores
                 if (lane == 0) {
@@ -202,10 +218,6 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ri
                             }
                     __syncwarp();
                 }
-                if (const int c = col0 + lane; a.bias && lane < EC && c < a.J)
-                    bias = OUT32       ? reinterpret_cast<const float *>(a.bias)[c]
-                               : a.out_f16 ? to_f32(reinterpret_cast<const __half *>(a.bias)[c])
-                                           : to_f32(reinterpret_cast<const __nv_bfloat16 *>(a.bias)[c]);
             }
             if (u == 0) {
                 if (!mbar_wait_or_abort(&p.tfull[buf], (tc / S::NBUF) & 1, &p.abort_flag, &g_wait_error, 5)) dead = true;
@@ -227,7 +239,9 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ri
                     uint32_t r[16];
                     tmem_issue16(tbase + (uint32_t)(buf * BN + part * 64 + u * EC + 16 * h), r);
                     __syncwarp();
-                    if (lane >> 4 == h) p.bias[e][lane & 15] = bias;
+                    // columns 16 k.. of the 64: half of the lanes hold them
+                    const int k = u * (EC / 16) + h;
+                    if (lane >> 4 == (k & 1)) p.bias[e][lane & 15] = k < 2 ? bias[0] : bias[1];
                     __syncwarp();
                     tmem_wait16(r);
                     const float4 *b = reinterpret_cast<const float4 *>(p.bias[e]);
