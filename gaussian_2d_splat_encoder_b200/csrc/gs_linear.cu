@@ -86,8 +86,10 @@ enum { EPI_NONE = 0, EPI_GELU = 1, EPI_SILU = 2, EPI_GELU_SLOPE = 3, EPI_SILU_SL
 //            64-byte swizzle (a thread writes its row without bank conflicts) and moved by TMA; the residual
 //            comes by TMA into the same place, a unit ahead, and is added in registers before the only rounding.
 // PAIR: two CTAs share a 256 x 256 tile (cta_group::2): each loads its 128 rows of A and half of B's rows, so an
-// output costs two thirds of the L2 reads of a 128 x 256 tile; that traffic, not the tensor cores, bounds large
-// products (a 128 x 256 tile read 13 TB/s from L2 at 1130 TFLOP/s).  The leader issues all MMAs.
+// output costs half of the L2 reads and half of the issued MMAs of a 128 x 128 tile (16384x4096->4096 with a
+// residual: 387 us, 1420 TFLOP/s, against 569).  The leader issues all MMAs.
+// Bound by: long sums, the tensor cores and their loads' latency; short ones, the epilogue's instructions (GELU is
+// 11 of some 20 an output; 36864x128->512 takes 23.3 us where its bytes take 7.3).
 // Every wait is bounded; one that gives up records a code in g_wait_error and raises the CTA's abort flag.
 template <int BN, bool PAIR, bool OUT32, int EPI>
 struct Shape {
