@@ -12,8 +12,8 @@
 // The forward keeps, for the backward, the activation's slope instead of z: the epilogue has its parts at
 // hand, the backward needs no activation, and in 16-bit types it is a 16-bit fixed-point number in
 // [-1/6, 7/6] (GELU's and SiLU's slopes lie in [-0.13, 1.13]) with steps of 1/49152: an error of 1e-5 where a
-// bf16 z would cost 4e-3 |z|.  dz is rounded to the operand type once, as the products need it; db sums the
-// unrounded values.
+// bf16 z would cost 4e-3 |z|.  dz is rounded to the operand type once, as the products need it (a small one
+// keeps a second term); db sums the unrounded values.
 //
 // Sums over a long k with few output tiles are split along k over the SMs; the parts go to the workspace
 // in fp32 and a second kernel adds them in order (the same bits every time) and applies the epilogue.
@@ -56,7 +56,7 @@ __device__ __forceinline__ float slope_of(uint32_t c) {
 struct GemmArgs {
     long long I;          // rows of D
     int J;                // columns of D
-    int kb, npair;        // k-blocks of 64 per term product, term products (1, or 6 for fp32)
+    int kb, npair;        // k-blocks of 64 per term product, term products: 1, 2 (A in two terms), 6 (fp32)
     int a_mn, b_mn;       // operand has i / j adjacent instead of k
     int f16;              // operands fp16 (else bf16)
     int splits;           // > 1: parts of the k sum, raw fp32 to part
@@ -69,8 +69,8 @@ struct GemmArgs {
     long long ldr;
 };
 
-// term products of fp32 operands, small ones first: (a term, b term), 0 = high
-__constant__ const unsigned char PAIR_A[6] = {2, 0, 1, 1, 0, 0}, PAIR_B[6] = {0, 2, 1, 0, 1, 0};
+// term products, small ones first: (a term, b term), 0 = high; the six of fp32, then the two of A in two terms
+__constant__ const unsigned char PAIR_A[8] = {2, 0, 1, 1, 0, 0, 1, 0}, PAIR_B[8] = {0, 2, 1, 0, 1, 0, 0, 0};
 
 // What an epilogue does with z = acc + bias: nothing, an activation, or an activation and its slope.
 constexpr int EPI_WARPS = 16, UNIT = 2048, GEMM_THREADS = 64 + 32 * EPI_WARPS;
@@ -409,8 +409,8 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
                 const Item t(a, item);
                 const int j0 = t.j * BN + (PAIR ? rank * S::BROWS : 0), i0 = t.i * S::TILE_I + rank * BM;
                 const int k0 = t.from(a) * BK, k1 = t.to(a) * BK;
-                int kk = k0, pr = 0, left = t.blocks(a);
-                int ta = a.npair > 1 ? PAIR_A[0] : 0, tb = a.npair > 1 ? PAIR_B[0] : 0;
+                int kk = k0, pr = a.npair == 2 ? 6 : 0, left = t.blocks(a);
+                int ta = a.npair > 1 ? PAIR_A[pr] : 0, tb = a.npair > 1 ? PAIR_B[pr] : 0;
                 for (; left > 0; left--, it++) {
                     if (!mbar_wait_or_abort(&p.empty[st], parity, &p.abort_flag, &g_wait_error, 1)) break;
                     uint8_t *sa = smem + st * S::STAGE, *sb = sa + S::A_BYTES;
@@ -587,6 +587,7 @@ struct DzArgs {
     long long M, ldy;
     int N, ldp, cvec, rl;  // vectors of eight columns per block, row lanes
     int rows;              // blocks over the rows
+    int terms;             // of dz in 16-bit types
     PrepJobs prep;
 };
 template <typename T, bool VEC>
@@ -624,8 +625,18 @@ __global__ void __launch_bounds__(256) k_dz(const __grid_constant__ DzArgs a) {
         if (a.dz) {
             if (sizeof(T) == 4)
                 store_terms(v, reinterpret_cast<__nv_bfloat16 *>(a.dz) + m * a.ldp + c, a.M * a.ldp);
-            else
-                *reinterpret_cast<Raw8<T> *>(reinterpret_cast<T *>(a.dz) + m * a.ldp + c) = pack8<T>(v);
+            else {
+                Raw8<T> *to = reinterpret_cast<Raw8<T> *>(reinterpret_cast<T *>(a.dz) + m * a.ldp + c);
+                const Raw8<T> high = pack8<T>(v);
+                *to = high;
+                if (a.terms == 2) {  // what the first term leaves; nothing of an infinity or NaN
+                    f2 h[4];
+                    unpack8<T>(high, h);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) at(v, i) = fabsf(at(h, i)) <= 3.4028234e38f ? at(v, i) - at(h, i) : 0.f;
+                    *reinterpret_cast<Raw8<T> *>(reinterpret_cast<T *>(to) + a.M * a.ldp) = pack8<T>(v);
+                }
+            }
         }
     };
     auto fetch = [&](const T *p, Raw8<T> &o) {
@@ -794,7 +805,7 @@ Tiling tiling(long long I, int J, long long kb, int npair) {
         if (bn > 64 && J <= bn / 2) continue;
         const long long tiles = cdiv(I, ti) * cdiv(J, bn);
         // unsplit (in fp32 as few parts as the chain allows), or one part for every idle SM
-        const long long few = npair > 1 ? cdiv(kb, FP32_CHAIN) : 1;
+        const long long few = npair == 6 ? cdiv(kb, FP32_CHAIN) : 1;
         const long long many = tiles < units ? std::min({units / tiles, kb * npair / 4, kb}) : 1;
         for (long long s : {few, std::max(few, many)}) {
             const double waves = (double)cdiv(tiles * s, units), k = (double)cdiv(kb, s) * npair * block[w];
@@ -811,7 +822,7 @@ Tiling tiling(long long I, int J, long long kb, int npair) {
 
 // Workspace of a call: padded or split operands, the parts of split sums, column sums.
 struct Plan {
-    int es, terms, npair;  // element size of the operands' source, bf16 terms, term products
+    int es, terms, dz_terms;  // element size of the operands' source; terms of x and W, of dz
     int ldx, ldw, ldn;     // row strides of the padded x, W and dz
     bool prep_x, prep_w, need_dz;
     Tiling fwd, gx, gw;
@@ -829,7 +840,6 @@ Plan plan(const gs_linear_desc *d, bool bwd) {
     const bool f32 = d->dtype == GS_F32;
     p.es = f32 ? 4 : 2;
     p.terms = f32 ? 3 : 1;
-    p.npair = f32 ? 6 : 1;
     p.ldx = p.ldw = up8(d->K);
     p.ldn = up8(d->N);
     p.prep_x = f32 || ragged(d->ldx, d->unaligned & 1);
@@ -845,13 +855,16 @@ Plan plan(const gs_linear_desc *d, bool bwd) {
     p.o_x = take(p.prep_x ? (size_t)d->M * p.ldx * 2 * p.terms : 0);
     p.o_w = take(p.prep_w ? (size_t)d->N * p.ldw * 2 * p.terms : 0);
     if (!bwd) {
-        p.fwd = tiling(d->M, d->N, cdiv(d->K, BK), p.npair);
+        p.fwd = tiling(d->M, d->N, cdiv(d->K, BK), f32 ? 6 : 1);
         p.o_part = take(parts(p.fwd, d->M, d->N));
     } else {
         p.need_dz = f32 || d->act != GS_ACT_NONE || ragged(d->ldy, d->unaligned & 4);
-        p.o_dz = take(p.need_dz ? (size_t)d->M * p.ldn * 2 * p.terms : 0);
-        p.gx = tiling(d->M, d->K, cdiv(d->N, BK), p.npair);
-        p.gw = tiling(d->N, d->K, cdiv(d->M, BK), p.npair);
+        // rounding dz to 16 bits adds as much as rounding the result does.  Where dz is small (up to 2^16
+        // elements, whose products are bound by their launches) it keeps a second term instead.
+        p.dz_terms = f32 ? 3 : d->act != GS_ACT_NONE && d->M * d->N <= 1 << 16 ? 2 : 1;
+        p.o_dz = take(p.need_dz ? (size_t)d->M * p.ldn * 2 * p.dz_terms : 0);
+        p.gx = tiling(d->M, d->K, cdiv(d->N, BK), f32 ? 6 : p.dz_terms);
+        p.gw = tiling(d->N, d->K, cdiv(d->M, BK), f32 ? 6 : p.dz_terms);
         p.o_part = take(std::max(parts(p.gx, d->M, d->K), parts(p.gw, d->N, d->K)));
         // dz: blocks of 256 threads, up to 256 column vectors each, about four blocks per SM
         const int nv = p.ldn / 8;
@@ -935,6 +948,7 @@ struct Operand {
     const void *p;
     long long rows, cols, ld;
     int mn;  // the product's own axis is adjacent (else k is)
+    int terms;
 };
 struct Epilogue {
     const void *bias, *residual;
@@ -951,15 +965,15 @@ int product(const gs_linear_desc *d, const Plan &p, const Tiling &t, long long I
     const bool f32 = d->dtype == GS_F32, raw = t.splits > 1, out32 = f32 || raw;
     a.I = I; a.J = J;
     a.kb = (int)cdiv(K, BK);
-    a.npair = p.npair;
+    a.npair = f32 ? 6 : A.terms;
     a.a_mn = A.mn; a.b_mn = B.mn;
     a.f16 = d->dtype == GS_F16;
     a.out_f16 = a.f16;
     a.splits = t.splits; a.tiles_i = t.tiles_i; a.tiles_j = t.tiles_j;
     CUtensorMap m[5];
     const CUtensorMapDataType in = a.f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    bool ok = make_map(&m[0], in, 2, A.p, A.cols, A.rows, A.ld, p.terms, 64, A.mn ? BK : BM) &&
-              make_map(&m[1], in, 2, B.p, B.cols, B.rows, B.ld, p.terms, 64, B.mn ? BK : t.pair ? t.bn / 2 : t.bn);
+    bool ok = make_map(&m[0], in, 2, A.p, A.cols, A.rows, A.ld, A.terms, 64, A.mn ? BK : BM) &&
+              make_map(&m[1], in, 2, B.p, B.cols, B.rows, B.ld, B.terms, 64, B.mn ? BK : t.pair ? t.bn / 2 : t.bn);
     m[2] = m[3] = m[4] = m[0];
     if (raw) {
         a.out_tma = 1;
@@ -1006,8 +1020,8 @@ PrepJobs operands(const gs_linear_desc *d, const Plan &p, const void *x, const v
                   Operand &X, Operand &W) {
     PrepJobs jobs;
     memset(&jobs, 0, sizeof(jobs));
-    X = Operand{x, d->M, d->K, d->ldx, 0};
-    W = Operand{w, d->N, d->K, d->ldw, 0};
+    X = Operand{x, d->M, d->K, d->ldx, 0, p.terms};
+    W = Operand{w, d->N, d->K, d->ldw, 0, p.terms};
     if (want_x && p.prep_x) {
         jobs.job[jobs.n++] = PrepJob{x, ws + p.o_x, d->M, d->ldx, d->K, p.ldx};
         X.p = ws + p.o_x;
@@ -1046,7 +1060,7 @@ int backward(const gs_linear_desc *d, const Plan &p, const void *x, const void *
     char *ws = base_of(workspace);
     Operand X, W;
     const PrepJobs jobs = operands(d, p, x, w, ws, dw != nullptr, dx != nullptr, X, W);
-    Operand Z{dy, d->M, d->N, d->ldy, 0};
+    Operand Z{dy, d->M, d->N, d->ldy, 0, p.dz_terms};
     const bool make_dz = p.need_dz && (dx || dw);
     float *colsum = db ? reinterpret_cast<float *>(ws + p.o_col) : nullptr;
     if (make_dz) {
@@ -1056,7 +1070,7 @@ int backward(const gs_linear_desc *d, const Plan &p, const void *x, const void *
     const bool rows = make_dz || db;
     if (rows || jobs.n) {
         const DzArgs a{dy, slope, make_dz ? ws + p.o_dz : nullptr, colsum, d->M, d->ldy, d->N, p.ldn, p.dz_cvec, p.dz_rl,
-                       rows ? p.dz_rows : 0, jobs};
+                       rows ? p.dz_rows : 0, p.dz_terms, jobs};
         // whole 16-byte vectors of dy and of the kept slope
         const bool vec = !ragged(d->ldy, d->unaligned & 4) && d->N % 8 == 0 && ((uintptr_t)slope & 15) == 0;
         const dim3 grid((unsigned)(a.rows + jobs.blocks), (unsigned)(rows ? p.dz_cols : 1));
