@@ -21,7 +21,7 @@
 //
 // With an activation the FMA and MUFU pipes bind as much as memory does (GELU: 0.125 cycles of an SM per
 // element and evaluation), so each launch evaluates it once per element.  Measured: 4x384x384x64 bf16 with SiLU
-// 45 us (statistics 20, map 26; its bytes take 23), a training step of 4x192x192x128 with GELU first 79 us (19, 18,
+// 44 us (statistics 20, map 26; its bytes take 23), a training step of 4x192x192x128 with GELU first 79 us (19, 18,
 // 21, 26; bytes 23), 96x96x256 in one launch 13.4 us against 27 in two.
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -481,7 +481,7 @@ struct Map {
 // ---- forward, second launch: the map
 template <typename T, bool VEC, int PRE, int POST>
 __global__ void __launch_bounds__(MAX_T, 3) k_gn_map(NormArgs a) {
-    constexpr int B = 2;
+    constexpr int B = 4;
     extern __shared__ __align__(16) uint8_t dsm[];
     const Slice sl(a);
     float *mean = reinterpret_cast<float *>(dsm + ring_bytes<T, 1, B>()), *rstd = mean + a.chunk / a.cpg;
@@ -859,7 +859,7 @@ int forward(const NormArgs &a, cudaStream_t s) {
     const int W = a.cpg % V == 0 ? 1 : V;
     const int st = launch(W == 1 ? k_gn_stats<T, VEC, PRE, 1> : k_gn_stats<T, VEC, PRE, V>, grid, a,
                           ring_bytes<T, 1, 2>() + 2 * MAX_T * W * sizeof(float) + groups, s, false, FWD);
-    return st != GS_OK ? st : launch(k_gn_map<T, VEC, PRE, POST>, grid, a, ring_bytes<T, 1, 2>() + groups, s, true, FWD);
+    return st != GS_OK ? st : launch(k_gn_map<T, VEC, PRE, POST>, grid, a, ring_bytes<T, 1, 4>() + groups, s, true, FWD);
 }
 template <typename T, bool VEC, int PRE, int POST>
 int backward(const NormArgs &a, cudaStream_t s) {
