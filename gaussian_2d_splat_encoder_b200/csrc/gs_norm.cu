@@ -21,7 +21,7 @@
 //
 // With an activation the FMA and MUFU pipes bind as much as memory does (GELU: 0.125 cycles of an SM per
 // element and evaluation), so each launch evaluates it once per element.  Measured: 4x384x384x64 bf16 with SiLU
-// 44 us (statistics 20, map 26; its bytes take 23), a training step of 4x192x192x128 with GELU first 79 us (19, 18,
+// 44 us (statistics 20, map 24; its bytes take 23), a training step of 4x192x192x128 with GELU first 79 us (19, 18,
 // 21, 26; bytes 23), 96x96x256 in one launch 13.4 us against 27 in two.
 #include <cuda_runtime.h>
 #include <stdint.h>
