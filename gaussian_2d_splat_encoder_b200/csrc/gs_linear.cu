@@ -10,9 +10,8 @@
 // the nine term products that reach 2^-24: the same kernel runs over six times the k-blocks.
 //
 // The forward keeps, for the backward, the activation's slope instead of z: the epilogue has its parts at
-// hand, the backward needs no activation, and in 16-bit types it is a 16-bit fixed-point number in
-// [-1/6, 7/6] (GELU's and SiLU's slopes lie in [-0.13, 1.13]) with steps of 1/49152: an error of 1e-5 where a
-// bf16 z would cost 4e-3 |z|.  dz is rounded to the operand type once, as the products need it (a small one
+// hand and the backward needs no activation.  It is kept in fp32: in 16 bits either the small slopes of units
+// far below zero or those near one lose bits.  dz is rounded to the operand type once, as the products need it (a small one
 // keeps a second term); db sums the unrounded values.
 //
 // Sums over a long k with few output tiles are split along k over the SMs; the parts go to the workspace
@@ -25,6 +24,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/gsplat_b200.h"
 #include "gs_act.cuh"
@@ -42,17 +42,6 @@ constexpr int BM = 128, BK = 64;
 
 __device__ int g_wait_error;  // code of a bounded wait that gave up (gs_linear_error_flag), 0 if none did
 
-// ---- the kept slope: fp32, or 16-bit fixed point (0 and 1 exact, 65535 is NaN).  s 49152 + 8192 + 2^23 rounds
-// to the code in the low mantissa bits; the canonical NaN's low bits are 65535.
-__device__ __forceinline__ uint32_t slope_codes(f2 s) {  // two codes, the first in the low half
-    const f2 c = fma2(s, both(49152.f), both(8192.f + 8388608.f));
-    return __byte_perm(__float_as_uint(c.x), __float_as_uint(c.y), 0x5410);
-}
-__device__ __forceinline__ float slope_of(uint32_t c) {
-    const float s = (__uint_as_float(0x4B000000u | c) - (8192.f + 8388608.f)) * (1.f / 49152.f);
-    return c == 65535u ? __int_as_float(0x7fffffff) : s;
-}
-
 struct GemmArgs {
     long long I;          // rows of D
     int J;                // columns of D
@@ -65,7 +54,8 @@ struct GemmArgs {
     int out_f16;          // 16-bit output type
     int out_tma, res_tma; // whole 16-byte rows: TMA boxes, else element by element
     const void *bias, *residual;
-    void *out, *slope;
+    void *out;
+    float *slope;
     long long ldr;
 };
 
@@ -101,8 +91,9 @@ struct Shape {
     static constexpr int EC = OUT32 ? 16 : 32;        // columns of a unit
     static constexpr int UNITS = 64 / EC;
     static constexpr bool SLOPE = EPI >= EPI_GELU_SLOPE;
-    static constexpr uint32_t SLOTS = (2 + SLOPE) * UNIT;  // per epilogue warp: two for outputs and residuals
-    static constexpr int STAGES = (229376 - EPI_WARPS * SLOTS) / STAGE;  // 4 to 6
+    static constexpr int SLOPES = SLOPE ? EC / 16 : 0;       // 64-byte rows of fp32 hold 16 slopes
+    static constexpr uint32_t SLOTS = (2 + SLOPES) * UNIT;   // per epilogue warp: two for outputs and residuals
+    static constexpr int STAGES = (229376 - EPI_WARPS * SLOTS) / STAGE;  // 3 to 6
     static constexpr size_t SMEM = 1024 + STAGES * STAGE + EPI_WARPS * SLOTS;
     static constexpr int TILE_I = PAIR ? 2 * BM : BM;
 };
@@ -147,11 +138,9 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ri
     const int step = S::PAR * stride;
     int item = first + turn * stride, tc = turn, use = 0;
 
-    // byte of row r, column c in a unit: rows of 64 bytes, 16-byte chunks exchanged by the 64-byte swizzle
-    auto place_of = [](int r, int c) {
-        const int b = c * (OUT32 ? 4 : 2);
-        return r * 64 + (((b >> 4) ^ ((r >> 1) & 3)) << 4) + (b & 15);
-    };
+    // byte b of row r in a unit: rows of 64 bytes, 16-byte chunks exchanged by the 64-byte swizzle
+    auto swizzled = [](int r, int b) { return r * 64 + (((b >> 4) ^ ((r >> 1) & 3)) << 4) + (b & 15); };
+    auto place_of = [&](int r, int c) { return swizzled(r, c * (OUT32 ? 4 : 2)); };
     auto place = [&](int it, int u, int &col0, long long &row0) {
         const Item t(a, it);
         col0 = t.j * BN + part * 64 + u * EC;
@@ -271,15 +260,8 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ri
                     f2 s[8];
 #pragma unroll
                     for (int i = 0; i < 8; i++) v[i] = act(v[i], s[i]);
-                    if (OUT32) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) *chunk(slo, i) = pack16<float>(s + 2 * i);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 2; i++)
-                            *chunk(slo, 2 * h + i) = make_uint4(slope_codes(s[4 * i]), slope_codes(s[4 * i + 1]),
-                                                                slope_codes(s[4 * i + 2]), slope_codes(s[4 * i + 3]));
-                    }
+                    for (int i = 0; i < 4; i++) *chunk(slo + h * UNIT, i) = pack16<float>(s + 2 * i);
                 } else if (ACT != ACT_NONE) {
 #pragma unroll
                     for (int i = 0; i < 8; i++) v[i] = act(v[i]);
@@ -321,7 +303,9 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ri
             if (a.out_tma) {
                 if (lane == 0) {
                     tma_store_3d(tmO, out, col0, (int)row0, sp);
-                    if (SLOPE) tma_store_3d(tmS, slo, col0, (int)row0, 0);
+#pragma unroll
+                    for (int h = 0; h < S::SLOPES; h++)
+                        if (col0 + 16 * h < a.J) tma_store_3d(tmS, slo + h * UNIT, col0 + 16 * h, (int)row0, 0);
                     bulk_commit();
                 }
             } else {
@@ -329,14 +313,10 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ri
                     if (const int c = lane % EC; col0 + c < a.J) {
                         const long long at = (row0 + r) * a.J + col0 + c;
                         const int off = place_of(r, c);
-                        if (OUT32) {
-                            reinterpret_cast<float *>(a.out)[at] = *reinterpret_cast<const float *>(out + off);
-                            if (SLOPE) reinterpret_cast<float *>(a.slope)[at] = *reinterpret_cast<const float *>(slo + off);
-                        } else {
-                            reinterpret_cast<uint16_t *>(a.out)[at] = *reinterpret_cast<const uint16_t *>(out + off);
-                            if (SLOPE)
-                                reinterpret_cast<uint16_t *>(a.slope)[at] = *reinterpret_cast<const uint16_t *>(slo + off);
-                        }
+                        if (OUT32) reinterpret_cast<float *>(a.out)[at] = *reinterpret_cast<const float *>(out + off);
+                        else reinterpret_cast<uint16_t *>(a.out)[at] = *reinterpret_cast<const uint16_t *>(out + off);
+                        if (SLOPE)
+                            a.slope[at] = *reinterpret_cast<const float *>(slo + (c >> 4) * UNIT + swizzled(r, (c & 15) * 4));
                     }
                 fence_proxy_async();  // the next residual's copy overwrites what was just read
                 __syncwarp();
@@ -581,7 +561,8 @@ __global__ void __launch_bounds__(256) k_prep_operands(const __grid_constant__ P
 // ---- dz = dy slope as an operand (dz NULL: not written, dy serves), and its column sums per block of rows.
 // Blocks from `rows` on prepare x and W for the backward's products: a launch less.
 struct DzArgs {
-    const void *dy, *slope;
+    const void *dy;
+    const float *slope;
     void *dz;
     float *colsum;  // [blocks][N], or NULL
     long long M, ldy;
@@ -602,21 +583,16 @@ __global__ void __launch_bounds__(256) k_dz(const __grid_constant__ DzArgs a) {
     const int c = (blockIdx.y * a.cvec + cv) * 8;
     const bool live = r < a.rl && c < a.ldp;
     const long long lo = a.M * blockIdx.x / a.rows, hi = a.M * (blockIdx.x + 1LL) / a.rows;
-    const T *dy = reinterpret_cast<const T *>(a.dy) + c, *slope = reinterpret_cast<const T *>(a.slope) + c;
+    const T *dy = reinterpret_cast<const T *>(a.dy) + c;
+    const float *slope = a.slope + c;
     f2 s[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
-    // dy and its slope g (as the forward packed it), in row m
-    auto one = [&](long long m, const Raw8<T> &d, const Raw8<T> &g) {
+    // dy and its slope g, in row m
+    auto one = [&](long long m, const Raw8<T> &d, const Raw8<float> &g) {
         f2 v[4];
         unpack8<T>(d, v);
         if (a.slope) {
             f2 f[4];
-            if (sizeof(T) == 4) {
-                unpack8<T>(g, f);
-            } else {
-                const uint32_t x[4] = {g.q[0].x, g.q[0].y, g.q[0].z, g.q[0].w};
-#pragma unroll
-                for (int i = 0; i < 4; i++) f[i] = {slope_of(x[i] & 0xffffu), slope_of(x[i] >> 16)};
-            }
+            unpack8<float>(g, f);
 #pragma unroll
             for (int i = 0; i < 4; i++) v[i] = mul2(v[i], f[i]);  // (rounded: db's bits do not depend on dz being written)
         }
@@ -639,19 +615,20 @@ __global__ void __launch_bounds__(256) k_dz(const __grid_constant__ DzArgs a) {
             }
         }
     };
-    auto fetch = [&](const T *p, Raw8<T> &o) {
+    auto fetch = [&](const auto *p, auto &o) {
+        using E = std::decay_t<decltype(*p)>;
         if constexpr (VEC) {
 #pragma unroll
-            for (int k = 0; k < (int)sizeof(T) / 2; k++) o.q[k] = __ldcs(reinterpret_cast<const uint4 *>(p) + k);  // read once
+            for (int k = 0; k < (int)sizeof(E) / 2; k++) o.q[k] = __ldcs(reinterpret_cast<const uint4 *>(p) + k);  // read once
         } else {
             union {
-                Raw8<T> q;
-                T e[8];
+                Raw8<E> q;
+                E e[8];
             } u;
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 if (c + i < a.N) u.e[i] = p[i];
-                else from_f32(0.f, u.e[i]);  // (and 0 codes a finite slope)
+                else from_f32(0.f, u.e[i]);
             o = u.q;
         }
     };
@@ -659,7 +636,8 @@ __global__ void __launch_bounds__(256) k_dz(const __grid_constant__ DzArgs a) {
         long long m = lo + r;
         constexpr int R = 4;  // rows in flight
         for (; m + (R - 1) * a.rl < hi; m += R * a.rl) {
-            Raw8<T> d[R], g[R];
+            Raw8<T> d[R];
+            Raw8<float> g[R];
 #pragma unroll
             for (int k = 0; k < R; k++) {
                 fetch(dy + (m + k * a.rl) * a.ldy, d[k]);
@@ -669,7 +647,8 @@ __global__ void __launch_bounds__(256) k_dz(const __grid_constant__ DzArgs a) {
             for (int k = 0; k < R; k++) one(m + k * a.rl, d[k], g[k]);
         }
         for (; m < hi; m += a.rl) {
-            Raw8<T> d, g;
+            Raw8<T> d;
+            Raw8<float> g;
             fetch(dy + m * a.ldy, d);
             if (a.slope) fetch(slope + m * a.N, g);
             one(m, d, g);
@@ -702,7 +681,8 @@ struct JoinArgs {
     long long I, ldr, part_stride;
     int J, ldp, splits, sum_blocks, act;
     const void *bias, *residual;
-    void *out, *slope;
+    void *out;
+    float *slope;
     const float *colsum;
     int ncol, nsum;  // columns, and blocks that were summed
     void *db;
@@ -762,10 +742,7 @@ __global__ void __launch_bounds__(256) k_join(JoinArgs a) {
             if (k >= n) break;
             const long long at = i * a.J + c + k;
             float z = k & 1 ? v[k >> 1].y : v[k >> 1].x;
-            if (a.slope) {
-                if (sizeof(T) == 4) reinterpret_cast<float *>(a.slope)[at] = k & 1 ? sl[k >> 1].y : sl[k >> 1].x;
-                else reinterpret_cast<uint16_t *>(a.slope)[at] = (uint16_t)(slope_codes(sl[k >> 1]) >> (16 * (k & 1)));
-            }
+            if (a.slope) a.slope[at] = k & 1 ? sl[k >> 1].y : sl[k >> 1].x;
             if (a.residual) z = __fadd_rn(z, to_f32(reinterpret_cast<const T *>(a.residual)[i * a.ldr + c + k]));
             from_f32(z, reinterpret_cast<T *>(a.out)[at]);
         }
@@ -954,7 +931,8 @@ struct Epilogue {
     const void *bias, *residual;
     long long ldr;
     int act;
-    void *out, *slope;
+    void *out;
+    float *slope;
 };
 
 // D [I][J] over k = K; with splits the parts go to `part` and the caller joins them
@@ -983,10 +961,10 @@ int product(const gs_linear_desc *d, const Plan &p, const Tiling &t, long long I
         const CUtensorMapDataType ty = f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
         a.bias = e.bias; a.residual = e.residual; a.ldr = e.ldr; a.out = e.out; a.slope = e.slope;
         const auto whole = [&](const void *q, long long ld) { return ((uintptr_t)q & 15) == 0 && ld * es % 16 == 0; };
-        a.out_tma = whole(e.out, J) && (!e.slope || whole(e.slope, J));
+        a.out_tma = whole(e.out, J) && ((uintptr_t)e.slope & 15) == 0;  // (rows of slopes are as long or longer)
         a.res_tma = e.residual && whole(e.residual, e.ldr);
         if (a.out_tma) ok = ok && make_map(&m[2], ty, es, e.out, J, I, J, 1, ec, 32);
-        if (a.out_tma && e.slope) ok = ok && make_map(&m[3], ty, es, e.slope, J, I, J, 1, ec, 32);
+        if (a.out_tma && e.slope) ok = ok && make_map(&m[3], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, e.slope, J, I, J, 1, 16, 32);
         if (a.res_tma) ok = ok && make_map(&m[4], ty, es, e.residual, J, I, e.ldr, 1, ec, 32);
     }
     if (!ok) return cuda_error("gs_linear_act", "cuTensorMapEncodeTiled refused a tensor");
@@ -1055,7 +1033,7 @@ int forward(const gs_linear_desc *d, const Plan &p, const void *x, const void *w
 }
 
 template <typename T>
-int backward(const gs_linear_desc *d, const Plan &p, const void *x, const void *w, const void *slope, const void *dy,
+int backward(const gs_linear_desc *d, const Plan &p, const void *x, const void *w, const float *slope, const void *dy,
              void *dx, void *dw, void *db, void *workspace, cudaStream_t s) {
     char *ws = base_of(workspace);
     Operand X, W;
@@ -1106,7 +1084,7 @@ extern "C" size_t gs_linear_act_workspace_size(const gs_linear_desc *d, int back
 }
 
 extern "C" int gs_linear_act_fwd(const gs_linear_desc *d, const void *x, const void *w, const void *bias,
-                                 const void *residual, void *y, void *slope, void *workspace, size_t workspace_bytes,
+                                 const void *residual, void *y, float *slope, void *workspace, size_t workspace_bytes,
                                  void *stream) {
     if (!valid(d) || (residual && d->ldr < d->N)) return GS_ERR_BAD_ARGUMENT;
     if (d->M == 0) return GS_OK;
@@ -1122,7 +1100,7 @@ extern "C" int gs_linear_act_fwd(const gs_linear_desc *d, const void *x, const v
     return forward<__half>(d, p, x, w, e, workspace, s);
 }
 
-extern "C" int gs_linear_act_bwd(const gs_linear_desc *d, const void *x, const void *w, const void *slope,
+extern "C" int gs_linear_act_bwd(const gs_linear_desc *d, const void *x, const void *w, const float *slope,
                                  const void *dy, void *dx, void *dw, void *dbias, void *workspace,
                                  size_t workspace_bytes, void *stream) {
     if (!valid(d) || d->ldy < d->N) return GS_ERR_BAD_ARGUMENT;

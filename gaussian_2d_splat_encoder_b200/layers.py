@@ -252,8 +252,7 @@ def _linear_forward(x, weight, bias, residual, act, train):
     y = x.new_empty(shape)
     slope = None
     if train and act:
-        # the activation's slope, as the backward takes it: fp32, or 16-bit fixed point
-        slope = x.new_empty(shape, dtype=torch.float32 if x.dtype == torch.float32 else torch.int16)
+        slope = x.new_empty(shape, dtype=torch.float32)  # the activation's, for the backward
     ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes > _NO_WORKSPACE else None
     _lib.check(_lib.load().gs_linear_act_fwd(desc, px, pw, None if bias is None else bias.data_ptr(),
                                              None if residual is None else residual.data_ptr(), y.data_ptr(),

@@ -299,13 +299,13 @@ typedef struct {
 /* Workspace bytes of a forward (backward = 0) or a backward (1) call; 0 for an invalid descriptor, 256 where the
  * call needs none (workspace may then be NULL). */
 size_t gs_linear_act_workspace_size(const gs_linear_desc *d, int backward);
-/* bias, residual and slope may be NULL; slope [M][N] (2 bytes an element for 16-bit types, else 4) receives
- * the activation's slope for the backward, in the library's own encoding; not written without an activation. */
+/* bias, residual and slope may be NULL; slope [M][N] receives the activation's slope for the backward; not
+ * written without an activation. */
 int gs_linear_act_fwd(const gs_linear_desc *d, const void *x, const void *w, const void *bias, const void *residual,
-                      void *y, void *slope, void *workspace, size_t workspace_bytes, void *stream);
+                      void *y, float *slope, void *workspace, size_t workspace_bytes, void *stream);
 /* Gradients for upstream dy: dx [M][K], dw [N][K], dbias [N]; each may be NULL (not computed).
  * slope is the forward's, not read without an activation.  The residual's gradient is dy itself. */
-int gs_linear_act_bwd(const gs_linear_desc *d, const void *x, const void *w, const void *slope, const void *dy, void *dx,
+int gs_linear_act_bwd(const gs_linear_desc *d, const void *x, const void *w, const float *slope, const void *dy, void *dx,
                       void *dw, void *dbias, void *workspace, size_t workspace_bytes, void *stream);
 /* Reads (synchronously) the code of a bounded device wait of the linear kernels that gave up on the current
  * device since the library was loaded; 0 if none did.  Outputs of such a call are not valid. */
