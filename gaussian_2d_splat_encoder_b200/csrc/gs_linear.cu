@@ -11,8 +11,9 @@
 //
 // The forward keeps, for the backward, the activation's slope instead of z: the epilogue has its parts at
 // hand and the backward needs no activation.  It is kept in fp32: in 16 bits either the small slopes of units
-// far below zero or those near one lose bits.  dz is rounded to the operand type once, as the products need it (a small one
-// keeps a second term); db sums the unrounded values.
+// far below zero or those near one lose bits.  dz enters its
+// products in two terms of the operand type, dz = hi + lo (rounding it once would add as much error as rounding the
+// result does); db sums the unrounded values.
 //
 // Sums over a long k with few output tiles are split along k over the SMs; the parts go to the workspace
 // in fp32 and a second kernel adds them in order (the same bits every time) and applies the epilogue.
@@ -60,6 +61,9 @@ struct GemmArgs {
 };
 
 // term products, small ones first: (a term, b term), 0 = high; the six of fp32, then the two of A in two terms
+// fp16 has no exponents below its subnormals: lo is kept times 2^LO_BITS (at most 2^4 2^11 for the largest dz) and
+// its sum scaled back when the products with hi begin.
+constexpr int LO_BITS = 11;
 __constant__ const unsigned char PAIR_A[8] = {2, 0, 1, 1, 0, 0, 1, 0}, PAIR_B[8] = {0, 2, 1, 0, 1, 0, 0, 0};
 
 // What an epilogue does with z = acc + bias: nothing, an activation, or an activation and its slope.
@@ -442,6 +446,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
             int it = 0, tc = 0, st = 0, parity = 0;
             for (int item = first; item < n_items && !p.abort_flag; item += stride, tc++) {
                 int left = Item(a, item).blocks(a);
+                const int hi = a.npair == 2 && a.f16 ? left / 2 : -1;  // k-blocks left when hi follows lo
                 const int buf = tc % S::NBUF;
                 if (tc >= S::NBUF && !mbar_wait_or_abort(&p.tempty[buf], (tc / S::NBUF - 1) & 1, &p.abort_flag,
                                                          &g_wait_error, 2))
@@ -459,7 +464,8 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
                     uint64_t ad = descA + (uint32_t)st * (S::STAGE >> 4), bd = descB + (uint32_t)st * (S::STAGE >> 4);
 #pragma unroll
                     for (int q = 0; q < BK / 16; q++) {
-                        if (PAIR) mma_pair(dcol, ad, bd, idesc, more);
+                        if (q == 0 && left == hi) mma_scaled<PAIR ? 2 : 1, LO_BITS>(dcol, ad, bd, idesc);
+                        else if (PAIR) mma_pair(dcol, ad, bd, idesc, more);
                         else mma_bf16(dcol, ad, bd, idesc, more);
                         more = 1;
                         ad += stepA;
@@ -605,11 +611,14 @@ __global__ void __launch_bounds__(256) k_dz(const __grid_constant__ DzArgs a) {
                 Raw8<T> *to = reinterpret_cast<Raw8<T> *>(reinterpret_cast<T *>(a.dz) + m * a.ldp + c);
                 const Raw8<T> high = pack8<T>(v);
                 *to = high;
-                if (a.terms == 2) {  // what the first term leaves; nothing of an infinity or NaN
+                if (a.terms == 2) {  // lo: what the first term leaves; nothing of an infinity or NaN
                     f2 h[4];
                     unpack8<T>(high, h);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) at(v, i) = fabsf(at(h, i)) <= 3.4028234e38f ? at(v, i) - at(h, i) : 0.f;
+                    for (int i = 0; i < 8; i++) {
+                        constexpr float scale = std::is_same_v<T, __half> ? (float)(1 << LO_BITS) : 1.f;
+                        at(v, i) = fabsf(at(h, i)) <= 3.4028234e38f ? (at(v, i) - at(h, i)) * scale : 0.f;
+                    }
                     *reinterpret_cast<Raw8<T> *>(reinterpret_cast<T *>(to) + a.M * a.ldp) = pack8<T>(v);
                 }
             }
@@ -836,9 +845,7 @@ Plan plan(const gs_linear_desc *d, bool bwd) {
         p.o_part = take(parts(p.fwd, d->M, d->N));
     } else {
         p.need_dz = f32 || d->act != GS_ACT_NONE || ragged(d->ldy, d->unaligned & 4);
-        // rounding dz to 16 bits adds as much as rounding the result does.  Where dz is small (up to 2^16
-        // elements, whose products are bound by their launches) it keeps a second term instead.
-        p.dz_terms = f32 ? 3 : d->act != GS_ACT_NONE && d->M * d->N <= 1 << 16 ? 2 : 1;
+        p.dz_terms = f32 ? 3 : d->act != GS_ACT_NONE ? 2 : 1;  // (without an activation dz is dy)
         p.o_dz = take(p.need_dz ? (size_t)d->M * p.ldn * 2 * p.dz_terms : 0);
         p.gx = tiling(d->M, d->K, cdiv(d->N, BK), f32 ? 6 : p.dz_terms);
         p.gw = tiling(d->N, d->K, cdiv(d->M, BK), f32 ? 6 : p.dz_terms);

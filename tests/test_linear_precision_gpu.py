@@ -70,3 +70,37 @@ def test_gradients_of_saturated_units(ops, dtype):
         sums = 2 * U * (max(M, N) / 2 + 32)
         inside(dx, gx, half(dtype) * gx.abs() + (edz + sums * dz.abs()) @ W.abs() + least(dtype), "dx")
         inside(dw, gw, half(dtype) * gw.abs() + (edz + sums * dz.abs()).t() @ X.abs() + least(dtype), "dweight")
+
+
+def few_bits(*shape, seed, dtype, scale):
+    """Multiples of scale / 8 up to scale: short sums of their products are exact in fp32, so z is."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randint(-8, 9, shape, generator=g, device="cuda") * (scale / 8)).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("M,K,N,dy_scale", [(20, 16, 16, 1.0), (4096, 16, 16, 1.0), (4097, 16, 16, 1.0), (16, 16, 4096, 1.0),
+                                            (16, 16, 4104, 1.0), (16, 24, 5003, 1.0), (4999, 24, 19, 1.0),
+                                            (333, 24, 40, 2.0 ** -20)])
+def test_dz_is_not_rounded_to_the_type(ops, act, dtype, M, K, N, dy_scale):
+    """z exact, so the gradients' errors are dz's in the products and the results' own rounding.  dz keeps two terms of
+    x's type (h^2 of it; fp16's second term has 11 bits below fp16's smallest step), however many rows there are:
+    rounded once (h) it would break the bound of dx where N is small and of dweight where M is.  dbias sums dz itself."""
+    x, w = few_bits(M, K, seed=10, dtype=dtype, scale=1.0), few_bits(N, K, seed=11, dtype=dtype, scale=0.5)
+    b, dy = few_bits(N, seed=12, dtype=dtype, scale=1.0), rand(M, N, seed=13, dtype=dtype, scale=dy_scale)
+    ts = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(ops.linear_act(*ts, act=act), ts, dy)
+    X, W, B = x.double(), w.double(), b.double()
+    z, D, h = X @ W.t() + B, dy.double(), half(dtype)
+    dz = D * slope64(z, act)
+    slope = (ACT_U * U * (1 + z.abs()) if act == "gelu" else 64 * U * torch.sigmoid(z) * (1 + z.abs())) * D.abs() + U * dz.abs()
+    edz = slope + (2 ** -21 if dtype == torch.float32 else h * h) * dz.abs() + (least(dtype) * 2.0 ** -11 if dtype != torch.float32 else 0)
+
+    def sums(n):  # as check_linear's: the tensor cores add 16 at a time and may cut instead of rounding
+        return 2 * U * (n / 2 + 32)
+
+    lo = least(dtype) + 1e-30
+    inside(dx, dz @ W, h * (dz @ W).abs() + (edz + sums(N) * dz.abs()) @ W.abs() + lo, "dx")
+    inside(dw, dz.t() @ X, h * (dz.t() @ X).abs() + (edz + sums(M) * dz.abs()).t() @ X.abs() + lo, "dweight")
+    inside(db, dz.sum(0), h * dz.sum(0).abs() + (slope + (M / 2 + 32) * U * dz.abs()).sum(0) + lo, "dbias")
