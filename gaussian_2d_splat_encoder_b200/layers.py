@@ -83,6 +83,22 @@ def _rows_of(t, first):
     return t.shape[-1] if stride is None else stride
 
 
+def _save(ctx, *tensors):
+    ctx.save_for_backward(*tensors)
+    ctx.saved = [None if t is None else (t.shape, t.dtype, t.device) for t in tensors]
+
+
+def _unpack(ctx):
+    """The saved tensors.  Hooks on them (save_on_cpu, a checkpoint) may hand back copies in other strides, so a
+    backward takes layouts from what it gets here, never from the forward."""
+    tensors = ctx.saved_tensors
+    for t, kept in zip(tensors, ctx.saved):
+        if t is not None and (t.shape, t.dtype, t.device) != kept:
+            raise RuntimeError(f"a saved tensor came back as {tuple(t.shape)} {t.dtype} on {t.device}, kept was "
+                               f"{tuple(kept[0])} {kept[1]} on {kept[2]}")
+    return tensors
+
+
 # ------------------------------------------------------------------------------------ GroupNorm
 @functools.lru_cache(maxsize=1024)
 def _norm_plan(B, rows, channels, groups, dtype, param_dtype, act, act_first, eps, x_row, x_img, dy_row, dy_img):
@@ -114,8 +130,8 @@ def _norm_forward(x, weight, bias, groups, eps, act, act_first, train):
     B, channels = shape[0], shape[-1]
     p = weight if weight is not None else bias
     key = (B, x.numel() // (B * channels), channels, groups, _DTYPES[x.dtype], 0 if p is None else _DTYPES[p.dtype],
-           act, act_first, eps, x_row, x_img)
-    desc, nbytes, _, _ = _norm_plan(*key, 0, 0)
+           act, act_first, eps)
+    desc, nbytes, _, _ = _norm_plan(*key, x_row, x_img, 0, 0)
     if nbytes == 0:
         raise ValueError(f"unsupported sizes: {tuple(shape)} in {groups} groups")
     y = x.new_empty(shape)
@@ -131,14 +147,16 @@ def _norm_forward(x, weight, bias, groups, eps, act, act_first, train):
 
 
 def _norm_backward(ctx, dy):
-    x, weight, bias, buf = ctx.saved_tensors
+    x, weight, bias, buf = _unpack(ctx)
     dev = x.device
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return _norm_backward(ctx, dy)
     need = ctx.needs_input_grad
+    x, x_row, x_img = _image_layout(x)
+    weight, bias, buf = (t if t is None else t.contiguous() for t in (weight, bias, buf))
     dy, dy_row, dy_img = _image_layout(dy)
-    desc, _, nbytes, _ = _norm_plan(*ctx.key, dy_row, dy_img)
+    desc, _, nbytes, _ = _norm_plan(*ctx.key, x_row, x_img, dy_row, dy_img)
     dx = x.new_empty(x.shape) if need[0] else None
     dw = weight.new_empty(weight.shape) if need[1] else None
     db = bias.new_empty(bias.shape) if need[2] else None
@@ -156,7 +174,7 @@ class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act, act_first):
         y, x, buf, ctx.key = _norm_forward(x, weight, bias, groups, eps, act, act_first, True)
-        ctx.save_for_backward(x, weight, bias, buf)
+        _save(ctx, x, weight, bias, buf)
         return y
 
     backward = staticmethod(once_differentiable(_norm_backward))
@@ -231,6 +249,10 @@ def _row_layout(t):
     return (t.contiguous(), n) if row is None or row < n else (t, row)
 
 
+def _unaligned(px, pw, pg):
+    return (1 if px & 15 else 0) | (2 if pw & 15 else 0) | (4 if pg & 15 else 0)
+
+
 def _linear_forward(x, weight, bias, residual, act, train):
     dev = x.device
     if _elsewhere(dev):
@@ -243,9 +265,8 @@ def _linear_forward(x, weight, bias, residual, act, train):
         residual, ldr = _row_layout(residual)
     N, K = weight.shape
     px, pw = x.data_ptr(), weight.data_ptr()
-    unaligned = (1 if px & 15 else 0) | (2 if pw & 15 else 0)
-    key = (x.numel() // K, N, K, _DTYPES[x.dtype], act, ldx, ldw)
-    desc, nbytes, _, _ = _linear_plan(*key, ldr, 0, unaligned)
+    key = (x.numel() // K, N, K, _DTYPES[x.dtype], act)
+    desc, nbytes, _, _ = _linear_plan(*key, ldx, ldw, ldr, 0, _unaligned(px, pw, 0))
     if nbytes == 0:
         raise ValueError(f"unsupported sizes: {tuple(x.shape)} and {tuple(weight.shape)}")
     shape = x.shape[:-1] + (N,)
@@ -259,27 +280,29 @@ def _linear_forward(x, weight, bias, residual, act, train):
                                              None if slope is None else slope.data_ptr(),
                                              None if ws is None else ws.data_ptr(), nbytes, _raw_stream(dev.index)),
                "gs_linear_act_fwd")
-    return y, x, weight, slope, key + (unaligned,)
+    return y, x, weight, slope, key
 
 
 def _linear_backward(ctx, dy):
-    x, weight, slope = ctx.saved_tensors
     need = ctx.needs_input_grad
     if not (need[0] or need[1] or need[2]):
         return None, None, None, dy if need[3] else None, None
+    x, weight, slope = _unpack(ctx)
     dev = x.device
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return _linear_backward(ctx, dy)
+    x, ldx = _row_layout(x)
+    weight, ldw = _row_layout(weight)
+    slope = None if slope is None else slope.contiguous()
     g, ldy = _row_layout(dy)
-    *key, unaligned = ctx.key
-    pg = g.data_ptr()
-    desc, _, nbytes, _ = _linear_plan(*key, 0, ldy, unaligned | (4 if pg & 15 else 0))
+    px, pw, pg = x.data_ptr(), weight.data_ptr(), g.data_ptr()
+    desc, _, nbytes, _ = _linear_plan(*ctx.key, ldx, ldw, 0, ldy, _unaligned(px, pw, pg))
     dx = x.new_empty(x.shape) if need[0] else None
     dw = weight.new_empty(weight.shape) if need[1] else None
     db = weight.new_empty(weight.shape[0]) if need[2] else None
     ws = x.new_empty(nbytes, dtype=torch.uint8)
-    _lib.check(_lib.load().gs_linear_act_bwd(desc, x.data_ptr(), weight.data_ptr(),
+    _lib.check(_lib.load().gs_linear_act_bwd(desc, px, pw,
                                              None if slope is None else slope.data_ptr(), pg,
                                              None if dx is None else dx.data_ptr(),
                                              None if dw is None else dw.data_ptr(),
@@ -292,7 +315,7 @@ class _LinearAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
         y, x, weight, slope, ctx.key = _linear_forward(x, weight, bias, residual, act, True)
-        ctx.save_for_backward(x, weight, slope)
+        _save(ctx, x, weight, slope)
         return y
 
     backward = staticmethod(once_differentiable(_linear_backward))

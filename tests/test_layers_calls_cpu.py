@@ -1,0 +1,93 @@
+"""What the layer operators hand to the library, seen on the CPU: autograd runs in earnest, the launches are recorded
+instead of made."""
+
+import ctypes as C
+
+import pytest
+import torch
+
+
+class Recorder:
+    """The library with the four launching entries replaced by a list of (name, descriptor's fields, arguments)."""
+
+    def __init__(self, lib):
+        self.lib, self.calls = lib, []
+
+    def __getattr__(self, name):
+        if not name.endswith(("_fwd", "_bwd")):
+            return getattr(self.lib, name)
+
+        def call(desc, *args):
+            d = desc._obj
+            self.calls.append((name, {f: getattr(d, f) for f, _ in d._fields_}, args))
+            return 0
+
+        return call
+
+
+@pytest.fixture
+def ops(lib, monkeypatch):
+    from gaussian_2d_splat_encoder_b200 import _lib, layers
+
+    rec = Recorder(lib)
+    monkeypatch.setattr(_lib, "load", lambda: rec)
+    monkeypatch.setattr(_lib, "require_cuda", lambda *t: t[0].device)
+    monkeypatch.setattr(layers, "_elsewhere", lambda dev: False)
+    monkeypatch.setattr(layers, "_raw_stream", lambda index: 0)
+    layers._norm_plan.cache_clear()
+    layers._linear_plan.cache_clear()
+    layers.rec = rec
+    yield layers
+    layers._norm_plan.cache_clear()
+    layers._linear_plan.cache_clear()
+    del layers.rec
+
+
+def compact_copies():
+    """Saved tensors come back as copies of their own, as torch.autograd.graph.save_on_cpu hands them back."""
+    return torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(memory_format=torch.contiguous_format),
+                                                    lambda t: t)
+
+
+@pytest.mark.parametrize("view", ["slice", "expanded", "images"])
+def test_norm_backward_takes_the_layout_of_what_it_reads(ops, view):
+    wide = torch.randn(2, 5, 96)
+    x = {"slice": wide[..., 32:64], "expanded": wide[:1, :1, :32].expand(2, 5, 32), "images": wide[:, ::2, :32]}[view]
+    x = x.detach().requires_grad_(True)
+    with compact_copies():
+        y = ops.group_norm_act(x, 4, act="gelu")
+    torch.autograd.grad(y, x, torch.zeros_like(y))
+    (_, fwd, _), (_, bwd, _) = ops.rec.calls
+    assert (fwd["x_row"], fwd["x_img"]) == {"slice": (96, 480), "expanded": (0, 0), "images": (192, 480)}[view]
+    assert (bwd["x_row"], bwd["x_img"]) == (32, 32 * x.shape[1])
+
+
+@pytest.mark.parametrize("offset", [0, 3])
+def test_linear_backward_takes_the_layout_of_what_it_reads(ops, offset):
+    wide, wt = torch.randn(9, 200), torch.randn(50, 120)
+    x = wide[:, offset:offset + 80].detach().requires_grad_(True)
+    w = wt[::2, offset:offset + 80].detach().requires_grad_(True)
+    with compact_copies():
+        y = ops.linear_act(x, w, act="silu")
+    torch.autograd.grad(y, (x, w), torch.zeros_like(y))
+    (_, fwd, _), (_, bwd, args) = ops.rec.calls
+    assert (fwd["ldx"], fwd["ldw"]) == (200, 240) and bool(fwd["unaligned"] & 3) == bool(offset)
+    assert (bwd["ldx"], bwd["ldw"]) == (80, 80)
+    assert bwd["unaligned"] == sum(bit << k for k, bit in enumerate([args[0] & 15 != 0, args[1] & 15 != 0, args[3] & 15 != 0]))
+
+
+def test_plain_backward_keeps_the_forward_layout(ops):
+    x = torch.randn(2, 5, 96)[..., 32:64].requires_grad_(True)
+    y = ops.group_norm_act(x, 4)
+    torch.autograd.grad(y, x, torch.zeros_like(y))
+    assert all((d["x_row"], d["x_img"]) == (96, 480) for _, d, _ in ops.rec.calls)
+
+
+@pytest.mark.parametrize("change", [lambda t: t.double(), lambda t: t[..., :1], lambda t: t.to("meta")])
+def test_changed_saved_tensors_are_refused(ops, change):
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+        for y in (ops.group_norm_act(torch.randn(2, 5, 32, requires_grad=True), 4),
+                  ops.linear_act(torch.randn(5, 32, requires_grad=True), torch.randn(8, 32))):
+            with pytest.raises(RuntimeError, match="saved tensor came back"):
+                y.sum().backward()
+    assert [n for n, _, _ in ops.rec.calls] == ["gs_group_norm_act_fwd", "gs_linear_act_fwd"]

@@ -1,0 +1,68 @@
+"""Calls of the layer operators that torch allows around them: hooks on saved tensors, checkpoints."""
+
+import pytest
+import torch
+
+from layers_util import rand
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope="module")
+def ops(lib):
+    from gaussian_2d_splat_encoder_b200 import layers
+
+    return layers
+
+
+def both_ways(run, leaves, dy, around):
+    """Gradients of run(*leaves) plainly and inside `around`."""
+    plain = torch.autograd.grad(run(*leaves), leaves, dy)
+    with around:
+        y = run(*leaves)
+    return plain, torch.autograd.grad(y, leaves, dy)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("view", ["slice", "unaligned", "images", "expanded"])
+def test_saved_on_cpu(ops, view, dtype):
+    """Saved tensors that come back compact: the same gradients, to the bit, as the layout changes no sum."""
+    wide, w, b = rand(3, 50, 96, seed=1, dtype=dtype), rand(32, seed=2, shift=1.0), rand(32, seed=3)
+    x = {"slice": wide[..., 32:64], "unaligned": wide[..., 5:37], "images": wide[:, ::2, :32],
+         "expanded": wide[:1, :1, :32].expand(3, 50, 32)}[view].detach().requires_grad_(True)
+    leaves = [x, w.requires_grad_(True), b.requires_grad_(True)]
+    for act, first in (("gelu", True), ("silu", False)):
+        plain, hooked = both_ways(lambda *t: ops.group_norm_act(t[0], 4, t[1], t[2], act=act, act_first=first), leaves,
+                                  rand(*x.shape, seed=4, dtype=dtype), torch.autograd.graph.save_on_cpu())
+        assert all(torch.equal(p, h) for p, h in zip(plain, hooked))
+    wt = rand(80, 64, seed=5, dtype=dtype, scale=0.2)
+    wl = (wt[::2, 32:] if view == "images" else wt[:, 3:35] if view == "unaligned" else wt[:, :32]).detach().requires_grad_(True)
+    bl = rand(wl.shape[0], seed=6, dtype=dtype).requires_grad_(True)
+    for act in ("none", "gelu"):
+        plain, hooked = both_ways(lambda *t: ops.linear_act(*t, act=act), [x, wl, bl],
+                                  rand(*x.shape[:-1], wl.shape[0], seed=7, dtype=dtype), torch.autograd.graph.save_on_cpu())
+        assert all(torch.equal(p, h) for p, h in zip(plain, hooked))
+
+
+def test_checkpointed(ops):
+    from torch.utils.checkpoint import checkpoint
+
+    wide, w = rand(2, 40, 96, seed=8, dtype=torch.bfloat16), rand(48, 32, seed=9, dtype=torch.bfloat16, scale=0.2)
+    x = wide[..., 32:64].detach().requires_grad_(True)
+    w.requires_grad_(True)
+
+    def block(x, w):
+        return ops.linear_act(ops.group_norm_act(x, 4, act="gelu", act_first=True), w, act="silu")
+
+    dy = rand(2, 40, 48, seed=10, dtype=torch.bfloat16)
+    plain = torch.autograd.grad(block(x, w), (x, w), dy)
+    for reentrant in (False, True):
+        y = checkpoint(block, x, w, use_reentrant=reentrant)
+        if reentrant:  # (runs its own backward inside, so by .backward())
+            y.backward(dy)
+            got = (x.grad, w.grad)
+        else:
+            got = torch.autograd.grad(y, (x, w), dy)
+        assert all(torch.equal(p, g) for p, g in zip(plain, got))
