@@ -935,6 +935,8 @@ extern "C" int gs_group_norm_act_bwd(const gs_norm_desc *d, const void *x, const
     a.nslice = dx ? a.B * a.splits * a.nchunk : 0;
     a.part = reinterpret_cast<float *>(al((uintptr_t)workspace));
     a.cpart = reinterpret_cast<float *>(reinterpret_cast<char *>(a.part) + part_bytes(a));
-    const bool vec = aligned(x, a.x_row, a.x_img) && aligned(dy, a.dy_row, a.dy_img) && (!dx || aligned(dx, a.C, 0));
+    // (whole vectors of channels too: without dx no tightly packed row says so)
+    const bool vec = a.C % V == 0 && aligned(x, a.x_row, a.x_img) && aligned(dy, a.dy_row, a.dy_img) &&
+                     (!dx || aligned(dx, a.C, 0));
     return by_type<true>(d, a, vec, (cudaStream_t)stream);
 }

@@ -66,3 +66,17 @@ def test_checkpointed(ops):
         else:
             got = torch.autograd.grad(y, (x, w), dy)
         assert all(torch.equal(p, g) for p, g in zip(plain, got))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_parameters_only_off_eight_channels(ops, dtype):
+    """Strides on eight and twelve channels, dx not wanted: the parameters' gradients are those of the full backward
+    (one pixel's row expanded over the map ends its memory at the twelfth channel)."""
+    w, b = rand(12, seed=11, shift=1.0).requires_grad_(True), rand(12, seed=12).requires_grad_(True)
+    wide = rand(1, 50, 16, seed=13, dtype=dtype)
+    for x, dy in ((wide[..., :12], wide[..., :12]),
+                  (rand(1, 1, 12, seed=14, dtype=dtype).expand(1, 50, 12), rand(1, 1, 12, seed=15, dtype=dtype).expand(1, 50, 12))):
+        got = torch.autograd.grad(ops.group_norm_act(x, 3, w, b, act="silu"), (w, b), dy)
+        xs = x.detach().clone(memory_format=torch.contiguous_format).requires_grad_(True)
+        ref = torch.autograd.grad(ops.group_norm_act(xs, 3, w, b, act="silu"), (xs, w, b), dy.contiguous())
+        assert all(torch.equal(g, r) for g, r in zip(got, ref[1:]))
