@@ -68,6 +68,7 @@ SIGNATURES = {
     "gs_linear_act_fwd": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
     "gs_linear_act_bwd": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
     "gs_linear_error_flag": (C.c_int, [_P]),
+    "gs_linear_debug_wait": (C.c_int, [C.c_uint32, _P]),
     "gs_last_error": (C.c_char_p, []),
     "gs_kernel_launches": (C.c_uint64, []),
     "gs_profile_enable": (None, [C.c_int]),
@@ -118,7 +119,7 @@ def check(status: int, what: str = "") -> None:
     if status == GS_ERR_WORKSPACE:
         raise RuntimeError(f"{what}: workspace too small")
     if status == GS_ERR_TIMEOUT:
-        raise RuntimeError(f"{what}: device wait timed out")
+        raise RuntimeError(f"{what}: device wait timed out {msg}".rstrip())
     raise RuntimeError(f"{what}: CUDA error: {msg}")
 
 

@@ -41,8 +41,6 @@ namespace {
 constexpr int SMS = 148;  // of a B200: tiles, splits and the workspace are a matter of sizes alone
 constexpr int BM = 128, BK = 64;
 
-__device__ int g_wait_error;  // code of a bounded wait that gave up (gs_linear_error_flag), 0 if none did
-
 struct GemmArgs {
     long long I;          // rows of D
     int J;                // columns of D
@@ -58,6 +56,7 @@ struct GemmArgs {
     void *out;
     float *slope;
     long long ldr;
+    int *wait_error;      // host word for the code of a bounded wait that gives up
 };
 
 // term products, small ones first: (a term, b term), 0 = high; the six of fp32, then the two of A in two terms
@@ -84,7 +83,7 @@ enum { EPI_NONE = 0, EPI_GELU = 1, EPI_SILU = 2, EPI_GELU_SLOPE = 3, EPI_SILU_SL
 // residual: 387 us, 1420 TFLOP/s, against 569).  The leader issues all MMAs.
 // Bound by: long sums, the tensor cores and their loads' latency; short ones, the epilogue's instructions (GELU is
 // 11 of some 20 an output; 36864x128->512 takes 23.3 us where its bytes take 7.3).
-// Every wait is bounded; one that gives up records a code in g_wait_error and raises the CTA's abort flag.
+// Every wait is bounded; one that gives up writes its code to wait_error and raises the CTA's abort flag.
 template <int BN, bool PAIR, bool OUT32, int EPI>
 struct Shape {
     static constexpr int BROWS = PAIR ? BN / 2 : BN;  // rows of B in this CTA
@@ -215,12 +214,12 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ri
                 }
             }
             if (u == 0) {
-                if (!mbar_wait_or_abort(&p.tfull[buf], (tc / S::NBUF) & 1, &p.abort_flag, &g_wait_error, 5)) dead = true;
+                if (!mbar_wait_or_abort(&p.tfull[buf], (tc / S::NBUF) & 1, &p.abort_flag, a.wait_error, 5)) dead = true;
                 tc_fence_after();
             }
             if (live && pending) {
                 // (after an abort too: the copy lands in this CTA's shared memory)
-                if (!mbar_wait(&p.rbar[e][sl], (use >> 1) & 1, &g_wait_error, 6)) {
+                if (!mbar_wait(&p.rbar[e][sl], (use >> 1) & 1, a.wait_error, 6)) {
                     p.abort_flag = 1;
                     dead = true;
                 }
@@ -328,7 +327,7 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ri
             use++;
         }
     }
-    if (pending) mbar_wait(&p.rbar[e][use & 1], (use >> 1) & 1, &g_wait_error, 8);
+    if (pending) mbar_wait(&p.rbar[e][use & 1], (use >> 1) & 1, a.wait_error, 8);
     if (lane == 0) bulk_wait<0>();
     __syncwarp();
 }
@@ -396,7 +395,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
                 int kk = k0, pr = a.npair == 2 ? 6 : 0, left = t.blocks(a);
                 int ta = a.npair > 1 ? PAIR_A[pr] : 0, tb = a.npair > 1 ? PAIR_B[pr] : 0;
                 for (; left > 0; left--, it++) {
-                    if (!mbar_wait_or_abort(&p.empty[st], parity, &p.abort_flag, &g_wait_error, 1)) break;
+                    if (!mbar_wait_or_abort(&p.empty[st], parity, &p.abort_flag, a.wait_error, 1)) break;
                     uint8_t *sa = smem + st * S::STAGE, *sb = sa + S::A_BYTES;
                     // both CTAs' copies complete on the leader's barrier
                     if (rank == 0) mbar_arrive_expect_tx(&p.full[st], S::STAGE * (PAIR ? 2 : 1));
@@ -449,14 +448,14 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
                 const int hi = a.npair == 2 && a.f16 ? left / 2 : -1;  // k-blocks left when hi follows lo
                 const int buf = tc % S::NBUF;
                 if (tc >= S::NBUF && !mbar_wait_or_abort(&p.tempty[buf], (tc / S::NBUF - 1) & 1, &p.abort_flag,
-                                                         &g_wait_error, 2))
+                                                         a.wait_error, 2))
                     break;
                 tc_fence_after();
                 const uint32_t dcol = tbase + (uint32_t)buf * BN;
                 bool ok = true;
                 uint32_t more = 0;
                 for (; left > 0; left--, it++) {
-                    if (!mbar_wait_or_abort(&p.full[st], parity, &p.abort_flag, &g_wait_error, 3)) {
+                    if (!mbar_wait_or_abort(&p.full[st], parity, &p.abort_flag, a.wait_error, 3)) {
                         ok = false;
                         break;
                     }
@@ -486,7 +485,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
             // all MMAs of this CTA or pair (also those of an aborted item) have finished once mdone flips
             if (PAIR) mma_commit_pair(&p.mdone);
             else mma_commit(&p.mdone);
-            mbar_wait(&p.mdone, 0, &g_wait_error, 4);
+            mbar_wait(&p.mdone, 0, a.wait_error, 4);
         }
     } else {
         epilogue<BN, PAIR, OUT32, EPI>(a, p, smem + STAGES * S::STAGE, &tmO, &tmS, &tmR, first, stride, n_items, rank);
@@ -497,7 +496,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
     if (PAIR) cluster_arrive_wait();  // no CTA leaves while its peer's copies, MMAs or arrivals may reach it
     if (p.abort_flag && threadIdx.x == 0 && rank == 0)
         // copies that were issued but never consumed still land in shared memory: wait for them
-        for (int j = p.consumed; j < p.issued; j++) mbar_wait(&p.full[j % STAGES], (j / STAGES) & 1, &g_wait_error, 7);
+        for (int j = p.consumed; j < p.issued; j++) mbar_wait(&p.full[j % STAGES], (j / STAGES) & 1, a.wait_error, 7);
     __syncthreads();
     if (PAIR) cluster_arrive_wait();
     tc_fence_after();
@@ -898,6 +897,34 @@ bool make_map(CUtensorMap *tm, CUtensorMapDataType type, int es, const void *bas
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// The word that waits report to: pinned host memory that every device sees, so that the host reads it without a copy
+// or a wait.  NULL where there is no device.
+int *wait_error() {
+    static int *const word = [] {
+        // (an allocation is no work of a stream: made while one is captured too)
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        const bool set = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
+        int *p = nullptr;
+        if (cudaHostAlloc(reinterpret_cast<void **>(&p), sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess) p = nullptr;
+        if (set) cudaThreadExchangeStreamCaptureMode(&mode);
+        if (p) *p = 0;
+        return p;
+    }();
+    return word;
+}
+int take_wait_error(int *word) { return __atomic_load_n(word, __ATOMIC_RELAXED) ? __atomic_exchange_n(word, 0, __ATOMIC_ACQ_REL) : 0; }
+// reports what an earlier call's waits left, once
+int check_waits(const char *where) {
+    int *const word = wait_error();
+    if (!word) return cuda_error(where, "no pinned host memory");
+    const int code = take_wait_error(word);
+    if (!code) return GS_OK;
+    char msg[128];
+    snprintf(msg, sizeof(msg), "%s: a device wait of an earlier linear call gave up (code %d), its outputs are not valid", where, code);
+    gs_set_last_error(msg);
+    return GS_ERR_TIMEOUT;
+}
+
 template <int BN, bool PAIR, bool OUT32, int EPI>
 int launch(const CUtensorMap *m, const GemmArgs &a, bool follows, cudaStream_t s) {
     using S = Shape<BN, PAIR, OUT32, EPI>;
@@ -955,6 +982,7 @@ int product(const gs_linear_desc *d, const Plan &p, const Tiling &t, long long I
     a.f16 = d->dtype == GS_F16;
     a.out_f16 = a.f16;
     a.splits = t.splits; a.tiles_i = t.tiles_i; a.tiles_j = t.tiles_j;
+    a.wait_error = wait_error();
     CUtensorMap m[5];
     const CUtensorMapDataType in = a.f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     bool ok = make_map(&m[0], in, 2, A.p, A.cols, A.rows, A.ld, A.terms, 64, A.mn ? BK : BM) &&
@@ -1100,6 +1128,7 @@ extern "C" int gs_linear_act_fwd(const gs_linear_desc *d, const void *x, const v
         return GS_ERR_BAD_ARGUMENT;
     const Plan p = plan(d, false);
     if (p.bytes > 256 && (!workspace || workspace_bytes < p.bytes)) return GS_ERR_WORKSPACE;
+    if (const int st = check_waits("gs_linear_act_fwd")) return st;
     cudaStream_t s = (cudaStream_t)stream;
     const Epilogue e{bias, residual, d->ldr, d->act, y, d->act == GS_ACT_NONE ? nullptr : slope};
     if (d->dtype == GS_F32) return forward<float>(d, p, x, w, e, workspace, s);
@@ -1124,6 +1153,7 @@ extern "C" int gs_linear_act_bwd(const gs_linear_desc *d, const void *x, const v
         return GS_ERR_BAD_ARGUMENT;
     const Plan p = plan(d, true);
     if (p.bytes > 256 && (!workspace || workspace_bytes < p.bytes)) return GS_ERR_WORKSPACE;
+    if (const int st = check_waits("gs_linear_act_bwd")) return st;
     if (d->act == GS_ACT_NONE) slope = nullptr;
     if (d->dtype == GS_F32) return backward<float>(d, p, x, w, slope, dy, dx, dw, dbias, workspace, s);
     if (d->dtype == GS_BF16) return backward<__nv_bfloat16>(d, p, x, w, slope, dy, dx, dw, dbias, workspace, s);
@@ -1132,6 +1162,26 @@ extern "C" int gs_linear_act_bwd(const gs_linear_desc *d, const void *x, const v
 
 extern "C" int gs_linear_error_flag(int *flag_host) {
     if (!flag_host) return GS_ERR_BAD_ARGUMENT;
-    const cudaError_t e = cudaMemcpyFromSymbol(flag_host, g_wait_error, sizeof(int));
-    return e == cudaSuccess ? GS_OK : cuda_error("gs_linear_error_flag", cudaGetErrorString(e));
+    const cudaError_t e = cudaDeviceSynchronize();
+    if (e != cudaSuccess) return cuda_error("gs_linear_error_flag", cudaGetErrorString(e));
+    int *const word = wait_error();
+    if (!word) return cuda_error("gs_linear_error_flag", "no pinned host memory");
+    *flag_host = take_wait_error(word);
+    return GS_OK;
+}
+
+// one thread waits for a barrier that nothing arrives at, and reports as k_gemm does
+__global__ void k_wait_in_vain(unsigned limit, int *err) {
+    __shared__ uint64_t bar;
+    mbar_init(&bar, 1);
+    fence_barrier_init();
+    mbar_wait(&bar, 0, err, 255, limit);
+}
+extern "C" int gs_linear_debug_wait(uint32_t limit, void *stream) {
+    if (limit > 1024) return GS_ERR_BAD_ARGUMENT;
+    int *const word = wait_error();
+    if (!word) return cuda_error("gs_linear_debug_wait", "no pinned host memory");
+    k_wait_in_vain<<<1, 1, 0, (cudaStream_t)stream>>>(limit, word);
+    gs_count_launch(1);
+    return done("gs_linear_debug_wait");
 }

@@ -11,6 +11,10 @@ or projection that is trained needs the same pieces one by one, differentiable, 
 Both take fp32, bf16 or fp16 CUDA tensors, keep every sum and statistic in fp32, round once to the tensor's
 type and give the same bits for the same inputs.  They run on the current stream of the tensors' device
 and can be captured into a CUDA graph.  The gradients are once differentiable.
+
+The waits inside linear_act's kernels are bounded.  One that gives up leaves that call's outputs invalid; calls are
+asynchronous, so the next call of linear_act (or its backward) raises RuntimeError, or ``check_linear_waits()``, which
+waits for the device first: after the replays of a captured graph, or before results are used for good.
 """
 
 from __future__ import annotations
@@ -352,3 +356,12 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     if grad and torch.is_grad_enabled():
         return _LinearAct.apply(x, weight, bias, residual, code)
     return _linear_forward(x, weight, bias, residual, code, False)[0]
+
+
+def check_linear_waits() -> None:
+    """Waits for the current device and raises RuntimeError if a device wait of an earlier ``linear_act`` (or its
+    backward, or a replay of either) gave up since the last such error: outputs since then may be invalid."""
+    L, code = _lib.load(), C.c_int(0)
+    _lib.check(L.gs_linear_error_flag(C.byref(code)), "gs_linear_error_flag")
+    if code.value:
+        raise RuntimeError(f"linear_act: a device wait gave up (code {code.value}); outputs of earlier calls are not valid")

@@ -307,9 +307,13 @@ int gs_linear_act_fwd(const gs_linear_desc *d, const void *x, const void *w, con
  * slope is the forward's, not read without an activation.  The residual's gradient is dy itself. */
 int gs_linear_act_bwd(const gs_linear_desc *d, const void *x, const void *w, const float *slope, const void *dy, void *dx,
                       void *dw, void *dbias, void *workspace, size_t workspace_bytes, void *stream);
-/* Reads (synchronously) the code of a bounded device wait of the linear kernels that gave up on the current
- * device since the library was loaded; 0 if none did.  Outputs of such a call are not valid. */
+/* The linear kernels' device waits are bounded.  One that gives up leaves its call's outputs invalid; the call has
+ * returned by then, so the next gs_linear_act_fwd or _bwd of the process returns GS_ERR_TIMEOUT (once, without
+ * launching).  This call waits for the current device and takes the code (0: none gave up) in its place, as after
+ * the replay of a captured graph. */
 int gs_linear_error_flag(int *flag_host);
+/* Launches a wait that gives up after `limit` (at most 1024) polls, to see a program's handling of one. */
+int gs_linear_debug_wait(uint32_t limit, void *stream);
 
 /* Text of the last CUDA error seen by the calling thread (empty when none). */
 const char *gs_last_error(void);

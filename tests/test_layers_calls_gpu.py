@@ -80,3 +80,26 @@ def test_norm_parameters_only_off_eight_channels(ops, dtype):
         xs = x.detach().clone(memory_format=torch.contiguous_format).requires_grad_(True)
         ref = torch.autograd.grad(ops.group_norm_act(xs, 3, w, b, act="silu"), (xs, w, b), dy.contiguous())
         assert all(torch.equal(g, r) for g, r in zip(got, ref[1:]))
+
+
+def test_a_wait_that_gave_up_is_reported(ops, lib):
+    """The next call raises, once; the check function waits and raises; nothing is left behind."""
+    x, w = rand(20, 16, seed=16), rand(8, 16, seed=17).requires_grad_(True)
+    ref = ops.linear_act(x, w, act="silu")
+    ops.check_linear_waits()
+    assert lib.gs_linear_debug_wait(1025, None) == 2
+    assert lib.gs_linear_debug_wait(16, None) == 0
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="gave up"):
+        ops.linear_act(x, w, act="silu")
+    y = ops.linear_act(x, w, act="silu")
+    assert torch.equal(y, ref)
+    assert lib.gs_linear_debug_wait(16, None) == 0
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="gave up"):
+        torch.autograd.grad(y, w, ref.detach(), retain_graph=True)
+    torch.autograd.grad(y, w, ref.detach())
+    assert lib.gs_linear_debug_wait(16, None) == 0
+    with pytest.raises(RuntimeError, match="gave up"):
+        ops.check_linear_waits()
+    ops.check_linear_waits()
