@@ -10,7 +10,8 @@ or projection that is trained needs the same pieces one by one, differentiable, 
 
 Both take fp32, bf16 or fp16 CUDA tensors, keep every sum and statistic in fp32, round once to the tensor's
 type and give the same bits for the same inputs.  They run on the current stream of the tensors' device
-and can be captured into a CUDA graph.  The gradients are once differentiable.
+and can be captured into a CUDA graph.  The gradients are once differentiable, in reverse mode
+alone: dual tensors and the transforms of torch.func are refused.
 
 The waits inside linear_act's kernels are bounded.  One that gives up leaves that call's outputs invalid; calls are
 asynchronous, so the next call of linear_act (or its backward) raises RuntimeError, or ``check_linear_waits()``, which
@@ -23,6 +24,7 @@ import ctypes as C
 import functools
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -59,6 +61,14 @@ def _dtype_code(name, t):
     if t.dtype not in _DTYPES:
         raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
     return _DTYPES[t.dtype]
+
+
+def _refuse_tangents(*tensors):
+    """The kernels see values alone: the tangent of a dual tensor would be dropped without a word."""
+    if forward_ad._current_level < 0:
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("the layer operators have no forward-mode derivatives (got a dual tensor)")
 
 
 def _elsewhere(dev):
@@ -151,6 +161,7 @@ def _norm_forward(x, weight, bias, groups, eps, act, act_first, train):
 
 
 def _norm_backward(ctx, dy):
+    _refuse_tangents(dy)
     x, weight, bias, buf = _unpack(ctx)
     dev = x.device
     if _elsewhere(dev):
@@ -205,6 +216,7 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
     without a copy; so do channel slices of a wider map and expanded tensors, while other strides are
     copied.  Returns a contiguous tensor of x's shape and type.  C is at most 2048."""
     dev = _lib.require_cuda(x, weight, bias)
+    _refuse_tangents(x, weight, bias)
     code = _act_code(act)
     _dtype_code("x", x)
     if x.dim() < 2:
@@ -288,6 +300,7 @@ def _linear_forward(x, weight, bias, residual, act, train):
 
 
 def _linear_backward(ctx, dy):
+    _refuse_tangents(dy)
     need = ctx.needs_input_grad
     if not (need[0] or need[1] or need[2]):
         return None, None, None, dy if need[3] else None, None
@@ -335,6 +348,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     rounded once, after the residual.  Rows may be strided (channel slices of a wider map); other strides are
     copied.  Returns a contiguous tensor [..., N]."""
     _lib.require_cuda(x, weight, bias, residual)
+    _refuse_tangents(x, weight, bias, residual)
     code = _act_code(act)
     _dtype_code("x", x)
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:

@@ -91,3 +91,45 @@ def test_changed_saved_tensors_are_refused(ops, change):
             with pytest.raises(RuntimeError, match="saved tensor came back"):
                 y.sum().backward()
     assert [n for n, _, _ in ops.rec.calls] == ["gs_group_norm_act_fwd", "gs_linear_act_fwd"]
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_dual_tensors_are_refused(ops, which):
+    from torch.autograd import forward_ad
+
+    ts = [torch.randn(5, 32), torch.randn(8, 32), torch.randn(8), torch.randn(5, 8)]
+    with forward_ad.dual_level():
+        ts[which] = forward_ad.make_dual(ts[which], torch.ones_like(ts[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.linear_act(ts[0], ts[1], ts[2], act="gelu", residual=ts[3])
+        ns = [torch.randn(2, 5, 8), torch.randn(8), torch.randn(8)]
+        if which < 3:
+            ns[which] = forward_ad.make_dual(ns[which], torch.ones_like(ns[which]))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                ops.group_norm_act(ns[0], 4, ns[1], ns[2])
+    assert not ops.rec.calls
+    # without a tangent a dual level changes nothing
+    with forward_ad.dual_level():
+        ops.linear_act(torch.randn(5, 32), torch.randn(8, 32))
+        ops.group_norm_act(torch.randn(2, 5, 8), 4)
+    assert len(ops.rec.calls) == 2
+
+
+def test_dual_gradients_are_refused(ops):
+    from torch.autograd import forward_ad
+
+    for y, x in ((ops.group_norm_act(x, 4), x) if k else (ops.linear_act(x, torch.randn(8, 32)), x)
+                 for k, x in enumerate(torch.randn(2, 5, 32, requires_grad=True) for _ in range(2))):
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, x, forward_ad.make_dual(torch.zeros_like(y), torch.ones_like(y)))
+    assert all(n.endswith("_fwd") for n, _, _ in ops.rec.calls)
+
+
+def test_function_transforms_are_refused(ops):
+    x, w = torch.randn(2, 5, 8), torch.randn(3, 8)
+    for f in (lambda t: ops.group_norm_act(t, 4).sum(), lambda t: ops.linear_act(t, w).sum()):
+        for transform in (lambda: torch.func.jvp(f, (x,), (x,)), lambda: torch.func.grad(f)(x),
+                          lambda: torch.func.vmap(f)(x.unsqueeze(1))):
+            with pytest.raises(RuntimeError):
+                transform()
+    assert not ops.rec.calls
