@@ -31,6 +31,7 @@ from . import _lib
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTS = {"none": 0, "gelu": 1, "silu": 2}
+_MAX_IMAGES = 1 << 30  # of a norm call
 _NO_WORKSPACE = 256  # a linear call whose size query answers this needs none
 
 
@@ -117,6 +118,8 @@ def _unpack(ctx):
 @functools.lru_cache(maxsize=1024)
 def _norm_plan(B, rows, channels, groups, dtype, param_dtype, act, act_first, eps, x_row, x_img, dy_row, dy_img):
     """Descriptor of a call's sizes and the workspace of its forward and backward."""
+    if B > _MAX_IMAGES:  # (beyond its field in the descriptor, which would keep the low bits)
+        return None, 0, 0, None
     d = _NormDesc(B, channels, groups, dtype, param_dtype, act, act_first, eps, rows, x_row, x_img, dy_row, dy_img)
     L = _lib.load()
     size = L.gs_group_norm_act_workspace_size
@@ -214,7 +217,8 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
     num_groups = C is an instance norm.  weight and bias [C] are float32 or of x's type, both alike, and
     default to 1 and 0.  An NCHW tensor in channels_last memory format enters as ``x.permute(0, 2, 3, 1)``
     without a copy; so do channel slices of a wider map and expanded tensors, while other strides are
-    copied.  Returns a contiguous tensor of x's shape and type.  C is at most 2048."""
+    copied.  Returns a contiguous tensor of x's shape and type.  C is at most 2048, images and the
+    rows of one at most 2^30."""
     dev = _lib.require_cuda(x, weight, bias)
     _refuse_tangents(x, weight, bias)
     code = _act_code(act)

@@ -133,3 +133,10 @@ def test_function_transforms_are_refused(ops):
             with pytest.raises(RuntimeError):
                 transform()
     assert not ops.rec.calls
+
+
+@pytest.mark.parametrize("images", [(1 << 30) + 1, (1 << 32) + 4])
+def test_more_images_than_the_descriptor_holds(ops, images):
+    with pytest.raises(ValueError, match="unsupported sizes"):
+        ops.group_norm_act(torch.ones(1, 1, 1).expand(images, 1, 1), 1)
+    assert not ops.rec.calls
