@@ -127,7 +127,9 @@ def _norm_plan(B, rows, channels, groups, dtype, param_dtype, act, act_first, ep
 
 
 def _image_layout(t):
-    """`t` [B, ..., C] with its row and image strides; a copy where the layout has no such strides."""
+    """`t` [B, ..., C] with its row and image strides; a copy where the layout has no such strides (or the values
+    a pending sign)."""
+    t = t.resolve_neg()
     if t.is_contiguous():
         C_ = t.shape[-1]
         return t, C_, t.numel() // max(1, t.shape[0])
@@ -235,10 +237,10 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
     grad = x.requires_grad
     if weight is not None:
         _check_param("weight", weight, x, channels)
-        grad, weight = grad or weight.requires_grad, weight.contiguous()
+        grad, weight = grad or weight.requires_grad, weight.resolve_neg().contiguous()
     if bias is not None:
         _check_param("bias", bias, x, channels)
-        grad, bias = grad or bias.requires_grad, bias.contiguous()
+        grad, bias = grad or bias.requires_grad, bias.resolve_neg().contiguous()
         if weight is not None and weight.dtype != bias.dtype:
             raise ValueError(f"weight and bias must be of one type, got {weight.dtype} and {bias.dtype}")
     args = (x, weight, bias, num_groups, float(eps), code, int(bool(act_first)))
@@ -261,7 +263,9 @@ def _linear_plan(M, N, K, dtype, act, ldx, ldw, ldr, ldy, unaligned):
 
 
 def _row_layout(t):
-    """`t` [..., n] with the stride of its flattened rows, at least n; a copy where there is none."""
+    """`t` [..., n] with the stride of its flattened rows, at least n; a copy where there is none (or the values have
+    a pending sign)."""
+    t = t.resolve_neg()
     n = t.shape[-1]
     if t.is_contiguous():
         return t, n
@@ -370,7 +374,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
             if t.dtype != x.dtype:
                 raise ValueError(f"{name} must be {x.dtype} like x, got {t.dtype}")
             grad = grad or t.requires_grad
-    bias = None if bias is None else bias.contiguous()
+    bias = None if bias is None else bias.resolve_neg().contiguous()
     if grad and torch.is_grad_enabled():
         return _LinearAct.apply(x, weight, bias, residual, code)
     return _linear_forward(x, weight, bias, residual, code, False)[0]

@@ -140,3 +140,28 @@ def test_more_images_than_the_descriptor_holds(ops, images):
     with pytest.raises(ValueError, match="unsupported sizes"):
         ops.group_norm_act(torch.ones(1, 1, 1).expand(images, 1, 1), 1)
     assert not ops.rec.calls
+
+
+def test_pending_signs_are_applied(ops, monkeypatch):
+    """Real views of conjugates (z.conj().imag) carry a sign that is not in memory yet."""
+    seen = []
+
+    def reader(name):
+        def call(desc, *args):
+            def first(p):
+                return C.cast(p, C.POINTER(C.c_float))[0]
+
+            # x, weight, bias (and the residual, where the linear forward has it)
+            seen.append([first(p) for p in args[:4 if "linear" in name else 3]])
+            return 0
+
+        return call
+
+    for name in ("gs_group_norm_act_fwd", "gs_linear_act_fwd"):
+        setattr(ops.rec, name, reader(name))
+    for view in (torch._neg_view, lambda t: torch.complex(torch.zeros_like(t), t).conj().imag):
+        x, p = view(torch.full((2, 5, 1), 3.0)), view(torch.full((1,), 5.0))
+        assert x.is_neg() and p.is_neg()
+        ops.group_norm_act(x, 1, p, p)
+        ops.linear_act(x, p.view(1, 1), p, residual=x)
+    assert seen == [[-3, -5, -5], [-3, -5, -5, -3]] * 2
