@@ -514,11 +514,15 @@ struct PrepJob {
     long long rows, ld;  // source row stride
     int cols, ldp;       // destination row stride
 };
+// What lies beyond bf16's largest number has that for its head.  An infinity is in the last term alone, which meets
+// only the other operand's head (0 where the value is 0, or infinite itself): in the first it would meet that operand's
+// lower terms too, zeros and either sign, and give NaN.
 __device__ __forceinline__ void split3(float x, float &h, float &m, float &l) {
-    h = __bfloat162float(__float2bfloat16_rn(x));
-    // an infinite or NaN head has no remainder
-    const float r = fabsf(h) <= 3.4028234e38f ? x - h : 0.f;
-    m = __bfloat162float(__float2bfloat16_rn(r));
+    constexpr float MOST = 3.3895313892515355e38f;  // (2 - 2^-7) 2^127
+    const bool inf = fabsf(x) > 3.4028234e38f;
+    h = inf ? 0.f : fabsf(x) > MOST ? copysignf(MOST, x) : __bfloat162float(__float2bfloat16_rn(x));
+    const float r = x - h;
+    m = inf ? 0.f : __bfloat162float(__float2bfloat16_rn(r));
     l = r - m;
 }
 __device__ __forceinline__ void store_terms(const f2 *v, __nv_bfloat16 *dst, long long term_stride) {

@@ -353,7 +353,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     x [..., K], weight [N, K] (nn.Linear's, or a 1x1 convolution's ``weight.flatten(1)``), bias [N],
     residual [..., N] of the output's shape; all of one type, float32, bfloat16 or float16.  ``act`` is
     "none", "gelu" (erf form) or "silu".  Sums are fp32 (fp32 inputs keep fp32 accuracy); the result is
-    rounded once, after the residual.  Rows may be strided (channel slices of a wider map); other strides are
+    rounded once, after the residual, and each gradient once.  Infinities come out as the formula has them but for
+    two cases that give NaN: fp32 infinities of both factors that meet, and 16-bit ones of x or weight in a gradient.  Rows may be strided (channel slices of a wider map); other strides are
     copied.  Returns a contiguous tensor [..., N]."""
     _lib.require_cuda(x, weight, bias, residual)
     _refuse_tangents(x, weight, bias, residual)

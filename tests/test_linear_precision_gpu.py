@@ -104,3 +104,26 @@ def test_dz_is_not_rounded_to_the_type(ops, act, dtype, M, K, N, dy_scale):
     inside(dx, dz @ W, h * (dz @ W).abs() + (edz + sums(N) * dz.abs()) @ W.abs() + lo, "dx")
     inside(dw, dz.t() @ X, h * (dz.t() @ X).abs() + (edz + sums(M) * dz.abs()).t() @ X.abs() + lo, "dweight")
     inside(db, dz.sum(0), h * dz.sum(0).abs() + (slope + (M / 2 + 32) * U * dz.abs()).sum(0) + lo, "dbias")
+
+
+def test_fp32_infinities_and_the_largest_numbers(ops):
+    """fp32 operands enter as bf16 terms: an infinity has the formula's result (64 bits' is the same), and numbers
+    above bf16's largest are numbers.  Sizes of a padded row, of whole rows, of split sums."""
+    for M, K, N in ((40, 33, 20), (300, 64, 72), (5, 2000, 24)):
+        x, w, dy = rand(M, K, seed=20), rand(N, K, seed=21), rand(M, N, seed=22)
+        w[3, 5], x[2, 5], dy[4, 1] = 0.0, 1.0, 0.5
+        for at in ("x", "w", "dy"):
+            a = dict(x=x.clone(), w=w.clone(), dy=dy.clone())
+            a[at][1, 7], a[at][4, 9] = float("inf"), -float("inf")
+            X, W = a["x"].requires_grad_(True), a["w"].requires_grad_(True)
+            y = ops.linear_act(X, W)
+            got = [y.detach(), *torch.autograd.grad(y, (X, W), a["dy"])]
+            Xd, Wd, D = (a[k].detach().double() for k in ("x", "w", "dy"))
+            for g, r in zip(got, (Xd @ Wd.t(), D @ Wd, D.t() @ Xd)):
+                assert torch.equal(g.isnan(), r.isnan()) and torch.equal(g.isinf(), r.isinf())
+                assert torch.equal(g[g.isinf()].double(), r[r.isinf()])
+        x[1, 7], x[2, 5] = 3.4e38, -3.402823e38
+        y = ops.linear_act(x, w * 2.0 ** -20)
+        ref = x.double() @ (w * 2.0 ** -20).double().t()
+        e = 2 * U * (K / 2 + 32) * (x.double().abs() @ (w * 2.0 ** -20).double().abs().t())
+        inside(y, ref, e + 1e-30, "largest")
