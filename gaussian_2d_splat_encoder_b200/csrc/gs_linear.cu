@@ -929,6 +929,15 @@ int check_waits(const char *where) {
     return GS_ERR_TIMEOUT;
 }
 
+// The driver encodes tensor maps only on a thread with a context.  One that has made no such call yet (a new thread's
+// first linear call, autograd's in a backward that begins with a product) gets its device's here.
+int bind_device(const char *where) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaSetDevice(dev);
+    return e == cudaSuccess ? GS_OK : cuda_error(where, cudaGetErrorString(e));
+}
+
 template <int BN, bool PAIR, bool OUT32, int EPI>
 int launch(const CUtensorMap *m, const GemmArgs &a, bool follows, cudaStream_t s) {
     using S = Shape<BN, PAIR, OUT32, EPI>;
@@ -1132,6 +1141,7 @@ extern "C" int gs_linear_act_fwd(const gs_linear_desc *d, const void *x, const v
         return GS_ERR_BAD_ARGUMENT;
     const Plan p = plan(d, false);
     if (p.bytes > 256 && (!workspace || workspace_bytes < p.bytes)) return GS_ERR_WORKSPACE;
+    if (const int st = bind_device("gs_linear_act_fwd")) return st;
     if (const int st = check_waits("gs_linear_act_fwd")) return st;
     cudaStream_t s = (cudaStream_t)stream;
     const Epilogue e{bias, residual, d->ldr, d->act, y, d->act == GS_ACT_NONE ? nullptr : slope};
@@ -1157,6 +1167,7 @@ extern "C" int gs_linear_act_bwd(const gs_linear_desc *d, const void *x, const v
         return GS_ERR_BAD_ARGUMENT;
     const Plan p = plan(d, true);
     if (p.bytes > 256 && (!workspace || workspace_bytes < p.bytes)) return GS_ERR_WORKSPACE;
+    if (const int st = bind_device("gs_linear_act_bwd")) return st;
     if (const int st = check_waits("gs_linear_act_bwd")) return st;
     if (d->act == GS_ACT_NONE) slope = nullptr;
     if (d->dtype == GS_F32) return backward<float>(d, p, x, w, slope, dy, dx, dw, dbias, workspace, s);

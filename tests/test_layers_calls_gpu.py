@@ -103,3 +103,24 @@ def test_a_wait_that_gave_up_is_reported(ops, lib):
     with pytest.raises(RuntimeError, match="gave up"):
         ops.check_linear_waits()
     ops.check_linear_waits()
+
+
+def test_a_new_threads_first_call(ops):
+    """Each call is the first of its thread that touches the device: a forward, and a backward of the product alone."""
+    import threading
+
+    x, w = rand(64, 32, seed=18, dtype=torch.bfloat16), rand(16, 32, seed=19, dtype=torch.bfloat16).requires_grad_(True)
+    z = rand(1, 64, 32, seed=24, dtype=torch.bfloat16)
+    dy = rand(64, 16, seed=23, dtype=torch.bfloat16)
+    ref = [ops.linear_act(x, w), ops.group_norm_act(z, 4)]
+    torch.cuda.synchronize()
+    calls = [lambda: ops.linear_act(x, w), lambda: ops.group_norm_act(z, 4)]
+    for call, r in zip(calls, ref):
+        got = []
+        t = threading.Thread(target=lambda: got.append(call()))
+        t.start()
+        t.join()
+        torch.cuda.synchronize()
+        assert len(got) == 1 and torch.equal(got[0], r)
+    (dw,) = torch.autograd.grad(ref[0], w, dy)
+    assert bool(dw.isfinite().all())
