@@ -16,7 +16,9 @@
 // result does); db sums the unrounded values.
 //
 // Sums over a long k with few output tiles are split along k over the SMs; the parts go to the workspace
-// in fp32 and a second kernel adds them in order (the same bits every time) and applies the epilogue.
+// in fp32 and a second kernel adds them in order (the same bits every time) and applies the epilogue.  What the
+// parts of one product take there is bounded: a forward or dx runs over panels of rows, dW over groups of parts
+// whose sum so far is kept in the first part's place.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
@@ -47,7 +49,8 @@ struct GemmArgs {
     int kb, npair;        // k-blocks of 64 per term product, term products: 1, 2 (A in two terms), 6 (fp32)
     int a_mn, b_mn;       // operand has i / j adjacent instead of k
     int f16;              // operands fp16 (else bf16)
-    int splits;           // > 1: parts of the k sum, raw fp32 to part
+    int splits;           // > 1: parts of the k sum, raw fp32
+    int first, nparts, slot;  // of them the launch's: the first, their number, the place of the first
     int tiles_i, tiles_j;
     // epilogue
     int out_f16;          // 16-bit output type
@@ -109,7 +112,7 @@ struct Pipe {  // one CTA's barriers
     __align__(16) float bias[EPI_WARPS][16];  // read as float4
 };
 
-// row tile, column tile, split of an item
+// row tile, column tile, part (counted from the launch's first) of an item
 struct Item {
     int i, j, s;
     __device__ __forceinline__ Item(const GemmArgs &a, int item) {
@@ -119,8 +122,8 @@ struct Item {
         s = item / a.tiles_i;
     }
     // its k-blocks, and how many it multiplies over all term products
-    __device__ __forceinline__ int from(const GemmArgs &a) const { return (int)((long long)a.kb * s / a.splits); }
-    __device__ __forceinline__ int to(const GemmArgs &a) const { return (int)((long long)a.kb * (s + 1) / a.splits); }
+    __device__ __forceinline__ int from(const GemmArgs &a) const { return (int)((long long)a.kb * (a.first + s) / a.splits); }
+    __device__ __forceinline__ int to(const GemmArgs &a) const { return (int)((long long)a.kb * (a.first + s + 1) / a.splits); }
     __device__ __forceinline__ int blocks(const GemmArgs &a) const { return (to(a) - from(a)) * a.npair; }
 };
 
@@ -187,7 +190,7 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ri
         const float bias[2] = {ahead[0], ahead[1]};
         load_bias(item + step);
         const Item tile(a, item);
-        const int sp = tile.s, base = tile.j * BN + part * 64;
+        const int sp = a.slot + tile.s, base = tile.j * BN + part * 64;
         const long long row0 = (long long)tile.i * S::TILE_I + rank * BM + q * 32;
 #pragma unroll 1
         for (int u = 0; u < S::UNITS && !dead; u++) {
@@ -346,7 +349,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = PAIR ? (int)cluster_rank() : 0;
     const int first = PAIR ? blockIdx.x / 2 : blockIdx.x, stride = PAIR ? gridDim.x / 2 : gridDim.x;
-    const int n_items = a.tiles_i * a.tiles_j * a.splits;
+    const int n_items = a.tiles_i * a.tiles_j * a.nparts;
 
     if (warp == 1) {
         if (PAIR) {
@@ -689,9 +692,10 @@ __global__ void __launch_bounds__(256) k_dz(const __grid_constant__ DzArgs a) {
 // ---- adds the k splits' parts in order and applies the epilogue; blocks from sum_blocks on fold the column
 // sums of dz into db
 struct JoinArgs {
-    const float *part;
+    float *part;
     long long I, ldr, part_stride;
-    int J, ldp, splits, sum_blocks, act;
+    int J, ldp, parts, sum_blocks, act;
+    int more;  // other parts follow: the sum so far goes to the first's place
     const void *bias, *residual;
     void *out;
     float *slope;
@@ -725,15 +729,19 @@ __global__ void __launch_bounds__(256) k_join(JoinArgs a) {
     for (long long t = blockIdx.x * 256LL + threadIdx.x; t < n; t += a.sum_blocks * 256LL) {
         const long long i = t / nv;
         const int c = (int)(t - i * nv) * 4;
-        const float *p = a.part + i * a.ldp + c;
+        float *p = a.part + i * a.ldp + c;
         float4 s = *reinterpret_cast<const float4 *>(p);
 #pragma unroll 8
-        for (int k = 1; k < a.splits; k++) {
+        for (int k = 1; k < a.parts; k++) {
             const float4 e = *reinterpret_cast<const float4 *>(p + k * a.part_stride);
             s.x += e.x;
             s.y += e.y;
             s.z += e.z;
             s.w += e.w;
+        }
+        if (a.more) {
+            *reinterpret_cast<float4 *>(p) = s;
+            continue;
         }
         f2 v[2] = {{s.x, s.y}, {s.z, s.w}}, sl[2];
         const int n = min(4, a.J - c);
@@ -782,10 +790,12 @@ bool valid(const gs_linear_desc *d) {
 // add up rather than round it (1.7e-6 of the result over 1536 terms, growing with their number); the join rounds.
 constexpr int FP32_CHAIN = 8;
 struct Tiling {
-    int bn, pair, tiles_i, tiles_j, splits;
+    int bn, pair, splits;
+    long long rows;  // of D a launch takes
+    int slots;       // places for parts in the workspace
 };
 Tiling tiling(long long I, int J, long long kb, int npair) {
-    Tiling best{64, 0, 0, 0, 1};
+    Tiling best{64, 0, 1, I, 1};
     double least = 0;
     const int widths[3] = {256, 128, 64};
     const double block[3] = {720, 600, 590}, epi[3] = {12000, 5500, 3700};
@@ -802,11 +812,32 @@ Tiling tiling(long long I, int J, long long kb, int npair) {
             const double cost = waves * std::max(k, epi[w]) + std::min(k, epi[w]) + join;
             if (least == 0 || cost < least) {
                 least = cost;
-                best = Tiling{bn, pair, (int)cdiv(I, ti), (int)cdiv(J, bn), (int)s};
+                best = Tiling{bn, pair, (int)s, I, (int)s};
             }
         }
     }
     return best;
+}
+
+// The parts of one product take PART_BYTES of the workspace, or what 256 rows or two parts do where that is more:
+// unbounded, 16384x4096->4096 in fp32 took 2.15 GB, and dW as many times its size as there are 512 rows.  What goes
+// over it by k-blocks alone (parts are then as many as a sum may have terms) is cut into panels of rows, which
+// multiply as fast while a panel fills the SMs, or, where `rows` is false (dW, whose k is long), into groups of parts.
+constexpr long long PART_BYTES = 256 << 20;
+Tiling bounded(long long I, int J, long long kb, int npair, bool rows) {
+    Tiling t = tiling(I, J, kb, npair);
+    const long long row = (long long)t.splits * ((J + 3) & ~3) * 4;  // bytes of one row's parts
+    if (t.splits == 1 || row * I <= PART_BYTES) return t;
+    if (rows) {
+        const long long most = std::max(256LL, PART_BYTES / row / 256 * 256);
+        if (most < I) {
+            t = tiling(most, J, kb, npair);
+            t.rows = most;
+        }
+    } else {
+        t.slots = (int)std::min<long long>(t.splits, std::max(2LL, PART_BYTES / (row / t.splits * I)));
+    }
+    return t;
 }
 
 // Workspace of a call: padded or split operands, the parts of split sums, column sums.
@@ -820,8 +851,8 @@ struct Plan {
 };
 bool ragged(long long ld, int unaligned) { return unaligned || ld % 8 != 0; }
 
-size_t parts(const Tiling &t, long long I, int J) {
-    return t.splits > 1 ? al((size_t)t.splits * I * ((J + 3) & ~3) * 4) : 0;
+size_t parts(const Tiling &t, int J) {
+    return t.splits > 1 ? al((size_t)t.slots * t.rows * ((J + 3) & ~3) * 4) : 0;
 }
 Plan plan(const gs_linear_desc *d, bool bwd) {
     Plan p;
@@ -844,15 +875,15 @@ Plan plan(const gs_linear_desc *d, bool bwd) {
     p.o_x = take(p.prep_x ? (size_t)d->M * p.ldx * 2 * p.terms : 0);
     p.o_w = take(p.prep_w ? (size_t)d->N * p.ldw * 2 * p.terms : 0);
     if (!bwd) {
-        p.fwd = tiling(d->M, d->N, cdiv(d->K, BK), f32 ? 6 : 1);
-        p.o_part = take(parts(p.fwd, d->M, d->N));
+        p.fwd = bounded(d->M, d->N, cdiv(d->K, BK), f32 ? 6 : 1, true);
+        p.o_part = take(parts(p.fwd, d->N));
     } else {
         p.need_dz = f32 || d->act != GS_ACT_NONE || ragged(d->ldy, d->unaligned & 4);
         p.dz_terms = f32 ? 3 : d->act != GS_ACT_NONE ? 2 : 1;  // (without an activation dz is dy)
         p.o_dz = take(p.need_dz ? (size_t)d->M * p.ldn * 2 * p.dz_terms : 0);
-        p.gx = tiling(d->M, d->K, cdiv(d->N, BK), f32 ? 6 : p.dz_terms);
-        p.gw = tiling(d->N, d->K, cdiv(d->M, BK), f32 ? 6 : p.dz_terms);
-        p.o_part = take(std::max(parts(p.gx, d->M, d->K), parts(p.gw, d->N, d->K)));
+        p.gx = bounded(d->M, d->K, cdiv(d->N, BK), f32 ? 6 : p.dz_terms, true);
+        p.gw = bounded(d->N, d->K, cdiv(d->M, BK), f32 ? 6 : p.dz_terms, false);
+        p.o_part = take(std::max(parts(p.gx, d->K), parts(p.gw, d->K)));
         // dz: blocks of 256 threads, up to 256 column vectors each, about four blocks per SM
         const int nv = p.ldn / 8;
         p.dz_cvec = std::min(nv, 256);
@@ -887,12 +918,13 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     }();
     return fn;
 }
-// [terms][rows][cols] elements of es bytes with row stride ld: boxes of box_cols x box_rows, swizzled
+// [terms][rows][cols] elements of es bytes with row stride ld and term stride `term`: boxes of box_cols x box_rows,
+// swizzled
 bool make_map(CUtensorMap *tm, CUtensorMapDataType type, int es, const void *base, long long cols, long long rows,
-              long long ld, int terms, int box_cols, int box_rows) {
+              long long ld, int terms, long long term, int box_cols, int box_rows) {
     // rows of operand boxes are 128 bytes, of output and residual units 64
     const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)terms};
-    const cuuint64_t str[2] = {(cuuint64_t)ld * es, (cuuint64_t)(terms > 1 ? rows : 1) * ld * es};
+    const cuuint64_t str[2] = {(cuuint64_t)ld * es, (cuuint64_t)(terms > 1 ? term : ld) * es};
     const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1}, one[3] = {1, 1, 1};
     auto fn = encode_fn();
     return fn && fn(tm, type, 3, const_cast<void *>(base), dims, str, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -944,7 +976,7 @@ int launch(const CUtensorMap *m, const GemmArgs &a, bool follows, cudaStream_t s
     auto kern = k_gemm<BN, PAIR, OUT32, EPI>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM) != cudaSuccess)
         return done("gs_linear_act");
-    const int items = a.tiles_i * a.tiles_j * a.splits;
+    const int items = a.tiles_i * a.tiles_j * a.nparts;
     gs_launch(kern, dim3(PAIR ? 2 * std::min(items, SMS / 2) : std::min(items, SMS)), GEMM_THREADS, S::SMEM, s, follows,
               PAIR ? 2 : 1, m[0], m[1], m[2], m[3], m[4], a);
     gs_count_launch(1);
@@ -973,6 +1005,7 @@ struct Operand {
     long long rows, cols, ld;
     int mn;  // the product's own axis is adjacent (else k is)
     int terms;
+    long long term;  // stride of the terms
 };
 struct Epilogue {
     const void *bias, *residual;
@@ -982,9 +1015,10 @@ struct Epilogue {
     float *slope;
 };
 
-// D [I][J] over k = K; with splits the parts go to `part` and the caller joins them
-int product(const gs_linear_desc *d, const Plan &p, const Tiling &t, long long I, int J, long long K, const Operand &A,
-            const Operand &B, const Epilogue &e, void *part, bool follows, cudaStream_t s) {
+// Parts first.. of D [I][J] over k = K, one after the other from place `slot` of `part` on for the caller to join; a
+// product of one part is finished
+int product(const gs_linear_desc *d, const Tiling &t, long long I, int J, long long K, const Operand &A, const Operand &B,
+            const Epilogue &e, void *part, int first, int nparts, int slot, bool follows, cudaStream_t s) {
     GemmArgs a;
     memset(&a, 0, sizeof(a));
     const bool f32 = d->dtype == GS_F32, raw = t.splits > 1, out32 = f32 || raw;
@@ -994,16 +1028,19 @@ int product(const gs_linear_desc *d, const Plan &p, const Tiling &t, long long I
     a.a_mn = A.mn; a.b_mn = B.mn;
     a.f16 = d->dtype == GS_F16;
     a.out_f16 = a.f16;
-    a.splits = t.splits; a.tiles_i = t.tiles_i; a.tiles_j = t.tiles_j;
+    a.splits = t.splits; a.first = first; a.nparts = nparts; a.slot = slot;
+    a.tiles_i = (int)cdiv(I, t.pair ? 256 : 128);
+    a.tiles_j = (int)cdiv(J, t.bn);
     a.wait_error = wait_error();
     CUtensorMap m[5];
     const CUtensorMapDataType in = a.f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    bool ok = make_map(&m[0], in, 2, A.p, A.cols, A.rows, A.ld, A.terms, 64, A.mn ? BK : BM) &&
-              make_map(&m[1], in, 2, B.p, B.cols, B.rows, B.ld, B.terms, 64, B.mn ? BK : t.pair ? t.bn / 2 : t.bn);
+    bool ok = make_map(&m[0], in, 2, A.p, A.cols, A.rows, A.ld, A.terms, A.term, 64, A.mn ? BK : BM) &&
+              make_map(&m[1], in, 2, B.p, B.cols, B.rows, B.ld, B.terms, B.term, 64, B.mn ? BK : t.pair ? t.bn / 2 : t.bn);
     m[2] = m[3] = m[4] = m[0];
     if (raw) {
         a.out_tma = 1;
-        ok = ok && make_map(&m[2], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, part, J, I, (J + 3) & ~3, t.splits, 16, 32);
+        const long long ldp = (J + 3) & ~3;
+        ok = ok && make_map(&m[2], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, part, J, I, ldp, slot + nparts, I * ldp, 16, 32);
     } else {
         const int es = f32 ? 4 : 2, ec = f32 ? 16 : 32;
         const CUtensorMapDataType ty = f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
@@ -1011,9 +1048,9 @@ int product(const gs_linear_desc *d, const Plan &p, const Tiling &t, long long I
         const auto whole = [&](const void *q, long long ld) { return ((uintptr_t)q & 15) == 0 && ld * es % 16 == 0; };
         a.out_tma = whole(e.out, J) && ((uintptr_t)e.slope & 15) == 0;  // (rows of slopes are as long or longer)
         a.res_tma = e.residual && whole(e.residual, e.ldr);
-        if (a.out_tma) ok = ok && make_map(&m[2], ty, es, e.out, J, I, J, 1, ec, 32);
-        if (a.out_tma && e.slope) ok = ok && make_map(&m[3], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, e.slope, J, I, J, 1, 16, 32);
-        if (a.res_tma) ok = ok && make_map(&m[4], ty, es, e.residual, J, I, e.ldr, 1, ec, 32);
+        if (a.out_tma) ok = ok && make_map(&m[2], ty, es, e.out, J, I, J, 1, 0, ec, 32);
+        if (a.out_tma && e.slope) ok = ok && make_map(&m[3], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, e.slope, J, I, J, 1, 0, 16, 32);
+        if (a.res_tma) ok = ok && make_map(&m[4], ty, es, e.residual, J, I, e.ldr, 1, 0, ec, 32);
     }
     if (!ok) return cuda_error("gs_linear_act", "cuTensorMapEncodeTiled refused a tensor");
     const int epi = raw || e.act == GS_ACT_NONE ? EPI_NONE : e.act == GS_ACT_GELU ? (e.slope ? EPI_GELU_SLOPE : EPI_GELU)
@@ -1021,22 +1058,58 @@ int product(const gs_linear_desc *d, const Plan &p, const Tiling &t, long long I
     return out32 ? launch_epi<true>(epi, t.bn, m, a, follows, s) : launch_epi<false>(epi, t.bn, m, a, follows, s);
 }
 
+// db from the column sums of dz
+struct Fold {
+    const float *colsum;
+    int ncol, nsum;
+    void *db;  // NULL: nothing
+};
+// Adds `parts` parts of D [I][J] (0: none), to the sum so far or to the epilogue, and folds db beside it.
 template <typename T>
-void join(const Tiling *t, long long I, int J, const Epilogue &e, const void *part, const float *colsum, int ncol, int nsum,
-          void *db, cudaStream_t s) {
+void join(long long I, int J, int parts, bool more, const Epilogue &e, void *part, const Fold &f, cudaStream_t s) {
     JoinArgs a;
     memset(&a, 0, sizeof(a));
-    if (t) {
-        a.part = reinterpret_cast<const float *>(part);
-        a.I = I; a.J = J; a.ldp = (J + 3) & ~3; a.part_stride = I * a.ldp; a.splits = t->splits;
+    if (parts) {
+        a.part = reinterpret_cast<float *>(part);
+        a.I = I; a.J = J; a.ldp = (J + 3) & ~3; a.part_stride = I * a.ldp; a.parts = parts; a.more = more;
         a.sum_blocks = (int)std::min<long long>(cdiv(I * (a.ldp / 4), 256), 8 * SMS);
         a.bias = e.bias; a.residual = e.residual; a.ldr = e.ldr; a.act = e.act; a.out = e.out; a.slope = e.slope;
     }
-    a.colsum = colsum; a.ncol = ncol; a.nsum = nsum; a.db = db;
-    const int fold = db ? (int)cdiv(ncol, 32) : 0;
+    a.colsum = f.colsum; a.ncol = f.ncol; a.nsum = f.nsum; a.db = f.db;
+    const int fold = f.db ? (int)cdiv(f.ncol, 32) : 0;
     if (a.sum_blocks + fold == 0) return;
     gs_launch(k_join<T>, dim3((unsigned)(a.sum_blocks + fold)), 256, 0, s, true, 1, a);  // (a product or dz came before)
     gs_count_launch(1);
+}
+// D [I][J] over k = K, panel by panel and group by group, each joined; db is folded by the last join
+template <typename T>
+int whole_product(const gs_linear_desc *d, const Tiling &t, long long I, int J, long long K, const Operand &A,
+                  const Operand &B, const Epilogue &e, void *part, const Fold &f, bool follows, cudaStream_t s) {
+    const size_t es = sizeof(T);
+    auto at = [](auto *p, long long bytes) {
+        using P = decltype(p);
+        return p ? (P)((const char *)p + bytes) : p;
+    };
+    for (long long r = 0; r < I; r += t.rows) {
+        const long long rows = std::min(t.rows, I - r);
+        Operand a = A;
+        if (t.rows < I) {  // (A is then read along k: its rows are D's)
+            a.p = at(A.p, r * A.ld * 2);
+            a.rows = rows;
+        }
+        const Epilogue ep{e.bias, at(e.residual, r * e.ldr * (long long)es), e.ldr, e.act, at(e.out, r * J * (long long)es),
+                          at(e.slope, r * J * 4)};
+        for (int first = 0; first < t.splits;) {
+            const int slot = first ? 1 : 0, n = std::min(t.slots - slot, t.splits - first);
+            if (const int st = product(d, t, rows, J, K, a, B, ep, part, first, n, slot, follows, s)) return st;
+            follows = true;
+            first += n;
+            const bool more = first < t.splits, last = !more && r + rows == I;
+            if (t.splits > 1) join<T>(rows, J, slot + n, more, ep, part, last ? f : Fold{}, s);
+        }
+    }
+    if (t.splits == 1) join<T>(0, 0, 0, false, e, nullptr, f, s);
+    return GS_OK;
 }
 
 char *base_of(void *ws) { return reinterpret_cast<char *>(al((uintptr_t)ws)); }
@@ -1046,8 +1119,8 @@ PrepJobs operands(const gs_linear_desc *d, const Plan &p, const void *x, const v
                   Operand &X, Operand &W) {
     PrepJobs jobs;
     memset(&jobs, 0, sizeof(jobs));
-    X = Operand{x, d->M, d->K, d->ldx, 0, p.terms};
-    W = Operand{w, d->N, d->K, d->ldw, 0, p.terms};
+    X = Operand{x, d->M, d->K, d->ldx, 0, p.terms, d->M * p.ldx};
+    W = Operand{w, d->N, d->K, d->ldw, 0, p.terms, (long long)d->N * p.ldw};
     if (want_x && p.prep_x) {
         jobs.job[jobs.n++] = PrepJob{x, ws + p.o_x, d->M, d->ldx, d->K, p.ldx};
         X.p = ws + p.o_x;
@@ -1074,10 +1147,8 @@ int forward(const gs_linear_desc *d, const Plan &p, const void *x, const void *w
         k_prep_operands<T><<<dim3((unsigned)jobs.blocks, (unsigned)jobs.n), 256, 0, s>>>(jobs);
         gs_count_launch(1);
     }
-    const int st = product(d, p, p.fwd, d->M, d->N, d->K, X, W, e, ws + p.o_part, jobs.n > 0, s);
-    if (st != GS_OK) return st;
-    if (p.fwd.splits > 1) join<T>(&p.fwd, d->M, d->N, e, ws + p.o_part, nullptr, 0, 0, nullptr, s);
-    return done("gs_linear_act_fwd");
+    const int st = whole_product<T>(d, p.fwd, d->M, d->N, d->K, X, W, e, ws + p.o_part, Fold{}, jobs.n > 0, s);
+    return st != GS_OK ? st : done("gs_linear_act_fwd");
 }
 
 template <typename T>
@@ -1086,7 +1157,7 @@ int backward(const gs_linear_desc *d, const Plan &p, const void *x, const void *
     char *ws = base_of(workspace);
     Operand X, W;
     const PrepJobs jobs = operands(d, p, x, w, ws, dw != nullptr, dx != nullptr, X, W);
-    Operand Z{dy, d->M, d->N, d->ldy, 0, p.dz_terms};
+    Operand Z{dy, d->M, d->N, d->ldy, 0, p.dz_terms, d->M * p.ldn};
     const bool make_dz = p.need_dz && (dx || dw);
     float *colsum = db ? reinterpret_cast<float *>(ws + p.o_col) : nullptr;
     if (make_dz) {
@@ -1105,23 +1176,20 @@ int backward(const gs_linear_desc *d, const Plan &p, const void *x, const void *
         gs_count_launch(1);
     }
     const bool first = rows || jobs.n;  // a launch of this call came before the products
-    int st = GS_OK;
+    const Fold fold{colsum, d->N, p.dz_rows, db};
     if (dx) {
         Operand B = W;
         B.mn = 1;
         const Epilogue e{nullptr, nullptr, 0, 0, dx, nullptr};
-        st = product(d, p, p.gx, d->M, d->K, d->N, Z, B, e, ws + p.o_part, first, s);
-        if (st != GS_OK) return st;
-        if (p.gx.splits > 1) join<T>(&p.gx, d->M, d->K, e, ws + p.o_part, nullptr, 0, 0, nullptr, s);
+        if (const int st = whole_product<T>(d, p.gx, d->M, d->K, d->N, Z, B, e, ws + p.o_part, dw ? Fold{} : fold, first, s)) return st;
     }
-    const Epilogue e{nullptr, nullptr, 0, 0, dw, nullptr};
     if (dw) {
         Operand A = Z, B = X;
         A.mn = B.mn = 1;
-        st = product(d, p, p.gw, d->N, d->K, d->M, A, B, e, ws + p.o_part, first || dx, s);
-        if (st != GS_OK) return st;
+        const Epilogue e{nullptr, nullptr, 0, 0, dw, nullptr};
+        if (const int st = whole_product<T>(d, p.gw, d->N, d->K, d->M, A, B, e, ws + p.o_part, fold, first || dx, s)) return st;
     }
-    join<T>(dw && p.gw.splits > 1 ? &p.gw : nullptr, d->N, d->K, e, ws + p.o_part, colsum, d->N, p.dz_rows, db, s);
+    if (!dx && !dw) join<T>(0, 0, 0, false, Epilogue{}, nullptr, fold, s);
     return done("gs_linear_act_bwd");
 }
 

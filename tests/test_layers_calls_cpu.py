@@ -165,3 +165,21 @@ def test_pending_signs_are_applied(ops, monkeypatch):
         ops.group_norm_act(x, 1, p, p)
         ops.linear_act(x, p.view(1, 1), p, residual=x)
     assert seen == [[-3, -5, -5], [-3, -5, -5, -3]] * 2
+
+
+def test_linear_workspace_is_bounded(lib, ops):
+    """fp32 sums of many parts: beside the operands' terms (6 bytes an element) the workspace holds at most 256 MiB of
+    parts, or 256 rows' or two of them, and the column sums; it does not grow with M N K."""
+    size, up8 = lib.gs_linear_act_workspace_size, lambda n: (n + 7) // 8 * 8
+    for M, K, N in ((16384, 4096, 4096), (589824, 1024, 1024), (65536, 4096, 4096), (4 << 20, 512, 300), (1 << 20, 2048, 130),
+                    (300, 1 << 17, 4096), (5, 4096, 1 << 17)):
+        d = ops._LinearDesc(M=M, N=N, K=K, dtype=0, act=1, ldx=K, ldw=K, ldr=N, ldy=N)
+        terms = [6 * M * up8(K), 6 * N * up8(K), 6 * M * up8(N)]
+
+        def most(rows, cols, k):  # of a product [rows][cols] over k
+            part = up8(cols) * 4
+            return max(256 << 20, 256 * part * (k // 512 + 1), 2 * rows * part if rows == N else 0)
+
+        fwd = terms[0] + terms[1] + most(M, N, K)
+        bwd = sum(terms) + max(most(M, K, N), most(N, K, 1)) + 600 * N * 4
+        assert 0 < size(C.byref(d), 0) <= fwd + 4096 and 0 < size(C.byref(d), 1) <= bwd + 4096, (M, K, N)

@@ -127,3 +127,27 @@ def test_fp32_infinities_and_the_largest_numbers(ops):
         ref = x.double() @ (w * 2.0 ** -20).double().t()
         e = 2 * U * (K / 2 + 32) * (x.double().abs() @ (w * 2.0 ** -20).double().abs().t())
         inside(y, ref, e + 1e-30, "largest")
+
+
+@pytest.mark.parametrize("M,K,N", [(8300, 1024, 4096), (8300, 1022, 4099)])
+def test_fp32_parts_in_panels_and_groups(ops, M, K, N):
+    """More parts than the workspace holds at once in each of the three products (17 of 16 MB for dweight): a forward
+    and dx over panels of rows, the last of them short, dweight over groups of parts."""
+    from layers_util import check_linear
+
+    x, w, b = rand(M, K, seed=30), rand(N, K, seed=31, scale=K ** -0.5), rand(N, seed=32)
+    r, dy = rand(M, N, seed=33), rand(M, N, seed=34)
+    ts = [t.clone().requires_grad_(True) for t in (x, w, b, r)]
+    y = ops.linear_act(ts[0], ts[1], ts[2], act="silu", residual=ts[3])
+    grads = torch.autograd.grad(y, ts, dy)
+    check_linear(y.detach(), grads, x, w, b, r, "silu", dy)
+    ds = [t.double().requires_grad_(True) for t in (x, w, b)]
+    Y = ACTS["silu"](ds[0] @ ds[1].t() + ds[2]) + r.double()
+    for name, a, e in zip(("y", "dx", "dw", "db"), (y.detach(), *grads), (Y.detach(), *torch.autograd.grad(Y, ds, dy.double()))):
+        rel = float((a.double() - e).norm() / e.norm())
+        assert rel <= 2e-6, (name, rel)
+    # parameters one by one: dbias folds beside whichever product is last
+    for live in ((0, 2), (1, 2), (2,)):
+        y = ops.linear_act(*[t if i in live else t.detach() for i, t in enumerate(ts[:3])], act="silu", residual=r)
+        got = torch.autograd.grad(y, [ts[i] for i in live], dy)
+        assert all(torch.equal(g, grads[i]) for g, i in zip(got, live))
