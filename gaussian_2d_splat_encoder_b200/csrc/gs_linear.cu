@@ -786,9 +786,11 @@ bool valid(const gs_linear_desc *d) {
 // least, in SM cycles as measured: a k-block 720, 600 and 590 (16384x4096->4096: 387, 569, 1099 us), a tile's
 // epilogue with GELU 12000, 5500 and 3700 (36864x128->512: 25.6, 23.3, 31.5 us), the shorter of the two
 // exposed once.  k splits while SMs are left over and a part keeps at least four k-blocks; their join costs a
-// launch, 5 us of the host's time, and the parts' bytes.  In fp32 a part has at most FP32_CHAIN k-blocks: the accumulators cut what they
-// add up rather than round it (1.7e-6 of the result over 1536 terms, growing with their number); the join rounds.
-constexpr int FP32_CHAIN = 8;
+// launch, 5 us of the host's time, and the parts' bytes.  A part has at
+// most so many k-blocks as its type allows, because the accumulators cut what they add up rather than round it: by 1.7e-6
+// of the result over 1536 terms, 7e-4 over 131072 of one sign, 6e-3 over 2^20; the join rounds.  512 terms in fp32
+// (six products each), in 16-bit types 16384 (9e-5, where the result's rounding is up to 5e-4 in fp16).
+constexpr int FP32_CHAIN = 8, CHAIN = 256;
 struct Tiling {
     int bn, pair, splits;
     long long rows;  // of D a launch takes
@@ -803,8 +805,8 @@ Tiling tiling(long long I, int J, long long kb, int npair) {
         const int bn = widths[w], pair = bn == 256, ti = pair ? 256 : 128, units = pair ? SMS / 2 : SMS;
         if (bn > 64 && J <= bn / 2) continue;
         const long long tiles = cdiv(I, ti) * cdiv(J, bn);
-        // unsplit (in fp32 as few parts as the chain allows), or one part for every idle SM
-        const long long few = npair == 6 ? cdiv(kb, FP32_CHAIN) : 1;
+        // as few parts as the chain allows, or one part for every idle SM
+        const long long few = cdiv(kb, npair == 6 ? FP32_CHAIN : CHAIN);
         const long long many = tiles < units ? std::min({units / tiles, kb * npair / 4, kb}) : 1;
         for (long long s : {few, std::max(few, many)}) {
             const double waves = (double)cdiv(tiles * s, units), k = (double)cdiv(kb, s) * npair * block[w];

@@ -151,3 +151,30 @@ def test_fp32_parts_in_panels_and_groups(ops, M, K, N):
         y = ops.linear_act(*[t if i in live else t.detach() for i, t in enumerate(ts[:3])], act="silu", residual=r)
         got = torch.autograd.grad(y, [ts[i] for i in live], dy)
         assert all(torch.equal(g, grads[i]) for g, i in zip(got, live))
+
+
+def test_long_sums_of_one_sign(ops):
+    """Sums of 2^18 positive terms with no tile to spare for splitting: an accumulator that cuts (2 u a step of 16
+    terms) may run over 16384 terms, 1024 steps, so a result is within h + 2048 u + 64 u of itself; one run over them
+    all loses 1.4e-3, three times fp16's h."""
+    dtype, L = torch.float16, 1 << 18
+    for M, K, N in ((L, 2048, 2048), (1024, L, 2304), (1024, 200, L // 2)):
+        x = rand(M, K, seed=40).abs().add_(0.5).to(dtype)
+        if K == L:  # forward
+            w = (rand(N, K, seed=41).abs_() + 0.5).mul_(1.0 / K).to(dtype)
+            y, ref = ops.linear_act(x, w), torch.zeros(M, N, dtype=torch.float64, device="cuda")
+            for i in range(0, K, 1 << 15):
+                ref += x[:, i:i + (1 << 15)].double() @ w[:, i:i + (1 << 15)].double().t()
+        else:  # dweight over the rows, dx over the outputs
+            w = torch.full((N, K), 2.0 ** -10, dtype=dtype, device="cuda").requires_grad_(True)
+            dy = (rand(M, N, seed=42).abs_() + 0.5).mul_(2.0 ** -10).to(dtype)
+            leaf = w if M == L else x.requires_grad_(True)
+            (y,) = torch.autograd.grad(ops.linear_act(x, w), leaf, dy)
+            if M == L:
+                ref = torch.zeros(N, K, dtype=torch.float64, device="cuda")
+                for i in range(0, M, 1 << 15):
+                    ref += dy[i:i + (1 << 15)].double().t() @ x.detach()[i:i + (1 << 15)].double()
+            else:
+                ref = dy.double() @ w.detach().double()
+        inside(y, ref, (half(dtype) + 2112 * U) * ref, (M, K, N))
+        del x, w, y, ref
