@@ -65,6 +65,7 @@ SIGNATURES = {
     "gs_group_norm_act_fwd": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
     "gs_group_norm_act_bwd": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
     "gs_linear_act_workspace_size": (C.c_size_t, [_P, C.c_int]),
+    "gs_linear_act_debug_tiles": (C.c_int, [_P, C.c_int, _P]),
     "gs_linear_act_fwd": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
     "gs_linear_act_bwd": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
     "gs_linear_error_flag": (C.c_int, [_P]),

@@ -1201,6 +1201,14 @@ extern "C" size_t gs_linear_act_workspace_size(const gs_linear_desc *d, int back
     return valid(d) ? plan(d, backward != 0).bytes : 0;
 }
 
+extern "C" int gs_linear_act_debug_tiles(const gs_linear_desc *d, int product, int64_t *out) {
+    if (!valid(d) || d->M == 0 || product < 0 || product > 2 || !out) return GS_ERR_BAD_ARGUMENT;
+    const Plan p = plan(d, product > 0);
+    const Tiling &t = product == 0 ? p.fwd : product == 1 ? p.gx : p.gw;
+    out[0] = t.bn; out[1] = t.splits; out[2] = t.rows; out[3] = t.slots;
+    return GS_OK;
+}
+
 extern "C" int gs_linear_act_fwd(const gs_linear_desc *d, const void *x, const void *w, const void *bias,
                                  const void *residual, void *y, float *slope, void *workspace, size_t workspace_bytes,
                                  void *stream) {

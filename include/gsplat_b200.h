@@ -299,6 +299,9 @@ typedef struct {
 /* Workspace bytes of a forward (backward = 0) or a backward (1) call; 0 for an invalid descriptor, 256 where the
  * call needs none (workspace may then be NULL). */
 size_t gs_linear_act_workspace_size(const gs_linear_desc *d, int backward);
+/* The tiles a product takes (0 the forward's, 1 dx, 2 dweight): out[0] the tile's columns (256: a pair of CTAs on 256
+ * rows, else one on 128), out[1] the parts of its sums, out[2] the rows of a panel, out[3] the places for parts. */
+int gs_linear_act_debug_tiles(const gs_linear_desc *d, int product, int64_t *out);
 /* bias, residual and slope may be NULL; slope [M][N] receives the activation's slope for the backward; not
  * written without an activation. */
 int gs_linear_act_fwd(const gs_linear_desc *d, const void *x, const void *w, const void *bias, const void *residual,

@@ -183,3 +183,17 @@ def test_linear_workspace_is_bounded(lib, ops):
         fwd = terms[0] + terms[1] + most(M, N, K)
         bwd = sum(terms) + max(most(M, K, N), most(N, K, 1)) + 600 * N * 4
         assert 0 < size(C.byref(d), 0) <= fwd + 4096 and 0 < size(C.byref(d), 1) <= bwd + 4096, (M, K, N)
+
+
+def test_linear_sizes_take_the_tiles_they_test(lib, ops):
+    """The GPU tests of these sizes cover pairs and single CTAs, whole and split sums only while the sizes take them."""
+    from linear_tiles import SIZES
+
+    out = (C.c_int64 * 4)()
+    for (M, K, N), want in SIZES.items():
+        for dtype in (1, 2):
+            d = ops._LinearDesc(M=M, N=N, K=K, dtype=dtype, act=1, ldx=K, ldw=K, ldr=N, ldy=N)
+            for product, w in enumerate(want):
+                assert lib.gs_linear_act_debug_tiles(C.byref(d), product, out) == 0
+                assert (out[0], out[1] > 1) == w, ((M, K, N), product, list(out))
+    assert lib.gs_linear_act_debug_tiles(C.byref(d), 3, out) == 2 and lib.gs_linear_act_debug_tiles(C.byref(d), 0, None) == 2
