@@ -335,7 +335,9 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ri
     __syncwarp();
 }
 
-template <int BN, bool PAIR, bool OUT32, int EPI>
+// LO: fp16's dz in two terms, the first scaled (a kernel of its own: the test for it in every k-block cost 5 % of
+// 16384x4096->4096, 382 us without and 404 with)
+template <int BN, bool PAIR, bool OUT32, int EPI, bool LO>
 __global__ void __launch_bounds__(GEMM_THREADS, 1)
     k_gemm(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
            const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmS,
@@ -448,7 +450,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
             int it = 0, tc = 0, st = 0, parity = 0;
             for (int item = first; item < n_items && !p.abort_flag; item += stride, tc++) {
                 int left = Item(a, item).blocks(a);
-                const int hi = a.npair == 2 && a.f16 ? left / 2 : -1;  // k-blocks left when hi follows lo
+                const int hi = left / 2;  // LO: k-blocks left when hi follows lo
                 const int buf = tc % S::NBUF;
                 if (tc >= S::NBUF && !mbar_wait_or_abort(&p.tempty[buf], (tc / S::NBUF - 1) & 1, &p.abort_flag,
                                                          a.wait_error, 2))
@@ -466,7 +468,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
                     uint64_t ad = descA + (uint32_t)st * (S::STAGE >> 4), bd = descB + (uint32_t)st * (S::STAGE >> 4);
 #pragma unroll
                     for (int q = 0; q < BK / 16; q++) {
-                        if (q == 0 && left == hi) mma_scaled<PAIR ? 2 : 1, LO_BITS>(dcol, ad, bd, idesc);
+                        if (LO && q == 0 && left == hi) mma_scaled<PAIR ? 2 : 1, LO_BITS>(dcol, ad, bd, idesc);
                         else if (PAIR) mma_pair(dcol, ad, bd, idesc, more);
                         else mma_bf16(dcol, ad, bd, idesc, more);
                         more = 1;
@@ -517,21 +519,34 @@ struct PrepJob {
     long long rows, ld;  // source row stride
     int cols, ldp;       // destination row stride
 };
-// What lies beyond bf16's largest number has that for its head.  An infinity is in the last term alone, which meets
-// only the other operand's head (0 where the value is 0, or infinite itself): in the first it would meet that operand's
-// lower terms too, zeros and either sign, and give NaN.
 __device__ __forceinline__ void split3(float x, float &h, float &m, float &l) {
+    h = __bfloat162float(__float2bfloat16_rn(x));
+    const float r = x - h;
+    m = __bfloat162float(__float2bfloat16_rn(r));
+    l = r - m;
+}
+// The same where a head would be infinite.  What lies beyond bf16's largest number has that for its head.  An infinity
+// is in the last term alone, which meets only the other operand's head (0 where the value is 0, or infinite itself):
+// in the first it would meet that operand's lower terms too, zeros and either sign, and give NaN.
+__device__ __forceinline__ void split3_large(float x, float &h, float &m, float &l) {
     constexpr float MOST = 3.3895313892515355e38f;  // (2 - 2^-7) 2^127
     const bool inf = fabsf(x) > 3.4028234e38f;
     h = inf ? 0.f : fabsf(x) > MOST ? copysignf(MOST, x) : __bfloat162float(__float2bfloat16_rn(x));
-    const float r = x - h;
-    m = inf ? 0.f : __bfloat162float(__float2bfloat16_rn(r));
-    l = r - m;
+    m = inf ? 0.f : __bfloat162float(__float2bfloat16_rn(x - h));
+    l = x - h - m;
 }
 __device__ __forceinline__ void store_terms(const f2 *v, __nv_bfloat16 *dst, long long term_stride) {
     f2 h[4], m[4], l[4];
+    float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; i++) split3(at(v, i), at(h, i), at(m, i), at(l, i));
+    for (int i = 0; i < 8; i++) {
+        split3(at(v, i), at(h, i), at(m, i), at(l, i));
+        most = fmaxf(most, fabsf(at(h, i)));
+    }
+    if (most > 3.4028234e38f) {  // (one test for the vector: it is not the common case)
+#pragma unroll
+        for (int i = 0; i < 8; i++) split3_large(at(v, i), at(h, i), at(m, i), at(l, i));
+    }
     *reinterpret_cast<uint4 *>(dst) = pack16<__nv_bfloat16>(h);
     *reinterpret_cast<uint4 *>(dst + term_stride) = pack16<__nv_bfloat16>(m);
     *reinterpret_cast<uint4 *>(dst + 2 * term_stride) = pack16<__nv_bfloat16>(l);
@@ -972,10 +987,10 @@ int bind_device(const char *where) {
     return e == cudaSuccess ? GS_OK : cuda_error(where, cudaGetErrorString(e));
 }
 
-template <int BN, bool PAIR, bool OUT32, int EPI>
+template <int BN, bool PAIR, bool OUT32, int EPI, bool LO>
 int launch(const CUtensorMap *m, const GemmArgs &a, bool follows, cudaStream_t s) {
     using S = Shape<BN, PAIR, OUT32, EPI>;
-    auto kern = k_gemm<BN, PAIR, OUT32, EPI>;
+    auto kern = k_gemm<BN, PAIR, OUT32, EPI, LO>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM) != cudaSuccess)
         return done("gs_linear_act");
     const int items = a.tiles_i * a.tiles_j * a.nparts;
@@ -984,16 +999,18 @@ int launch(const CUtensorMap *m, const GemmArgs &a, bool follows, cudaStream_t s
     gs_count_launch(1);
     return GS_OK;
 }
-template <bool OUT32, int EPI>
+template <bool OUT32, int EPI, bool LO = false>
 int launch_tile(int bn, const CUtensorMap *m, const GemmArgs &a, bool follows, cudaStream_t s) {
-    return bn == 256   ? launch<256, true, OUT32, EPI>(m, a, follows, s)
-           : bn == 128 ? launch<128, false, OUT32, EPI>(m, a, follows, s)
-                       : launch<64, false, OUT32, EPI>(m, a, follows, s);
+    return bn == 256   ? launch<256, true, OUT32, EPI, LO>(m, a, follows, s)
+           : bn == 128 ? launch<128, false, OUT32, EPI, LO>(m, a, follows, s)
+                       : launch<64, false, OUT32, EPI, LO>(m, a, follows, s);
 }
 template <bool OUT32>
 int launch_epi(int epi, int bn, const CUtensorMap *m, const GemmArgs &a, bool follows, cudaStream_t s) {
     switch (epi) {
-        case EPI_NONE: return launch_tile<OUT32, EPI_NONE>(bn, m, a, follows, s);
+        case EPI_NONE:
+            return a.f16 && a.npair == 2 ? launch_tile<OUT32, EPI_NONE, true>(bn, m, a, follows, s)
+                                         : launch_tile<OUT32, EPI_NONE>(bn, m, a, follows, s);
         case EPI_GELU: return launch_tile<OUT32, EPI_GELU>(bn, m, a, follows, s);
         case EPI_SILU: return launch_tile<OUT32, EPI_SILU>(bn, m, a, follows, s);
         case EPI_GELU_SLOPE: return launch_tile<OUT32, EPI_GELU_SLOPE>(bn, m, a, follows, s);
