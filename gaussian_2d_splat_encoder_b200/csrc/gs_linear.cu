@@ -797,36 +797,42 @@ bool valid(const gs_linear_desc *d) {
            d->ldy <= GS_LINEAR_MAX_LD && d->M * std::max(d->N, d->K) <= 1LL << 40;
 }
 
-// The tile of one product: pairs on 256 x 256, single CTAs on 128 x 128 or 128 x 64, whichever its waves cost
-// least, in SM cycles as measured: a k-block 720, 600 and 590 (16384x4096->4096: 387, 569, 1099 us), a tile's
-// epilogue with GELU 12000, 5500 and 3700 (36864x128->512: 25.6, 23.3, 31.5 us), the shorter of the two
-// exposed once.  k splits while SMs are left over and a part keeps at least four k-blocks; their join costs a
-// launch, 5 us of the host's time, and the parts' bytes.  A part has at
-// most so many k-blocks as its type allows, because the accumulators cut what they add up rather than round it: by 1.7e-6
-// of the result over 1536 terms, 7e-4 over 131072 of one sign, 6e-3 over 2^20; the join rounds.  512 terms in fp32
-// (six products each), in 16-bit types 16384 (9e-5, where the result's rounding is up to 5e-4 in fp16).
+// The tile of one product: pairs on 256 x 256, single CTAs on 128 x 128 or 128 x 64, whichever costs least, in SM
+// cycles as measured: a k-block 720, 600 and 590 (16384x4096->4096: 387, 569, 1099 us); a tile's epilogue 7100, 2500
+// and 1650 without an activation (36864x256->1024: 35.5, 43.3, 74.7 us), 9900, 3000 and 2050 with one (48.2, 50.6,
+// 81.9 us; 36864x128->512: 25.6, 23.3, 31.5).  A pair's epilogue runs under the next tile's k-blocks; a single
+// CTA's warps come back to the same accumulator, so theirs adds to them.  k splits while SMs are left over and a part keeps
+// at least four k-blocks: their join costs a launch, 5 us of the host's time, and the parts' bytes or, where the
+// output is small, a thread's walk over them (dweight of 100000x64->64: 31.8 us in 148 parts, 22.9 in 74, 26.3 in
+// 37).  Over 12 sizes, their
+// three products, bf16 and fp32, the choice takes at most 1.1 times the best's time but for eight of the smallest (18
+// to 38 us): 1.1 to 1.36.
+//
+// A part has at most so many k-blocks as its type allows, because the accumulators cut what they add up rather than
+// round it: by 1.7e-6 of the result over 1536 terms, 7e-4 over 131072 of one sign, 6e-3 over 2^20; the join rounds.
+// 512 terms in fp32 (six products each), in 16-bit types 16384 (9e-5, where fp16's rounding is up to 5e-4).
 constexpr int FP32_CHAIN = 8, CHAIN = 256;
 struct Tiling {
     int bn, pair, splits;
     long long rows;  // of D a launch takes
     int slots;       // places for parts in the workspace
 };
-Tiling tiling(long long I, int J, long long kb, int npair) {
+Tiling tiling(long long I, int J, long long kb, int npair, bool act) {
     Tiling best{64, 0, 1, I, 1};
     double least = 0;
     const int widths[3] = {256, 128, 64};
-    const double block[3] = {720, 600, 590}, epi[3] = {12000, 5500, 3700};
+    const double block[3] = {720, 600, 590}, epi[3] = {act ? 9900. : 7100., act ? 3000. : 2500., act ? 2050. : 1650.};
     for (int w = 0; w < 3; w++) {
         const int bn = widths[w], pair = bn == 256, ti = pair ? 256 : 128, units = pair ? SMS / 2 : SMS;
         if (bn > 64 && J <= bn / 2) continue;
         const long long tiles = cdiv(I, ti) * cdiv(J, bn);
-        // as few parts as the chain allows, or one part for every idle SM
+        // as few parts as the chain allows, or one for every second or every idle SM
         const long long few = cdiv(kb, npair == 6 ? FP32_CHAIN : CHAIN);
         const long long many = tiles < units ? std::min({units / tiles, kb * npair / 4, kb}) : 1;
-        for (long long s : {few, std::max(few, many)}) {
+        for (long long s : {few, std::max(few, many / 2), std::max(few, many)}) {
             const double waves = (double)cdiv(tiles * s, units), k = (double)cdiv(kb, s) * npair * block[w];
-            const double join = s > 1 ? 9000 + (double)s * I * J * 8 / 3000 : 0;
-            const double cost = waves * std::max(k, epi[w]) + std::min(k, epi[w]) + join;
+            const double join = s > 1 ? 9000 + s * std::max((double)I * J * 8 / 3000, 100.) : 0;
+            const double cost = (pair ? waves * std::max(k, epi[w]) + std::min(k, epi[w]) : waves * (k + epi[w])) + join;
             if (least == 0 || cost < least) {
                 least = cost;
                 best = Tiling{bn, pair, (int)s, I, (int)s};
@@ -841,14 +847,14 @@ Tiling tiling(long long I, int J, long long kb, int npair) {
 // over it by k-blocks alone (parts are then as many as a sum may have terms) is cut into panels of rows, which
 // multiply as fast while a panel fills the SMs, or, where `rows` is false (dW, whose k is long), into groups of parts.
 constexpr long long PART_BYTES = 256 << 20;
-Tiling bounded(long long I, int J, long long kb, int npair, bool rows) {
-    Tiling t = tiling(I, J, kb, npair);
+Tiling bounded(long long I, int J, long long kb, int npair, bool act, bool rows) {
+    Tiling t = tiling(I, J, kb, npair, act);
     const long long row = (long long)t.splits * ((J + 3) & ~3) * 4;  // bytes of one row's parts
     if (t.splits == 1 || row * I <= PART_BYTES) return t;
     if (rows) {
         const long long most = std::max(256LL, PART_BYTES / row / 256 * 256);
         if (most < I) {
-            t = tiling(most, J, kb, npair);
+            t = tiling(most, J, kb, npair, act);
             t.rows = most;
         }
     } else {
@@ -892,14 +898,14 @@ Plan plan(const gs_linear_desc *d, bool bwd) {
     p.o_x = take(p.prep_x ? (size_t)d->M * p.ldx * 2 * p.terms : 0);
     p.o_w = take(p.prep_w ? (size_t)d->N * p.ldw * 2 * p.terms : 0);
     if (!bwd) {
-        p.fwd = bounded(d->M, d->N, cdiv(d->K, BK), f32 ? 6 : 1, true);
+        p.fwd = bounded(d->M, d->N, cdiv(d->K, BK), f32 ? 6 : 1, d->act != GS_ACT_NONE, true);
         p.o_part = take(parts(p.fwd, d->N));
     } else {
         p.need_dz = f32 || d->act != GS_ACT_NONE || ragged(d->ldy, d->unaligned & 4);
         p.dz_terms = f32 ? 3 : d->act != GS_ACT_NONE ? 2 : 1;  // (without an activation dz is dy)
         p.o_dz = take(p.need_dz ? (size_t)d->M * p.ldn * 2 * p.dz_terms : 0);
-        p.gx = bounded(d->M, d->K, cdiv(d->N, BK), f32 ? 6 : p.dz_terms, true);
-        p.gw = bounded(d->N, d->K, cdiv(d->M, BK), f32 ? 6 : p.dz_terms, false);
+        p.gx = bounded(d->M, d->K, cdiv(d->N, BK), f32 ? 6 : p.dz_terms, false, true);
+        p.gw = bounded(d->N, d->K, cdiv(d->M, BK), f32 ? 6 : p.dz_terms, false, false);
         p.o_part = take(std::max(parts(p.gx, d->K), parts(p.gw, d->K)));
         // dz: blocks of 256 threads, up to 256 column vectors each, about four blocks per SM
         const int nv = p.ldn / 8;
