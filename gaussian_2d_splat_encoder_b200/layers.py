@@ -175,6 +175,8 @@ def _norm_backward(ctx, dy):
     need = ctx.needs_input_grad
     x, x_row, x_img = _image_layout(x)
     weight, bias, buf = (t if t is None else t.contiguous() for t in (weight, bias, buf))
+    if buf.data_ptr() & 7:  # (bytes may come back at any address; the statistics are read as pairs of floats)
+        buf = buf.clone()
     dy, dy_row, dy_img = _image_layout(dy)
     desc, _, nbytes, _ = _norm_plan(*ctx.key, x_row, x_img, dy_row, dy_img)
     dx = x.new_empty(x.shape) if need[0] else None

@@ -197,3 +197,16 @@ def test_linear_sizes_take_the_tiles_they_test(lib, ops):
                 assert lib.gs_linear_act_debug_tiles(C.byref(d), product, out) == 0
                 assert (out[0], out[1] > 1) == w, ((M, K, N), product, list(out))
     assert lib.gs_linear_act_debug_tiles(C.byref(d), 3, out) == 2 and lib.gs_linear_act_debug_tiles(C.byref(d), 0, None) == 2
+
+
+def test_norm_statistics_are_read_on_their_alignment(ops):
+    """A hook that keeps tensors in an arena hands the saved bytes back at any address."""
+    def at_odd_address(t):
+        return torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)
+
+    x = torch.randn(2, 5, 32, requires_grad=True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, at_odd_address):
+        y = ops.group_norm_act(x, 4)
+    torch.autograd.grad(y, x, torch.zeros_like(y))
+    (_, _, args) = ops.rec.calls[-1]
+    assert args[0] % 16 == 4 and args[3] % 8 == 0  # x as it came back, the statistics moved
