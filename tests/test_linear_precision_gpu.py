@@ -178,3 +178,44 @@ def test_long_sums_of_one_sign(ops):
                 ref = dy.double() @ w.detach().double()
         inside(y, ref, (half(dtype) + 2112 * U) * ref, (M, K, N))
         del x, w, y, ref
+
+
+@pytest.mark.parametrize("dtype,act", [(torch.bfloat16, "gelu"), (torch.float16, "silu")])
+@pytest.mark.parametrize("N", [4096, 4100])
+def test_16_bit_parts_in_panels(ops, N, dtype, act):
+    """A forward over 16448 terms has two parts, of more rows than the workspace holds at once: two panels, the second
+    short, by whole rows and element by element, with bias, residual and the kept slope."""
+    from layers_util import check_linear
+
+    M, K = 9000, 16448
+    x, w, b = rand(M, K, seed=50, dtype=dtype), rand(N, K, seed=51, dtype=dtype, scale=K ** -0.5), rand(N, seed=52, dtype=dtype)
+    r, dy = rand(M, N, seed=53, dtype=dtype), rand(M, N, seed=54, dtype=dtype)
+    ts = [t.clone().requires_grad_(True) for t in (x, b)]
+    y = ops.linear_act(ts[0], w, ts[1], act=act, residual=r)
+    dx, db = torch.autograd.grad(y, ts, dy)
+    check_linear(y.detach(), (dx, None, db, dy), x, w, b, r, act, dy)
+    Z = (x.double() @ w.double().t() + b.double()).requires_grad_(True)
+    Y = ACTS[act](Z)
+    (dz,) = torch.autograd.grad(Y, Z, dy.double())
+    for name, a, e in (("y", y, Y + r.double()), ("dx", dx, dz @ w.double()), ("db", db, dz.sum(0))):
+        rel = float((a.detach().double() - e.detach()).norm() / e.detach().norm())
+        assert rel <= half(dtype) + 2e-5, (name, rel)
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("act", ["none", "gelu"])
+def test_16_bit_parts_in_groups(ops, act, dtype):
+    """dweight over 70000 rows has five parts of 64 MB, one more than the workspace holds at once."""
+    M, K, N = 70000, 4096, 4096
+    x, w, dy = rand(M, K, seed=55, dtype=dtype), rand(N, K, seed=56, dtype=dtype, scale=K ** -0.5), rand(M, N, seed=57, dtype=dtype)
+    w.requires_grad_(True)
+    (dw,) = torch.autograd.grad(ops.linear_act(x, w, act=act), w, dy)
+    ref = torch.zeros(N, K, dtype=torch.float64, device="cuda")
+    with torch.no_grad():
+        W = w.double()
+        for i in range(0, M, 10000):
+            X, D = x[i:i + 10000].double(), dy[i:i + 10000].double()
+            ref += (D if act == "none" else D * slope64(X @ W.t(), act)).t() @ X
+    rel = float((dw.double() - ref).norm() / ref.norm())
+    assert rel <= half(dtype) + 2e-5, rel
+    torch.cuda.empty_cache()
