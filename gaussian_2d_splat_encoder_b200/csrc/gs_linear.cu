@@ -987,10 +987,14 @@ int check_waits(const char *where) {
 // The driver encodes tensor maps only on a thread with a context.  One that has made no such call yet (a new thread's
 // first linear call, autograd's in a backward that begins with a product) gets its device's here.
 int bind_device(const char *where) {
+    static thread_local int bound = -1;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && dev == bound) return GS_OK;
     if (e == cudaSuccess) e = cudaSetDevice(dev);
-    return e == cudaSuccess ? GS_OK : cuda_error(where, cudaGetErrorString(e));
+    if (e != cudaSuccess) return cuda_error(where, cudaGetErrorString(e));
+    bound = dev;
+    return GS_OK;
 }
 
 template <int BN, bool PAIR, bool OUT32, int EPI, bool LO>

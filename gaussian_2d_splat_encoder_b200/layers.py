@@ -81,6 +81,11 @@ def _elsewhere(dev):
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
+def _in_order(p):
+    """A parameter [C] with its values adjacent and no pending sign."""
+    return (p.resolve_neg() if p.is_neg() else p).contiguous()
+
+
 def _rows_of(t, first):
     """Stride of the flattened axes first..-2 of `t` (whose last axis is adjacent), or None where they do
     not form one axis."""
@@ -108,7 +113,7 @@ def _unpack(ctx):
     backward takes layouts from what it gets here, never from the forward."""
     tensors = ctx.saved_tensors
     for t, kept in zip(tensors, ctx.saved):
-        if t is not None and (t.shape, t.dtype, t.device) != kept:
+        if t is not None and (t.shape != kept[0] or t.dtype is not kept[1] or t.device != kept[2]):
             raise RuntimeError(f"a saved tensor came back as {tuple(t.shape)} {t.dtype} on {t.device}, kept was "
                                f"{tuple(kept[0])} {kept[1]} on {kept[2]}")
     return tensors
@@ -129,7 +134,8 @@ def _norm_plan(B, rows, channels, groups, dtype, param_dtype, act, act_first, ep
 def _image_layout(t):
     """`t` [B, ..., C] with its row and image strides; a copy where the layout has no such strides (or the values
     a pending sign)."""
-    t = t.resolve_neg()
+    if t.is_neg():
+        t = t.resolve_neg()
     if t.is_contiguous():
         C_ = t.shape[-1]
         return t, C_, t.numel() // max(1, t.shape[0])
@@ -239,10 +245,10 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
     grad = x.requires_grad
     if weight is not None:
         _check_param("weight", weight, x, channels)
-        grad, weight = grad or weight.requires_grad, weight.resolve_neg().contiguous()
+        grad, weight = grad or weight.requires_grad, _in_order(weight)
     if bias is not None:
         _check_param("bias", bias, x, channels)
-        grad, bias = grad or bias.requires_grad, bias.resolve_neg().contiguous()
+        grad, bias = grad or bias.requires_grad, _in_order(bias)
         if weight is not None and weight.dtype != bias.dtype:
             raise ValueError(f"weight and bias must be of one type, got {weight.dtype} and {bias.dtype}")
     args = (x, weight, bias, num_groups, float(eps), code, int(bool(act_first)))
@@ -267,7 +273,8 @@ def _linear_plan(M, N, K, dtype, act, ldx, ldw, ldr, ldy, unaligned):
 def _row_layout(t):
     """`t` [..., n] with the stride of its flattened rows, at least n; a copy where there is none (or the values have
     a pending sign)."""
-    t = t.resolve_neg()
+    if t.is_neg():
+        t = t.resolve_neg()
     n = t.shape[-1]
     if t.is_contiguous():
         return t, n
@@ -377,7 +384,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
             if t.dtype != x.dtype:
                 raise ValueError(f"{name} must be {x.dtype} like x, got {t.dtype}")
             grad = grad or t.requires_grad
-    bias = None if bias is None else bias.resolve_neg().contiguous()
+    bias = None if bias is None else _in_order(bias)
     if grad and torch.is_grad_enabled():
         return _LinearAct.apply(x, weight, bias, residual, code)
     return _linear_forward(x, weight, bias, residual, code, False)[0]
