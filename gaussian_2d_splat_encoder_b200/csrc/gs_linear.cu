@@ -11,9 +11,9 @@
 //
 // The forward keeps, for the backward, the activation's slope instead of z: the epilogue has its parts at
 // hand and the backward needs no activation.  It is kept in fp32: in 16 bits either the small slopes of units
-// far below zero or those near one lose bits.  dz enters its
-// products in two terms of the operand type, dz = hi + lo (rounding it once would add as much error as rounding the
-// result does); db sums the unrounded values.
+// far below zero or those near one lose bits.  dz enters its products in two terms of the operand type, dz = hi + lo
+// (rounding it once would add as much error as rounding the result does); db sums the unrounded values.  A training
+// step of 36864x256->1024 bf16 takes 243 us for it (169 with 16-bit slopes and dz in one term).
 //
 // Sums over a long k with few output tiles are split along k over the SMs; the parts go to the workspace
 // in fp32 and a second kernel adds them in order (the same bits every time) and applies the epilogue.  What the
@@ -84,8 +84,10 @@ enum { EPI_NONE = 0, EPI_GELU = 1, EPI_SILU = 2, EPI_GELU_SLOPE = 3, EPI_SILU_SL
 // PAIR: two CTAs share a 256 x 256 tile (cta_group::2): each loads its 128 rows of A and half of B's rows, so an
 // output costs half of the L2 reads and half of the issued MMAs of a 128 x 128 tile (16384x4096->4096 with a
 // residual: 387 us, 1420 TFLOP/s, against 569).  The leader issues all MMAs.
-// Bound by: long sums, the tensor cores and their loads' latency; short ones, the epilogue's instructions (GELU is
-// 11 of some 20 an output; 36864x128->512 takes 23.3 us where its bytes take 7.3).
+// Bound by: long sums, the tensor cores at the clock that the power limit leaves (busy 83 % of the time at 1.5 GHz);
+// short ones, the epilogue's latency: 36864x128->512 with GELU takes 23.3 us where its bytes take 7.3 with half of the
+// issue slots used (20 instructions an output, 11 of them GELU's) and no pipe above 42 %, its warps waiting in turn
+// for accumulators, shared memory and their own chains.
 // Every wait is bounded; one that gives up writes its code to wait_error and raises the CTA's abort flag.
 template <int BN, bool PAIR, bool OUT32, int EPI>
 struct Shape {
@@ -801,12 +803,11 @@ bool valid(const gs_linear_desc *d) {
 // cycles as measured: a k-block 720, 600 and 590 (16384x4096->4096: 387, 569, 1099 us); a tile's epilogue 7100, 2500
 // and 1650 without an activation (36864x256->1024: 35.5, 43.3, 74.7 us), 9900, 3000 and 2050 with one (48.2, 50.6,
 // 81.9 us; 36864x128->512: 25.6, 23.3, 31.5).  A pair's epilogue runs under the next tile's k-blocks; a single
-// CTA's warps come back to the same accumulator, so theirs adds to them.  k splits while SMs are left over and a part keeps
-// at least four k-blocks: their join costs a launch, 5 us of the host's time, and the parts' bytes or, where the
-// output is small, a thread's walk over them (dweight of 100000x64->64: 31.8 us in 148 parts, 22.9 in 74, 26.3 in
-// 37).  Over 12 sizes, their
-// three products, bf16 and fp32, the choice takes at most 1.1 times the best's time but for eight of the smallest (18
-// to 38 us): 1.1 to 1.36.
+// CTA's warps come back to the same accumulator, so theirs adds to them.  k splits while SMs are left over and a part
+// keeps at least four k-blocks: their join costs a launch, 5 us of the host's time, and the parts' bytes or, where
+// the output is small, a thread's walk over them (dweight of 100000x64->64: 31.8 us in 148 parts, 22.9 in 74, 26.3
+// in 37).  Over 12 sizes, their three products, bf16 and fp32, the choice takes at most 1.1 times the best's time but
+// for nine of the smallest (15 to 38 us): 1.1 to 1.36.
 //
 // A part has at most so many k-blocks as its type allows, because the accumulators cut what they add up rather than
 // round it: by 1.7e-6 of the result over 1536 terms, 7e-4 over 131072 of one sign, 6e-3 over 2^20; the join rounds.

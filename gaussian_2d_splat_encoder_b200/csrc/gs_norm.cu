@@ -14,15 +14,17 @@
 // SM, so each direction is two launches over the same slices, the second of which finds what L2 (126 MB)
 // still holds.  A block takes a run of rows of one image (and, where there are many groups, a chunk of
 // whole groups); a thread keeps one 16-byte vector of channels for all its rows, so parameters and sums stay
-// in registers and a warp reads contiguous memory.  A forward whose image and group chunk fit the registers
-// of a cluster is one launch: values are read once, the cluster joins its sums over distributed shared
-// memory.  Statistics are taken around means, never as a difference of large squares: four rows at a time
+// in registers and a warp reads contiguous memory.  A forward whose image and group chunk fit the shared
+// memory of a cluster's CTAs is one launch: values are read once, the cluster joins its sums over distributed
+// shared memory.  Statistics are taken around means, never as a difference of large squares: two rows at a time
 // exactly around their own mean, joined as (n, mean, M2).  All sums run in a fixed order.
 //
-// With an activation the FMA and MUFU pipes bind as much as memory does (GELU: 0.125 cycles of an SM per
-// element and evaluation), so each launch evaluates it once per element.  Measured: 4x384x384x64 bf16 with SiLU
-// 44 us (statistics 20, map 24; its bytes take 23), a training step of 4x192x192x128 with GELU first 79 us (19, 18,
-// 21, 26; bytes 23), 96x96x256 in one launch 13.4 us against 27 in two.
+// Each launch evaluates an activation once per element (GELU: 0.125 cycles of an SM's MUFU).  Measured: 4x384x384x64
+// bf16 with SiLU 44 us (its bytes take 23): statistics 18 to 20, x at half of memory's rate, its warps waiting for
+// loads; the map 24, MUFU busy 61 to 68 % of the time, warps queued before it and shared memory.  A training step of
+// 4x192x192x128 with GELU first 79 us (19, 18, 21, 26; bytes 23): issue slots 56 to 62 %, MUFU 36 to 56 %, FMA 46 to 52 %,
+// memory 21 to 39 %, so no unit is full: latency, with three to five warps a scheduler.  96x96x256 in one launch 13.4 us
+// against 27 in two.
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include <stdio.h>
@@ -788,7 +790,9 @@ bool plan(const gs_norm_desc *d, NormArgs &a) {
     // the second launch joins only those groups' sums
     chunks(a, a.G > 32 ? 64 : a.C);
     a.rl = std::max(1, MAX_T / a.cvec);
-    // one wave of three blocks per SM, but no fewer than four rows a thread
+    // Three blocks per SM, but no fewer than four rows a thread: one wave of the launches that hold three an SM, one
+    // and a half of the others (statistics off eight channels a group, the backward's map).  444, 296 and 592
+    // slices: 4x384x384x64 44, 52.5, 45.9 us, the training step of 4x192x192x128 78.5, 81.3, 87.4.
     const long long most = std::max<long long>(1, a.rows / (4LL * a.rl));
     const long long want = std::max<long long>(1, 3LL * SMS / std::max<long long>(1, (long long)a.B * a.nchunk));
     split(a, (int)std::min(most, want));

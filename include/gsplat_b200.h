@@ -267,7 +267,8 @@ typedef struct {
 } gs_norm_desc;
 
 /* Workspace bytes of a forward (backward = 0) or a backward (1) call; 0 for an invalid descriptor.  The
- * two calls share nothing through it. */
+ * two calls share nothing through it.  A backward keeps 8 bytes a channel for every slice of an image (one to 444
+ * slices an image, about 444 in all where there are fewer images). */
 size_t gs_group_norm_act_workspace_size(const gs_norm_desc *d, int backward);
 /* y [B][rows][C], tightly packed; stats (may be NULL without a backward) receives fp32 [B][groups][2]:
  * mean and 1 / sqrt(var + eps).  weight and bias [C] may be NULL (1 and 0). */
