@@ -64,7 +64,8 @@ struct GemmArgs {
 
 // term products, small ones first: (a term, b term), 0 = high; the six of fp32, then the two of A in two terms
 // fp16 has no exponents below its subnormals: lo is kept times 2^LO_BITS (at most 2^4 2^11 for the largest dz) and
-// its sum scaled back when the products with hi begin.
+// its sum scaled back when the products with hi begin.  Nor above 65504, which dz passes by the slope's 1.13: both terms
+// are of dz / 2, and the epilogue doubles the sum.
 constexpr int LO_BITS = 11;
 __constant__ const unsigned char PAIR_A[8] = {2, 0, 1, 1, 0, 0, 1, 0}, PAIR_B[8] = {0, 2, 1, 0, 1, 0, 0, 0};
 
@@ -129,7 +130,7 @@ struct Item {
     __device__ __forceinline__ int blocks(const GemmArgs &a) const { return (to(a) - from(a)) * a.npair; }
 };
 
-template <int BN, bool PAIR, bool OUT32, int EPI>
+template <int BN, bool PAIR, bool OUT32, int EPI, bool LO>
 __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ring_end, const CUtensorMap *tmO,
                                          const CUtensorMap *tmS, const CUtensorMap *tmR, int first, int stride, int n_items,
                                          int rank) {
@@ -251,6 +252,9 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, Pipe &p, uint8_t *ri
                         v[2 * i + 1] = add2({__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3])}, {f.z, f.w});
                     }
                 }
+                if (LO && live && !dead)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[i] = add2(v[i], v[i]);
                 if (u == S::UNITS - 1 && h == EC / 16 - 1) {  // this warp's part of the accumulator is drained
                     tc_fence_before();
                     __syncwarp();
@@ -495,7 +499,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
             mbar_wait(&p.mdone, 0, a.wait_error, 4);
         }
     } else {
-        epilogue<BN, PAIR, OUT32, EPI>(a, p, smem + STAGES * S::STAGE, &tmO, &tmS, &tmR, first, stride, n_items, rank);
+        epilogue<BN, PAIR, OUT32, EPI, LO>(a, p, smem + STAGES * S::STAGE, &tmO, &tmS, &tmR, first, stride, n_items, rank);
     }
 
     tc_fence_before();
@@ -631,6 +635,10 @@ __global__ void __launch_bounds__(256) k_dz(const __grid_constant__ DzArgs a) {
             if (sizeof(T) == 4)
                 store_terms(v, reinterpret_cast<__nv_bfloat16 *>(a.dz) + m * a.ldp + c, a.M * a.ldp);
             else {
+                constexpr bool HALF = std::is_same_v<T, __half>;
+                if (HALF && a.terms == 2)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) v[i] = mul2(v[i], both(0.5f));
                 Raw8<T> *to = reinterpret_cast<Raw8<T> *>(reinterpret_cast<T *>(a.dz) + m * a.ldp + c);
                 const Raw8<T> high = pack8<T>(v);
                 *to = high;
@@ -639,7 +647,7 @@ __global__ void __launch_bounds__(256) k_dz(const __grid_constant__ DzArgs a) {
                     unpack8<T>(high, h);
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        constexpr float scale = std::is_same_v<T, __half> ? (float)(1 << LO_BITS) : 1.f;
+                        constexpr float scale = HALF ? (float)(1 << LO_BITS) : 1.f;
                         at(v, i) = fabsf(at(h, i)) <= 3.4028234e38f ? (at(v, i) - at(h, i)) * scale : 0.f;
                     }
                     *reinterpret_cast<Raw8<T> *>(reinterpret_cast<T *>(to) + a.M * a.ldp) = pack8<T>(v);

@@ -9,9 +9,11 @@ or projection that is trained needs the same pieces one by one, differentiable, 
   ``splat_features`` or ``gather_splat_latents`` and the layers of a residual block
 
 Both take fp32, bf16 or fp16 CUDA tensors, keep every sum and statistic in fp32, round once to the tensor's
-type and give the same bits for the same inputs.  They run on the current stream of the tensors' device
-and can be captured into a CUDA graph.  The gradients are once differentiable, in reverse mode
-alone: dual tensors and the transforms of torch.func are refused.
+type and give the same bits for the same inputs; activations and their slopes are within 7e-7 (1 + |z|) of the
+exact ones.  They run on the current stream of the tensors' device and can be captured into a CUDA graph (a
+training step with ``torch.autograd.grad``, once eager graphs of the same leaves are gone, as torch asks).  The
+gradients are once differentiable, in reverse mode alone: dual tensors and the transforms of torch.func are
+refused.
 
 The waits inside linear_act's kernels are bounded.  One that gives up leaves that call's outputs invalid; calls are
 asynchronous, so the next call of linear_act (or its backward) raises RuntimeError, or ``check_linear_waits()``, which
@@ -361,7 +363,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
 
     x [..., K], weight [N, K] (nn.Linear's, or a 1x1 convolution's ``weight.flatten(1)``), bias [N],
     residual [..., N] of the output's shape; all of one type, float32, bfloat16 or float16.  ``act`` is
-    "none", "gelu" (erf form) or "silu".  Sums are fp32 (fp32 inputs keep fp32 accuracy); the result is
+    "none", "gelu" (erf form) or "silu".  Sums are fp32 (fp32 inputs of 1e-34 and more keep fp32 accuracy); the result is
     rounded once, after the residual, and each gradient once.  Infinities come out as the formula has them but for
     two cases that give NaN: fp32 infinities of both factors that meet, and 16-bit ones of x or weight in a gradient.  Rows may be strided (channel slices of a wider map); other strides are
     copied.  Returns a contiguous tensor [..., N]."""

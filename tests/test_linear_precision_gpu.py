@@ -219,3 +219,28 @@ def test_16_bit_parts_in_groups(ops, act, dtype):
     rel = float((dw.double() - ref).norm() / ref.norm())
     assert rel <= half(dtype) + 2e-5, rel
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("M,K,N", [(300, 24, 40), (4000, 256, 1030)])
+def test_fp16_dz_beyond_its_range(ops, M, K, N):
+    """Gradients near fp16's largest number times a slope of up to 1.13 pass it; dx and dweight, whose factors are small,
+    do not."""
+    dtype, h = torch.float16, half(torch.float16)
+    x, w = few_bits(M, K, seed=60, dtype=dtype, scale=2.0 ** -6), few_bits(N, K, seed=61, dtype=dtype, scale=2.0 ** -6)
+    b = torch.full((N,), 1.5, dtype=dtype, device="cuda")
+    dy = (65504 - 4096 * rand(M, N, seed=62).abs()).to(dtype) * torch.where(rand(M, N, seed=63) > 0, 1.0, -1.0).to(dtype)
+    ts = [t.clone().requires_grad_(True) for t in (x, w)]
+    dx, dw = torch.autograd.grad(ops.linear_act(ts[0], ts[1], b, act="gelu"), ts, dy)
+    X, W, D = x.double(), w.double(), dy.double()
+    z = X @ W.t() + b.double()
+    dz = D * slope64(z, "gelu")
+    assert bool((dz.abs() > 65504).any())
+    edz = ACT_U * U * (1 + z.abs()) * D.abs() + (U + h * h) * dz.abs()
+    sums = [2 * U * (n / 2 + 32) for n in (N, M)]
+    for got, ref, bound, what in ((dx, dz @ W, (edz + sums[0] * dz.abs()) @ W.abs(), "dx"),
+                                  (dw, dz.t() @ X, (edz + sums[1] * dz.abs()).t() @ X.abs(), "dweight")):
+        # long sums pass fp16's range themselves here and there (4000 terms of some 7e4 2^-7: 4e4 in the mean, one in
+        # eight beyond 65520, from where on their rounding is infinite)
+        over = (ref.abs() + bound >= 65504) & got.isinf()
+        assert torch.equal(got[over].sign().double(), ref[over].sign()) and over.float().mean() < 0.25
+        inside(torch.where(over, 0, got), torch.where(over, 0, ref), h * ref.abs() + bound + least(dtype), what)
